@@ -255,12 +255,21 @@ def _scalars(step):
     return 1.0 - LR * DECAY, LR / (1.0 - BETAS[0] ** step), 1.0 / math.sqrt(1.0 - BETAS[1] ** step)
 
 
+def _optimizer(state, bits, **moments):
+    """The optimizer that a program keeps, made at the first pass, with the moments that it has by then."""
+    if "optimizer" not in state:
+        from virconv_amd import optim
+        state["optimizer"] = optim.AdamW(state["params"], lr=LR, betas=BETAS, eps=EPS_ADAM, weight_decay=DECAY, state_bits=bits, seed=SEED)
+        for k, (p, g) in enumerate(zip(state["params"], state["grads"])):
+            p.grad = g
+            state["optimizer"].state[p].update(step=state["step"] - 1, **{name: t[k] for name, t in moments.items()})
+    return state["optimizer"]
+
+
 def _adamw_32(state):
     flat = state["flat"]
     if own:
-        from virconv_amd import optim
-        optim.adamw_step(state["params"], state["grads"], state["exp_avgs"], state["exp_avg_sqs"], step=state["step"], lr=LR, betas=BETAS,
-                         eps=EPS_ADAM, weight_decay=DECAY)
+        _optimizer(state, 32, exp_avg=state["exp_avgs"], exp_avg_sq=state["exp_avg_sqs"]).step()
         return flat
     keep, size, scale = _scalars(state["step"])
     g = state["flat_grads"].float()
@@ -307,9 +316,7 @@ def _encode(x, top, bits):
 def _adamw_8(state):
     flat = state["flat"]
     if own:
-        from virconv_amd import optim
-        optim.adamw_step_8bit(state["params"], state["grads"], state["exp_avgs"], state["exp_avg_rmss"], state["exponents"], step=state["step"],
-                              lr=LR, betas=BETAS, eps=EPS_ADAM, weight_decay=DECAY, seed=SEED)
+        _optimizer(state, 8, exp_avg=state["exp_avgs"], exp_avg_rms=state["exp_avg_rmss"], exponents=state["exponents"]).step()
         return flat
     keep, size, scale = _scalars(state["step"])
     p, g, m, r = (t.view(-1, BLOCK).float() for t in (flat["params"], state["flat_grads"], flat["exp_avgs"], flat["exp_avg_rmss"]))
