@@ -55,8 +55,8 @@ typedef enum vc_operand {
 const char* vc_version(void);
 /* Layout version of the structs that cross this boundary (vc_plan_desc, vc_pass_program, vc_trace_record, ...).  A binding compares
  * vc_abi_version() with the VC_ABI_VERSION it was written against before it fills any of them: a field added to a struct (round 5:
- * vc_pass_program.pack_all; round 6: vc_plan_desc.allow_unfenced_projection, vc_adam_tensor) otherwise reads as a silent zero on the other side. */
-#define VC_ABI_VERSION 7
+ * vc_pass_program.pack_all; round 6: vc_plan_desc.allow_unfenced_projection, vc_adam_tensor; then vc_adamw_tensor) otherwise reads as a silent zero on the other side. */
+#define VC_ABI_VERSION 8
 int vc_abi_version(void);
 const char* vc_last_error(void);
 /* developer switch for A/B measurements (tools/kbench.py): "conv_variant" = 1 | 2 */
@@ -277,6 +277,63 @@ typedef struct vc_adam_tensor {
 size_t vc_clip_adamw_workspace_bytes(int n_tensors);
 int vc_clip_adamw(const vc_adam_tensor* tensors, int n_tensors, float lr, float beta1, float beta2, float eps, float weight_decay,
                   int64_t step, float max_norm, int scale_grads, float* total_norm, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------------ row operators of a training step
+ * Layer norm, products grouped by ragged row segments, and AdamW over many tensors: what a network of row-wise layers around the sparse
+ * convolutions trains with.  Their tensors may be fp32, fp16 or bf16; everything is computed in fp32 and rounded once per output.          */
+typedef enum vc_dtype { VC_F32 = 0, VC_F16 = 1, VC_BF16 = 2 } vc_dtype;
+
+/* Layer norm of n rows of c elements: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps), var the mean square of x - mean.
+ * x: row r at x + r * x_stride (elements, >= c), y: (n, c) dense.  weight / bias: c elements of weight_dtype / bias_dtype (the tensors'
+ * type or VC_F32), or NULL (1 / 0).  mean, rstd: n floats each for the backward pass, or both NULL.                                        */
+int vc_layer_norm_forward(const void* x, int64_t x_stride, int64_t n, int64_t c, int dtype, const void* weight, int weight_dtype,
+                          const void* bias, int bias_dtype, float eps, void* y, float* mean, float* rstd, void* stream);
+/* dx = rstd * (g - mean(g) - xh * mean(g * xh)) with g = dy * weight, xh = (x - mean) * rstd; dweight = sum over the rows of dy * xh, dbias
+ * = sum over the rows of dy, in weight_dtype / bias_dtype.  dx, dweight, dbias: any may be NULL (not wanted).  n = 0: the sums are zeros.
+ * workspace: vc_layer_norm_backward_workspace_bytes, needed when dweight or dbias is wanted; no state in it.  Fixed order of additions.    */
+size_t vc_layer_norm_backward_workspace_bytes(int64_t n, int64_t c, int dtype);
+int vc_layer_norm_backward(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, int64_t n, int64_t c, int dtype,
+                           const void* weight, int weight_dtype, int bias_dtype, const float* mean, const float* rstd, void* dx, void* dweight,
+                           void* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Products of row groups with one weight matrix each.  Group g: rows [offsets[g], offsets[g + 1]) of x (offsets: groups + 1 rising int32 or
+ * int64 values ON THE DEVICE; values are cut to a rising sequence within [0, rows]); weight (groups, out, in), bias (groups, out) or NULL.
+ *   forward          y_r  = weight[g] x_r + bias[g]
+ *   backward_input   dx_r = weight[g]^T dy_r
+ *   backward_weight  dweight[g] = sum of dy_r x_r^T, dbias[g] = sum of dy_r (dbias NULL: not wanted); zeros for a group without rows
+ * Rows of no group come out as zeros and add to no gradient.  All tensors of one dtype; VC_F32 products are accurate to 2^-23 of each product
+ * (operands cut exactly into three bf16 pieces; an infinite operand gives NaN).  x_stride, dy_stride: elements from row to row.
+ * direction: 0 forward, 1 backward_input, 2 backward_weight.                                                                                */
+size_t vc_grouped_linear_workspace_bytes(int direction, int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype);
+int vc_grouped_linear_forward(const void* x, int64_t x_stride, int64_t rows, const void* weight, const void* bias, const void* offsets,
+                              int offset_bits, int64_t groups, int64_t in, int64_t out, int dtype, void* y, void* workspace,
+                              size_t workspace_bytes, void* stream);
+int vc_grouped_linear_backward_input(const void* dy, int64_t dy_stride, int64_t rows, const void* weight, const void* offsets, int offset_bits,
+                                     int64_t groups, int64_t in, int64_t out, int dtype, void* dx, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, int64_t rows, const void* offsets,
+                                      int offset_bits, int64_t groups, int64_t in, int64_t out, int dtype, void* dweight, void* dbias,
+                                      void* workspace, size_t workspace_bytes, void* stream);
+
+/* One AdamW step of any number of tensors (vc_clip_adamw's arithmetic without the clip; host array of descriptors, device pointers in it):
+ *     m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^step) * m / (sqrt(v) / sqrt(1 - b2^step) + eps)
+ * dtype: of the parameters and gradients.  state_bits 32: exp_avg = m and exp_avg_sq = v are fp32.  state_bits 8: exp_avg = m and
+ * exp_avg_sq = sqrt(v) are OCP e4m3 values over a power of two for every 128 elements: value * 2^(exponent - 7), exponents: (blocks, 2) int8
+ * [of m, of sqrt(v)], blocks = ceil(n / 128).  A value is rounded to one of its two e4m3 neighbours with the probability of its distance
+ * from the other: 16 bits of M(M(M(M(seed) + step) + key) ^ element), M the finalizer of MurmurHash3; the low half for m.  All-zero codes
+ * and exponents are the state before step 1.  Descriptors with n = 0 are skipped.  Written memory must not overlap (checked).             */
+typedef struct vc_adamw_tensor {
+  void* param;         /* n elements of dtype, updated in place */
+  const void* grad;    /* n elements of dtype */
+  void* exp_avg;       /* n floats, or n e4m3 codes */
+  void* exp_avg_sq;    /* n floats, or n e4m3 codes of the square root */
+  int8_t* exponents;   /* 8-bit states */
+  int64_t n;
+  uint32_t key;        /* the tensor's place in the model: tells its random numbers from another tensor's */
+  int32_t vec_;        /* not read */
+} vc_adamw_tensor;
+int vc_adamw(const vc_adamw_tensor* tensors, int64_t n_tensors, int dtype, int state_bits, double lr, double beta1, double beta2, double eps,
+             double weight_decay, int64_t step, uint32_t seed, void* stream);
 
 /* ------------------------------------------------------------------------------------------------ K9 projection
  * Voxel index -> image pixel index.  Replaces index2points + index2uv +

@@ -12,7 +12,7 @@ import ctypes as C
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
-ABI_VERSION = 7     # = VC_ABI_VERSION of include/virconv_hip.h (struct layouts this file mirrors)
+ABI_VERSION = 8     # = VC_ABI_VERSION of include/virconv_hip.h (struct layouts this file mirrors)
 LIB_PATH = os.environ.get("VIRCONV_LIB", os.path.join(_HERE, "libvirconv_hip.so"))  # override: A/B builds only
 
 OPERAND_TYPES = {"f32": 0, "f16": 1, "bf16": 2}  # vc_operand (include/virconv_hip.h)
@@ -34,6 +34,14 @@ SIGNATURES = {
     "vc_weighted_sum_backward": (_I, [_P, _P, _I64, _I64, _P, _P]),
     "vc_clip_adamw_workspace_bytes": (_SZ, [_I]),
     "vc_clip_adamw": (_I, [_P, _I, _F, _F, _F, _F, _F, _I64, _F, _I, _P, _P, _SZ, _P]),
+    "vc_layer_norm_forward": (_I, [_P, _I64, _I64, _I64, _I, _P, _I, _P, _I, _F, _P, _P, _P, _P]),
+    "vc_layer_norm_backward_workspace_bytes": (_SZ, [_I64, _I64, _I]),
+    "vc_layer_norm_backward": (_I, [_P, _I64, _P, _I64, _I64, _I64, _I, _P, _I, _I, _P, _P, _P, _P, _P, _P, _SZ, _P]),
+    "vc_grouped_linear_workspace_bytes": (_SZ, [_I, _I64, _I64, _I64, _I64, _I]),
+    "vc_grouped_linear_forward": (_I, [_P, _I64, _I64, _P, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _SZ, _P]),
+    "vc_grouped_linear_backward_input": (_I, [_P, _I64, _I64, _P, _P, _I, _I64, _I64, _I64, _I, _P, _P, _SZ, _P]),
+    "vc_grouped_linear_backward_weight": (_I, [_P, _I64, _P, _I64, _I64, _P, _I, _I64, _I64, _I64, _I, _P, _P, _P, _SZ, _P]),
+    "vc_adamw": (_I, [_P, _I64, _I, _I, _D, _D, _D, _D, _D, _I64, C.c_uint32, _P]),
     "vc_hash_workspace_bytes": (_SZ, [_I64]),
     "vc_hash_build": (_I, [_P, _I64, _I, _P, _P, _SZ, _P]),
     "vc_subm_rulebook": (_I, [_P, _I64, _I, _P, _P, _P, _P, _SZ, _P, _P, _P]),

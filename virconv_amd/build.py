@@ -16,6 +16,9 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libvirconv_hip.so")
 ARCH = "gfx950"
 
+# no packed fp32 instructions (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32): some of their forms have given wrong results on MI355X now and then
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
 # per-source extra flags: the index kernels must not contract mul+add (bit-exact integer outputs vs the oracle)
 SOURCES = {
     "index_kernels.hip": ["-ffp-contract=off"],
@@ -31,6 +34,10 @@ SOURCES = {
     "nms_kernels.hip": ["-ffp-contract=off"],
     "group_kernels.hip": [],
     "optim_kernels.hip": [],
+    # the AdamW step is defined operation by operation (8-bit states: bit-equal to the same operations of torch), so nothing is contracted
+    "adamw_kernels.hip": ["-ffp-contract=off", *NO_PACKED_FP32],
+    "norm_kernels.hip": [*NO_PACKED_FP32],
+    "grouped_kernels.hip": [*NO_PACKED_FP32],
     "unit.hip": [],
     "pass.hip": [],
     "plan.hip": [],

@@ -1,0 +1,313 @@
+// AdamW over many tensors at once, with the two moments in 32 or in 8 bits.
+//
+//   m = b1 m + (1 - b1) g;  v = b2 v + (1 - b2) g^2;  p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// in fp32 whatever the parameters' type, every operation rounded by itself (this file is built without contraction), the parameter rounded
+// once to its own type.  The step is one pass over its data and nothing else: what bounds it is HBM -- 28 bytes an element with fp32
+// parameters and 32-bit moments, 16 with 8-bit ones, 10 with bf16 parameters and 8-bit moments.
+//
+// 8-bit moments.  m and r = sqrt(v) are held as e4m3 values over a power of two per 128 elements: value * 2^(exponent - 7), the block's
+// largest magnitude lying in [128, 256) before the power is taken off.  r and not v: the root halves the range that a block has to span.
+// A power of two and not the largest magnitude itself: when a block's exponent moves, values that lie on the grid stay on it.  The grid's
+// steps (6 to 12 per cent of a value) are far wider than what one step changes of a moment (1 - b2 = 1 per cent of v), so rounding to the
+// nearest value would leave a moment where it is for good; it is rounded up with the probability of its distance from the lower
+// neighbour instead, which keeps every moment's mean.  The random numbers are a function of (seed, step, tensor, element), so a run can be
+// repeated, and resumed, bit for bit.  An infinite or undefined moment is held as NaN; it does not take part in its block's exponent.
+#include "common.h"
+
+#include <math.h>
+
+#include <algorithm>
+#include <vector>
+
+namespace vc {
+
+static constexpr int kAdamwTensors = 48;    // per launch: the table travels in the kernel's arguments (48 x 56 + 49 x 4 bytes < 4 KB)
+static constexpr int kAdamwChunk = 2048;    // elements of one block: 256 threads x 8
+static constexpr int kStateBlock = 128;     // elements that share an exponent: 16 lanes x 8
+
+struct AdamwTable {
+  vc_adamw_tensor t[kAdamwTensors];
+  unsigned block0[kAdamwTensors + 1];
+  int n;
+};
+
+struct AdamwArgs {
+  float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, keep, step_size, inv_bc2_sqrt;
+};
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+  static __device__ __forceinline__ float up(float x) { return x; }
+  static __device__ __forceinline__ float down(float x) { return x; }
+};
+template <> struct Elem<_Float16> {
+  static __device__ __forceinline__ float up(_Float16 x) { return (float)x; }
+  static __device__ __forceinline__ _Float16 down(float x) { return (_Float16)x; }
+};
+template <> struct Elem<__bf16> {
+  static __device__ __forceinline__ float up(__bf16 x) { return (float)x; }
+  static __device__ __forceinline__ __bf16 down(float x) { return (__bf16)x; }
+};
+
+// eight consecutive elements: one 16- or two 16-byte accesses where the tensor's pointers allow it
+template <typename T> struct alignas(sizeof(T) * 8 < 16 ? sizeof(T) * 8 : 16) Eight { T v[8]; };
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int64_t i, int64_t n, bool vec, float (&out)[8]) {
+  if (vec && i + 8 <= n) {
+    const Eight<T> e = *reinterpret_cast<const Eight<T>*>(p + i);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) out[k] = Elem<T>::up(e.v[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) out[k] = i + k < n ? Elem<T>::up(p[i + k]) : 0.f;
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, int64_t i, int64_t n, bool vec, const float (&x)[8]) {
+  if (vec && i + 8 <= n) {
+    Eight<T> e;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e.v[k] = Elem<T>::down(x[k]);
+    *reinterpret_cast<Eight<T>*>(p + i) = e;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i + k < n) p[i + k] = Elem<T>::down(x[k]);
+  }
+}
+
+__device__ __forceinline__ int adamw_find(const AdamwTable& B) {
+  // the last tensor that begins at or before this block: one lane a tensor
+  const int lane = threadIdx.x & 63;
+  const unsigned b0 = lane < B.n ? B.block0[lane] : 0xffffffffu;
+  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(b0 <= blockIdx.x)) - 1);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) adamw32_kernel(AdamwTable B, AdamwArgs a) {
+  const int s = adamw_find(B);
+  const vc_adamw_tensor& S = B.t[s];
+  const int64_t n = S.n, i = (int64_t)(blockIdx.x - B.block0[s]) * kAdamwChunk + threadIdx.x * 8;
+  if (i >= n) return;
+  const bool vec = S.vec_;
+  float p[8], g[8], m[8], v[8];
+  load8((const T*)S.grad, i, n, vec, g);
+  load8((const float*)S.exp_avg, i, n, vec, m);
+  load8((const float*)S.exp_avg_sq, i, n, vec, v);
+  load8((const T*)S.param, i, n, vec, p);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    m[k] = m[k] * a.beta1 + g[k] * a.one_minus_beta1;
+    v[k] = v[k] * a.beta2 + g[k] * g[k] * a.one_minus_beta2;
+    p[k] = p[k] * a.keep - a.step_size * (m[k] / (sqrtf(v[k]) * a.inv_bc2_sqrt + a.eps));
+  }
+  store8((float*)S.exp_avg, i, n, vec, m);
+  store8((float*)S.exp_avg_sq, i, n, vec, v);
+  store8((T*)S.param, i, n, vec, p);
+}
+
+__device__ __forceinline__ uint32_t mix32(uint32_t x) {   // the finalizer of MurmurHash3
+  x ^= x >> 16; x *= 0x85ebca6bu; x ^= x >> 13; x *= 0xc2b2ae35u; x ^= x >> 16;
+  return x;
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_rotated(uint32_t x) {
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ uint32_t max16(uint32_t x) {   // over the 16 lanes of a row, in every lane: rotations by 8, 4, 2, 1
+  x = max_rotated<0x128>(x); x = max_rotated<0x124>(x); x = max_rotated<0x122>(x); x = max_rotated<0x121>(x);
+  return x;
+}
+
+__device__ __forceinline__ void decode8(const void* codes, int64_t i, int64_t n, bool vec, int exponent, float (&out)[8]) {
+  const uint8_t* c = (const uint8_t*)codes;
+  uint32_t w[2] = {0, 0};
+  if (vec && i + 8 <= n) {
+    const uint2 e = *reinterpret_cast<const uint2*>(c + i);
+    w[0] = e.x; w[1] = e.y;
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i + k < n) w[k >> 2] |= (uint32_t)c[i + k] << (8 * (k & 3));
+  }
+  const float unit = __uint_as_float((uint32_t)(max(exponent, -119) + 120) << 23);   // 2^(exponent - 7)
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    out[4 * h + 0] = __builtin_amdgcn_cvt_f32_fp8(w[h], 0) * unit;
+    out[4 * h + 1] = __builtin_amdgcn_cvt_f32_fp8(w[h], 1) * unit;
+    out[4 * h + 2] = __builtin_amdgcn_cvt_f32_fp8(w[h], 2) * unit;
+    out[4 * h + 3] = __builtin_amdgcn_cvt_f32_fp8(w[h], 3) * unit;
+  }
+}
+
+// the magnitude's bits where it is finite, 0 otherwise: what the block's exponent is taken from
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
+  return b < 0x7f800000u ? b : 0u;
+}
+
+// one value onto the e4m3 grid: up with the probability of its distance from the lower neighbour (`r20`: 20 random bits).  Below 2^-6 the
+// grid's step is 2^-9, as in the binade above: there 2^-6 is added before and taken off after.
+__device__ __forceinline__ float round_e4m3(float x, float scale, uint32_t r20) {
+  const float y = fabsf(x) * scale;
+  const float low = y < 0x1p-6f ? 0x1p-6f : 0.f;
+  float z = __uint_as_float((__float_as_uint(y + low) + r20) & 0xfff00000u) - low;
+  z = y < 256.f ? z : __uint_as_float(0x7fc00000u);
+  return copysignf(z, x);
+}
+
+__device__ __forceinline__ void encode8(void* codes, int64_t i, int64_t n, bool vec, int exponent, const float (&x)[8], const uint32_t (&r20)[8]) {
+  const float scale = __uint_as_float((uint32_t)(134 - exponent) << 23);   // 2^(7 - exponent)
+  uint32_t w[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float z[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) z[k] = round_e4m3(x[4 * h + k], scale, r20[4 * h + k]);
+    int c = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
+    w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], c, true);
+  }
+  uint8_t* c = (uint8_t*)codes;
+  if (vec && i + 8 <= n) {
+    *reinterpret_cast<uint2*>(c + i) = make_uint2(w[0], w[1]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i + k < n) c[i + k] = (uint8_t)(w[k >> 2] >> (8 * (k & 3)));
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable B, AdamwArgs a) {
+  const int s = adamw_find(B);
+  const vc_adamw_tensor& S = B.t[s];
+  const int64_t n = S.n, i = (int64_t)(blockIdx.x - B.block0[s]) * kAdamwChunk + threadIdx.x * 8;
+  // 16 lanes share an exponent, and all 16 are here for the maximum: the lanes behind the last element carry zeros
+  const bool vec = S.vec_;
+  const int64_t blk = i / kStateBlock;
+  const bool live = blk * kStateBlock < n;
+  const int8_t* e = S.exponents + 2 * blk;
+  float p[8], g[8], m[8], r[8];
+  load8((const T*)S.grad, i, n, vec, g);
+  load8((const T*)S.param, i, n, vec, p);
+  decode8(S.exp_avg, i, n, vec, live ? e[0] : 0, m);
+  decode8(S.exp_avg_sq, i, n, vec, live ? e[1] : 0, r);
+  uint32_t mtop = 0, rtop = 0, random[8], r20[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    m[k] = m[k] * a.beta1 + g[k] * a.one_minus_beta1;
+    const float v = r[k] * r[k] * a.beta2 + g[k] * g[k] * a.one_minus_beta2;
+    r[k] = sqrtf(v);
+    p[k] = p[k] * a.keep - a.step_size * (m[k] / (r[k] * a.inv_bc2_sqrt + a.eps));
+    mtop = max(mtop, finite_bits(m[k]));
+    rtop = max(rtop, finite_bits(r[k]));
+    const uint64_t at = (uint64_t)(i + k);
+    random[k] = mix32(S.key ^ (uint32_t)at ^ (uint32_t)(at >> 32) * 0x9e3779b9u);
+  }
+  store8((T*)S.param, i, n, vec, p);
+  const int em = max((int)(max16(mtop) >> 23) - 127, -119), er = max((int)(max16(rtop) >> 23) - 127, -119);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) r20[k] = (random[k] & 0xffffu) << 4;
+  encode8(S.exp_avg, i, n, vec, em, m, r20);
+#pragma unroll
+  for (int k = 0; k < 8; ++k) r20[k] = (random[k] >> 16) << 4;
+  encode8(S.exp_avg_sq, i, n, vec, er, r, r20);
+  if (live && (threadIdx.x & 15) == 0) {
+    S.exponents[2 * blk] = (int8_t)em;
+    S.exponents[2 * blk + 1] = (int8_t)er;
+  }
+}
+
+static uint32_t host_mix32(uint32_t x) {
+  x ^= x >> 16; x *= 0x85ebca6bu; x ^= x >> 13; x *= 0xc2b2ae35u; x ^= x >> 16;
+  return x;
+}
+
+struct Span {
+  uintptr_t a, b;
+  bool operator<(const Span& o) const { return a < o.a; }
+};
+
+}  // namespace vc
+
+using namespace vc;
+
+extern "C" {
+
+int vc_adamw(const vc_adamw_tensor* tensors, int64_t n_tensors, int dtype, int state_bits, double lr, double beta1, double beta2, double eps,
+             double weight_decay, int64_t step, uint32_t seed, void* stream) {
+  VC_REQUIRE(n_tensors >= 0 && (n_tensors == 0 || tensors), "vc_adamw: %lld tensors at %p", (long long)n_tensors, (const void*)tensors);
+  VC_REQUIRE(dtype == VC_F32 || dtype == VC_F16 || dtype == VC_BF16, "vc_adamw: unknown dtype %d", dtype);
+  VC_REQUIRE(state_bits == 8 || state_bits == 32, "vc_adamw: states in %d bits (8 or 32)", state_bits);
+  VC_REQUIRE(step >= 1, "vc_adamw: step = %lld (the first step is 1)", (long long)step);
+  VC_REQUIRE(beta1 >= 0. && beta1 < 1. && beta2 >= 0. && beta2 < 1., "vc_adamw: betas (%g, %g) outside [0, 1)", beta1, beta2);
+  const int64_t psize = dtype == VC_F32 ? 4 : 2, ssize = state_bits / 8;
+  const uintptr_t pmask = psize == 4 ? 15 : 15, smask = ssize == 4 ? 15 : 7;
+  hipStream_t st = (hipStream_t)stream;
+  // what is written must not overlap: two blocks would race on it
+  Span stack[256];
+  std::vector<Span> heap;
+  Span* spans = stack;
+  if (4 * n_tensors > 256) {
+    try { heap.resize((size_t)(4 * n_tensors)); } catch (...) { set_error("vc_adamw: out of host memory"); return VC_ECAPACITY; }
+    spans = heap.data();
+  }
+  size_t n_spans = 0;
+  for (int64_t k = 0; k < n_tensors; ++k) {
+    const vc_adamw_tensor& T = tensors[k];
+    VC_REQUIRE(T.n >= 0, "vc_adamw: tensor %lld has n = %lld", (long long)k, (long long)T.n);
+    if (T.n == 0) continue;
+    VC_REQUIRE(T.param && T.grad && T.exp_avg && T.exp_avg_sq && (state_bits == 32 || T.exponents), "vc_adamw: tensor %lld has a NULL pointer", (long long)k);
+    VC_REQUIRE((((uintptr_t)T.param | (uintptr_t)T.grad) & (psize - 1)) == 0 && (((uintptr_t)T.exp_avg | (uintptr_t)T.exp_avg_sq) & (ssize - 1)) == 0,
+               "vc_adamw: tensor %lld is not aligned to its element size", (long long)k);
+    spans[n_spans++] = {(uintptr_t)T.param, (uintptr_t)T.param + T.n * psize};
+    spans[n_spans++] = {(uintptr_t)T.exp_avg, (uintptr_t)T.exp_avg + T.n * ssize};
+    spans[n_spans++] = {(uintptr_t)T.exp_avg_sq, (uintptr_t)T.exp_avg_sq + T.n * ssize};
+    if (state_bits == 8) spans[n_spans++] = {(uintptr_t)T.exponents, (uintptr_t)T.exponents + 2 * cdiv(T.n, kStateBlock)};
+  }
+  std::sort(spans, spans + n_spans);
+  for (size_t k = 1; k < n_spans; ++k)
+    VC_REQUIRE(spans[k].a >= spans[k - 1].b, "vc_adamw: two of the parameters and states overlap in memory");
+  AdamwArgs a;
+  a.beta1 = (float)beta1; a.beta2 = (float)beta2; a.one_minus_beta1 = (float)(1.0 - beta1); a.one_minus_beta2 = (float)(1.0 - beta2);
+  a.eps = (float)eps;
+  a.keep = (float)(1.0 - lr * weight_decay);
+  a.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
+  a.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
+  const uint32_t key = host_mix32(host_mix32(seed) + (uint32_t)step);
+  AdamwTable B;
+  int64_t k = 0;
+  while (k < n_tensors) {
+    B.n = 0;
+    unsigned blocks = 0;
+    for (; k < n_tensors && B.n < kAdamwTensors; ++k) {
+      if (tensors[k].n == 0) continue;
+      const int64_t need = cdiv(tensors[k].n, kAdamwChunk);
+      VC_REQUIRE(need < (1LL << 30), "vc_adamw: tensor %lld has %lld elements", (long long)k, (long long)tensors[k].n);
+      if (B.n && (int64_t)blocks + need >= (1LL << 30)) break;
+      vc_adamw_tensor& T = B.t[B.n];
+      T = tensors[k];
+      T.vec_ = ((((uintptr_t)T.param | (uintptr_t)T.grad) & pmask) | (((uintptr_t)T.exp_avg | (uintptr_t)T.exp_avg_sq) & smask)) == 0;
+      T.key = host_mix32(key + T.key);
+      B.block0[B.n++] = blocks;
+      blocks += (unsigned)need;
+    }
+    if (B.n == 0) break;
+    B.block0[B.n] = blocks;
+#define VC_ADAMW_LAUNCH(T)                                                                                              \
+  if (state_bits == 32) hipLaunchKernelGGL(adamw32_kernel<T>, dim3(blocks), dim3(256), 0, st, B, a);                    \
+  else hipLaunchKernelGGL(adamw8_kernel<T>, dim3(blocks), dim3(256), 0, st, B, a)
+    if (dtype == VC_F32) { VC_ADAMW_LAUNCH(float); }
+    else if (dtype == VC_F16) { VC_ADAMW_LAUNCH(_Float16); }
+    else { VC_ADAMW_LAUNCH(__bf16); }
+#undef VC_ADAMW_LAUNCH
+    VC_CHECK_LAUNCH("adamw_kernel");
+  }
+  return VC_OK;
+}
+
+}  // extern "C"

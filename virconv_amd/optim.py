@@ -10,11 +10,15 @@ that rewrites them per iteration (fastai's ``OneCycle``, ``torch.optim.lr_schedu
 (``step``, ``exp_avg``, ``exp_avg_sq`` per parameter) has the keys and shapes of ``torch.optim.AdamW``'s, so optimizer checkpoints move
 between the two.  It wants what ``feature_pass.flatten_parameters`` returns: a few contiguous fp32 tensors on the GPU (at most 16).
 There is no CPU path: without the HIP library the constructor raises.
+
+``AdamW`` takes a model as it is -- any number of fp32, fp16 or bf16 parameters, any number of groups -- and keeps the moments in 32 or in
+8 bits (vc_adamw): one launch per 48 tensors, no clip inside.
 """
 from __future__ import annotations
 
 import ctypes as C
 
+import numpy as np
 import torch
 
 from . import _lib, ops
@@ -106,3 +110,212 @@ class ClipAdamW(torch.optim.Optimizer):
     def total_norm(self):
         """The gradient norm of the last step (device tensor; None before the first step)."""
         return self._norm
+
+
+STATE_BLOCK = 128    # elements that share an exponent in the 8-bit states
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """Do the elements of t fill one stretch of memory, each once (in any order of its axes)?"""
+    if t.is_contiguous():
+        return True
+    want = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW (torch.optim.AdamW's arithmetic: true weight decay, bias correction) over all parameters of a group in a few launches.
+
+    Parameters: fp32, fp16 or bf16 tensors on one GPU, dense in any order of their axes; gradients of the same type.  The step computes in
+    fp32 and rounds a parameter once.  ``state_bits=32``: the moments are fp32, with the keys and shapes of torch.optim.AdamW's state (a
+    checkpoint of either loads into the other).  ``state_bits=8``: 2 bytes an element instead of 8 -- ``exp_avg`` and ``exp_avg_rms`` (the
+    square root of the second moment) are float8_e4m3fn values over a power of two for every 128 elements (``exponents``, int8), rounded up or
+    down at random in proportion so that a moment follows changes smaller than its resolution.  The random numbers follow from ``seed``, the
+    step and the element's place: a run repeats, and resumes from a checkpoint, bit for bit.  ``decoded_state(p)`` gives the moments as
+    fp32 tensors.  A step counts on the host, so it cannot be captured into a graph."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
+        if state_bits not in (8, 32):
+            raise ValueError(f"AdamW: states in {state_bits} bits (8 or 32)")
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+        self.state_bits, self.seed = int(state_bits), int(seed)
+        self._seen = {}
+        self._lib = ops.get_backend().lib    # raises without libvirconv_hip.so
+        for g in self.param_groups:
+            self._check_group(g)
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._seen = {}
+        self._lib = ops.get_backend().lib
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed}
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        if hasattr(self, "_lib"):
+            self._check_group(self.param_groups[-1])
+
+    def _check_group(self, g):
+        b1, b2 = g["betas"]
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"AdamW: betas {g['betas']} outside [0, 1)")
+        if not (g["lr"] >= 0.0 and g["eps"] >= 0.0 and g["weight_decay"] >= 0.0):
+            raise ValueError(f"AdamW: lr {g['lr']}, eps {g['eps']}, weight_decay {g['weight_decay']} have to be 0 or more")
+        device = self.param_groups[0]["params"][0].device
+        for p in g["params"]:
+            if not p.is_cuda or p.device != device:
+                raise ValueError(f"AdamW: parameters have to be on one GPU, got {p.device} beside {device} (there is no CPU path)")
+            if p.dtype not in _PARAM_DTYPES or not _dense(p):
+                raise ValueError(f"AdamW: wants dense float32, float16 or bfloat16 parameters, got {p.dtype} of strides {p.stride()}")
+
+    def _new_state(self, p):
+        st = self.state[p]
+        st["step"] = 0
+        if self.state_bits == 32:
+            st["exp_avg"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+            st["exp_avg_sq"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
+        else:
+            zero = torch.zeros_like(p, dtype=torch.uint8, memory_format=torch.preserve_format)
+            st["exp_avg"], st["exp_avg_rms"] = zero.view(torch.float8_e4m3fn), zero.clone().view(torch.float8_e4m3fn)
+            st["exponents"] = torch.zeros((-(-p.numel() // STATE_BLOCK), 2), dtype=torch.int8, device=p.device)
+        return st
+
+    def _check_state(self, p, st):
+        """The state's tensors as the kernel takes them: types, sizes, order of elements and device (what a checkpoint may have changed)."""
+        second, dtype = ("exp_avg_sq", torch.float32) if self.state_bits == 32 else ("exp_avg_rms", torch.float8_e4m3fn)
+        if second not in st or (self.state_bits == 8 and "exponents" not in st):
+            raise ValueError(f"AdamW: a state without {second!r}: was it saved with other state_bits than {self.state_bits}?")
+        for k in ("exp_avg", second):
+            t = st[k]
+            if t.dtype != dtype or t.shape != p.shape or t.device != p.device or t.stride() != p.stride():
+                raise ValueError(f"AdamW: state {k!r} is {t.dtype} {tuple(t.shape)} {t.stride()} on {t.device}, the parameter wants {dtype} "
+                                 f"{tuple(p.shape)} {p.stride()} on {p.device}")
+        if self.state_bits == 8:
+            e = st["exponents"]
+            if e.dtype != torch.int8 or e.shape != (-(-p.numel() // STATE_BLOCK), 2) or not e.is_contiguous() or e.device != p.device:
+                raise ValueError(f"AdamW: state 'exponents' is {e.dtype} {tuple(e.shape)} on {e.device}")
+
+    def load_state_dict(self, state_dict):
+        # torch casts every floating-point state to the parameter's type: the moments keep their own here
+        super().load_state_dict(state_dict)
+        saved = state_dict["state"]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        for i, p in zip(ids, params):
+            if i not in saved:
+                continue
+            st = self.state[p]
+            for k, v in saved[i].items():
+                if k != "step" and torch.is_tensor(v):
+                    t = torch.empty_strided(p.shape, p.stride(), dtype=v.dtype, device=p.device) if v.shape == p.shape else \
+                        torch.empty(v.shape, dtype=v.dtype, device=p.device)
+                    st[k] = t.copy_(v)
+            if self.state_bits == 32 and "exp_avg" in st:
+                for k in ("exp_avg", "exp_avg_sq"):
+                    st[k] = st[k].float()
+            st["step"] = int(saved[i]["step"])
+            self._check_state(p, st)
+
+    def decoded_state(self, p):
+        """The two moments of parameter p as fp32 tensors of its shape: (exp_avg, exp_avg_sq)."""
+        st = self.state[p]
+        if self.state_bits == 32:
+            return st["exp_avg"].clone(), st["exp_avg_sq"].clone()
+        n = p.numel()
+        scale = torch.exp2(st["exponents"].float() - 7).repeat_interleave(STATE_BLOCK, 0)[:n]
+        out = []
+        for k, name in enumerate(("exp_avg", "exp_avg_rms")):
+            flat = torch.as_strided(st[name].view(torch.uint8), (n,), (1,)).view(torch.float8_e4m3fn).float() * scale[:, k]
+            out.append(torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format))
+            torch.as_strided(out[-1], (n,), (1,)).copy_(flat)
+        return out[0], out[1] * out[1]
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        place = 0
+        for g in self.param_groups:
+            ps = g["params"]
+            grads = [p.grad for p in ps]
+            if any(x is None for x in grads):
+                live = [k for k, x in enumerate(grads) if x is not None]
+                places = [place + k for k in live]
+                self._step_tensors(g, [ps[k] for k in live], [grads[k] for k in live], places)
+            else:
+                self._step_tensors(g, ps, grads, range(place, place + len(ps)))
+            place += len(ps)
+        return loss
+
+    def _step_tensors(self, g, ps, grads, places):
+        if not ps:
+            return
+        first = ps[0]
+        index = first.get_device()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a step counts on the host (bias correction, random numbers): it cannot be captured into a graph")
+        state = self.state
+        states = [state[p] if p in state else self._new_state(p) for p in ps]
+        second = "exp_avg_sq" if self.state_bits == 32 else "exp_avg_rms"
+        for p, st in zip(ps, states):
+            if second not in st:
+                self._check_state(p, st)      # raises
+        steps = {st["step"] for st in states}
+        dtypes = {p.dtype for p in ps}
+        if len(steps) != 1 or len(dtypes) != 1 or not all(type(s) is int for s in steps):
+            # parameters that joined later, or of several types: a call for each
+            for st in states:
+                if type(st["step"]) is not int:
+                    st["step"] = int(st["step"])
+            sets = {}
+            for k, (p, st) in enumerate(zip(ps, states)):
+                sets.setdefault((st["step"], p.dtype), []).append(k)
+            if len(sets) > 1:
+                for ks in sets.values():
+                    self._step_tensors(g, [ps[k] for k in ks], [grads[k] for k in ks], [places[k] for k in ks])
+                return
+        dtype, step = first.dtype, states[0]["step"] + 1
+        if not (all(map(torch.Tensor.is_contiguous, grads)) and all(map(torch.Tensor.is_contiguous, ps))):
+            grads = [x if not x.is_sparse and x.stride() == p.stride() else self._like(p, x) for p, x in zip(ps, grads)]
+        if {x.dtype for x in grads} != dtypes or {x.get_device() for x in grads} != {index} or {p.get_device() for p in ps} != {index}:
+            raise ValueError(f"AdamW: parameters and gradients have to be {dtype} on {first.device}")
+        moments = [st["exp_avg"] for st in states], [st[second] for st in states], [st.get("exponents") for st in states]
+        sizes = [p.numel() for p in ps]
+        seen = self._seen.get((id(g), places[0], len(ps)))
+        if seen is None or seen[0] != sizes or not all(a is b for x, y in zip(seen[1], moments) for a, b in zip(x, y)):
+            for p, st in zip(ps, states):     # moments that were not here at the last step (a checkpoint, a user's own): looked over once
+                self._check_state(p, st)
+            self._seen[id(g), places[0], len(ps)] = sizes, moments
+        table = np.zeros((len(ps), 7), np.int64)
+        table[:, 0] = [p.data_ptr() for p in ps]
+        table[:, 1] = [x.data_ptr() for x in grads]
+        table[:, 2] = [t.data_ptr() for t in moments[0]]
+        table[:, 3] = [t.data_ptr() for t in moments[1]]
+        if self.state_bits == 8:
+            table[:, 4] = [t.data_ptr() for t in moments[2]]
+        table[:, 5] = sizes
+        table[:, 6] = places
+        b1, b2 = g["betas"]
+        with torch.cuda.device(index):
+            _lib.check(self._lib.vc_adamw(table.ctypes.data, len(ps), _PARAM_DTYPES[dtype], self.state_bits, float(g["lr"]), float(b1), float(b2),
+                                          float(g["eps"]), float(g["weight_decay"]), step, self.seed & 0xffffffff,
+                                          torch._C._cuda_getCurrentRawStream(index)), "vc_adamw")
+        for st in states:
+            st["step"] = step
+
+    @staticmethod
+    def _like(p, grad):
+        if grad.is_sparse:
+            raise ValueError("AdamW: gradients have to be dense")
+        return torch.empty_like(p, memory_format=torch.preserve_format).copy_(grad)
+
+
+_PARAM_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # vc_dtype
