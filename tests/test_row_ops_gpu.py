@@ -388,6 +388,22 @@ def test_grouped_linear_beyond_two_to_the_31_elements(hip_backend):
     assert not y[:100].any() and not dx[:100].any()
 
 
+def test_gradients_are_of_first_order_and_say_so(hip_backend):
+    from virconv_amd import ops
+    x, w = rnd((20, 24), 1).requires_grad_(), rnd((24,), 2).requires_grad_()
+    m, offsets = rnd((2, 16, 24), 3).requires_grad_(), torch.tensor([0, 7, 20], device="cuda")
+    for f, leaves in ((lambda: ops.layer_norm(x, w), (x, w)), (lambda: ops.grouped_linear(x, m, offsets), (x, m))):
+        first = torch.autograd.grad(f().square().sum(), leaves)
+        again = torch.autograd.grad(f().square().sum(), leaves, create_graph=True)      # a graph may be asked for ...
+        assert all(torch.equal(a, b) for a, b in zip(first, again)) and all(t.requires_grad for t in again)
+        with pytest.raises(RuntimeError, match="first-order"):                         # ... its use is refused, not answered with zeros
+            torch.autograd.grad(again[0].sum(), leaves)
+    # only what is asked for is computed, and accumulation into .grad works
+    y = ops.layer_norm(x, w.detach()) + ops.grouped_linear(x, m.detach(), offsets).sum()
+    y.sum().backward()
+    assert x.grad is not None and w.grad is None and m.grad is None
+
+
 # ---------------------------------------------------------------------------------------------------------------- AdamW
 HYPER = dict(lr=2e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.02)
 

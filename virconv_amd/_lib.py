@@ -259,6 +259,29 @@ def load() -> C.CDLL:
     return lib
 
 
+HOST_PATH = os.path.join(_HERE, "_host_ops.so")
+_host = None
+
+
+def load_host():
+    """The native host side of the row operators (csrc/host_ops.cpp) on the loaded library; raises if it has not been built."""
+    global _host
+    if _host is not None:
+        return _host
+    lib = load()
+    if not os.path.exists(HOST_PATH):
+        raise VirConvError(f"{HOST_PATH} is missing: build it with `python -m virconv_amd.build`")
+    from importlib.machinery import ExtensionFileLoader
+    from importlib.util import module_from_spec, spec_from_file_location
+    spec = spec_from_file_location("_host_ops", HOST_PATH, loader=ExtensionFileLoader("_host_ops", HOST_PATH))
+    host = module_from_spec(spec)
+    spec.loader.exec_module(host)
+    names = [n for n in SIGNATURES if n.startswith(("vc_layer_norm_", "vc_grouped_linear_"))] + ["vc_adamw", "vc_last_error"]
+    host.bind({n: C.cast(getattr(lib, n), _P).value for n in names}, VirConvError)
+    _host = host
+    return host
+
+
 def check(status: int, what: str) -> None:
     if status != VC_OK:
         msg = load().vc_last_error().decode("utf-8", "replace")

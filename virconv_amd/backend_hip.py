@@ -49,56 +49,12 @@ def conv_out_shape(in_shape, ksize, stride, padding, dilation):
     return tuple((int(i) + 2 * p - d * (k - 1) - 1) // s + 1 for i, k, s, p, d in zip(in_shape, ksize, stride, padding, dilation))
 
 
-_DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # vc_dtype
-
-
-def _dtype(t: torch.Tensor, name: str) -> int:
-    code = _DTYPES.get(t.dtype)
-    if code is None:
-        raise _lib.VirConvError(f"{name}: expected float32, float16 or bfloat16, got {t.dtype}")
-    return code
-
-
-def _rows(t: torch.Tensor) -> Tuple[torch.Tensor, int]:
-    """(tensor, row stride) of a 2-D tensor whose rows are dense (a column slice of a wider matrix passes as it is)."""
-    n, c = t.shape
-    if (t.stride(1) == 1 or c == 1) and (t.stride(0) >= c or n <= 1):
-        return t, max(t.stride(0), c)
-    return t.contiguous(), c
-
-
-class _Device:
-    """The launches of a call go to the device of its tensors, on torch's current stream there."""
-    __slots__ = ("index", "guard", "stream")
-
-    def __init__(self, *tensors):
-        first = tensors[0]
-        if not first.is_cuda:
-            raise _lib.VirConvError("expected CUDA/HIP tensors; virconv_amd has no CPU path")
-        self.index = first.get_device()
-        for t in tensors[1:]:
-            if t is not None and t.get_device() != self.index:
-                raise _lib.VirConvError(f"the tensors of a call lie on different devices: {first.device} and {t.device}")
-        self.guard = None
-
-    def __enter__(self):
-        if torch._C._cuda_getDevice() != self.index:
-            self.guard = torch.cuda.device(self.index)
-            self.guard.__enter__()
-        self.stream = torch._C._cuda_getCurrentRawStream(self.index)
-        return self
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
-
-
 class HipBackend:
     name = "hip"
 
     def __init__(self):
         self.lib = _lib.load()
+        self.host = _lib.load_host()   # layer norm, grouped products, AdamW: the native host side (csrc/host_ops.cpp)
         self._pinned = None
         self._pin_ev = None
         self._trace_cap, self._trace_pairs = 0, None
@@ -968,77 +924,3 @@ class HipBackend:
                                            _ptr(beta), float(eps), 1 if relu else 0, _ptr(dx), _ptr(dgamma), _ptr(dbeta),
                                            _ptr(absmax_ws), _ptr(ws), ws_bytes, _stream()), "vc_bn_relu_backward")
         return dx, dgamma, dbeta
-
-    # ------------------------------------------------------------------ row operators: layer norm, grouped products
-    def layer_norm_forward(self, x, weight, bias, eps: float, want_stats: bool):
-        """x (N, C) -> y (N, C), mean (N,), rstd (N,) (None, None unless wanted)."""
-        dt = _dtype(x, "layer_norm: x")
-        with _Device(x, weight, bias) as dev:
-            n, c = x.shape
-            x, ld = _rows(x)
-            y = torch.empty((n, c), dtype=x.dtype, device=x.device)
-            stats = torch.empty((2, n), dtype=torch.float32, device=x.device) if want_stats else None
-            mean, rstd = (stats[0], stats[1]) if want_stats else (None, None)
-            check(self.lib.vc_layer_norm_forward(x.data_ptr(), ld, n, c, dt, _ptr(weight), 0 if weight is None else _dtype(weight, "layer_norm: weight"),
-                                                 _ptr(bias), 0 if bias is None else _dtype(bias, "layer_norm: bias"), eps, y.data_ptr(), _ptr(mean),
-                                                 _ptr(rstd), dev.stream), "vc_layer_norm_forward")
-        return y, mean, rstd
-
-    def layer_norm_backward(self, x, dy, weight, bias, mean, rstd, need_dx: bool, need_dw: bool, need_db: bool):
-        dt = _dtype(x, "layer_norm: x")
-        with _Device(x, dy, weight) as dev:
-            n, c = x.shape
-            x, ld = _rows(x)
-            dy, dld = _rows(dy)
-            dx = torch.empty((n, c), dtype=x.dtype, device=x.device) if need_dx else None
-            dw = torch.empty((c,), dtype=weight.dtype, device=x.device) if need_dw else None
-            db = torch.empty((c,), dtype=bias.dtype, device=x.device) if need_db else None
-            ws, ws_bytes = None, 0
-            if need_dw or need_db:
-                ws_bytes = self.lib.vc_layer_norm_backward_workspace_bytes(n, c, dt)
-                ws = torch.empty((ws_bytes,), dtype=torch.uint8, device=x.device)
-            check(self.lib.vc_layer_norm_backward(x.data_ptr(), ld, dy.data_ptr(), dld, n, c, dt, _ptr(weight), 0 if weight is None else _dtype(weight, "weight"),
-                                                  0 if bias is None else _dtype(bias, "bias"), mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dw), _ptr(db),
-                                                  _ptr(ws), ws_bytes, dev.stream), "vc_layer_norm_backward")
-        return dx, dw, db
-
-    def _grouped_workspace(self, direction, rows, groups, cin, cout, dt, device):
-        n = self.lib.vc_grouped_linear_workspace_bytes(direction, rows, groups, cin, cout, dt)
-        return (torch.empty((n,), dtype=torch.uint8, device=device) if n else None), n
-
-    def grouped_linear_forward(self, x, weight, offsets, bias):
-        dt = _dtype(x, "grouped_linear: x")
-        with _Device(x, weight, offsets, bias) as dev:
-            n, (groups, cout, cin) = x.shape[0], weight.shape
-            x, ld = _rows(x)
-            y = torch.empty((n, cout), dtype=x.dtype, device=x.device)
-            ws, ws_bytes = self._grouped_workspace(0, n, groups, cin, cout, dt, x.device)
-            check(self.lib.vc_grouped_linear_forward(x.data_ptr(), ld, n, weight.data_ptr(), _ptr(bias), offsets.data_ptr(), 8 * offsets.element_size(),
-                                                     groups, cin, cout, dt, y.data_ptr(), _ptr(ws), ws_bytes, dev.stream), "vc_grouped_linear_forward")
-        return y
-
-    def grouped_linear_backward_input(self, dy, weight, offsets):
-        dt = _dtype(dy, "grouped_linear: grad")
-        with _Device(dy, weight, offsets) as dev:
-            n, (groups, cout, cin) = dy.shape[0], weight.shape
-            dy, ld = _rows(dy)
-            dx = torch.empty((n, cin), dtype=dy.dtype, device=dy.device)
-            ws, ws_bytes = self._grouped_workspace(1, n, groups, cin, cout, dt, dy.device)
-            check(self.lib.vc_grouped_linear_backward_input(dy.data_ptr(), ld, n, weight.data_ptr(), offsets.data_ptr(), 8 * offsets.element_size(), groups,
-                                                            cin, cout, dt, dx.data_ptr(), _ptr(ws), ws_bytes, dev.stream),
-                  "vc_grouped_linear_backward_input")
-        return dx
-
-    def grouped_linear_backward_weight(self, x, dy, offsets, want_bias: bool):
-        dt = _dtype(x, "grouped_linear: x")
-        with _Device(x, dy, offsets) as dev:
-            n, cin, cout, groups = x.shape[0], x.shape[1], dy.shape[1], offsets.shape[0] - 1
-            x, ld = _rows(x)
-            dy, dld = _rows(dy)
-            dw = torch.empty((groups, cout, cin), dtype=x.dtype, device=x.device)
-            db = torch.empty((groups, cout), dtype=x.dtype, device=x.device) if want_bias else None
-            ws, ws_bytes = self._grouped_workspace(2, n, groups, cin, cout, dt, x.device)
-            check(self.lib.vc_grouped_linear_backward_weight(x.data_ptr(), ld, dy.data_ptr(), dld, n, offsets.data_ptr(), 8 * offsets.element_size(), groups,
-                                                             cin, cout, dt, dw.data_ptr(), _ptr(db), _ptr(ws), ws_bytes, dev.stream),
-                  "vc_grouped_linear_backward_weight")
-        return dw, db

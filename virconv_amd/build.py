@@ -1,4 +1,4 @@
-"""Build libvirconv_hip.so (gfx950) in-tree with hipcc.  ``python -m virconv_amd.build [--force]``.
+"""Build libvirconv_hip.so (gfx950, hipcc) and _host_ops.so (the host side that works on torch tensors, g++) in-tree.  ``python -m virconv_amd.build [--force]``.
 
 The shared object lands next to this file (``virconv_amd/libvirconv_hip.so``): it is git-ignored but travels to the
 GPU box with the gpurun snapshot.  hipcc cross-compiles without a GPU.
@@ -14,6 +14,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libvirconv_hip.so")
+HOST_LIB = os.path.join(HERE, "_host_ops.so")
 ARCH = "gfx950"
 
 # no packed fp32 instructions (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32): some of their forms have given wrong results on MI355X now and then
@@ -37,7 +38,7 @@ SOURCES = {
     # the AdamW step is defined operation by operation (8-bit states: bit-equal to the same operations of torch), so nothing is contracted
     "adamw_kernels.hip": ["-ffp-contract=off", *NO_PACKED_FP32],
     "norm_kernels.hip": [*NO_PACKED_FP32],
-    "grouped_kernels.hip": [*NO_PACKED_FP32],
+    "grouped_kernels.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", *NO_PACKED_FP32],
     "unit.hip": [],
     "pass.hip": [],
     "plan.hip": [],
@@ -68,9 +69,38 @@ def build(force: bool = False, verbose: bool = True) -> str:
     out, extra_env = os.environ.get("VIRCONV_LIB_OUT"), os.environ.get("VIRCONV_HIPCC_EXTRA", "").split()
     if out:
         return _build_to(out, os.path.join(HERE, "build_ab"), extra_env, verbose)
+    build_host(force, verbose)
     if not force and not _stale():
         return LIB
     return _build_to(LIB, os.path.join(HERE, "build"), extra_env, verbose, force_all=force)
+
+
+def build_host(force: bool = False, verbose: bool = True) -> str:
+    """_host_ops.so: csrc/host_ops.cpp against the headers of the installed torch (host code only; rebuilt when torch is another one)."""
+    import sysconfig
+    import torch
+    src, header = os.path.join(CSRC, "host_ops.cpp"), os.path.join(HERE, "..", "include", "virconv_hip.h")
+    root = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+           "-DTORCH_EXTENSION_NAME=_host_ops", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-isystem{d}" for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
+                                      os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_hipcc()))), "include"),
+                                      sysconfig.get_paths()["include"])),
+           src, "-o", HOST_LIB + ".tmp", "-L" + os.path.join(root, "lib"), "-lc10", "-ltorch_cpu", "-ltorch_python", "-lc10_hip"]
+    os.makedirs(os.path.join(HERE, "build"), exist_ok=True)
+    stamp, line = os.path.join(HERE, "build", "host_ops.cmd"), " ".join(cmd) + " # torch " + torch.__version__
+    if (not force and os.path.exists(HOST_LIB) and os.path.exists(stamp) and open(stamp).read() == line
+            and all(os.path.getmtime(d) < os.path.getmtime(HOST_LIB) for d in (src, header))):
+        return HOST_LIB
+    if verbose:
+        print("[virconv_amd.build]", " ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on host_ops.cpp:\n{r.stdout}\n{r.stderr}")
+    os.replace(HOST_LIB + ".tmp", HOST_LIB)
+    with open(stamp, "w") as f:
+        f.write(line)
+    return HOST_LIB
 
 
 def _build_to(LIB: str, objdir: str, extra_env, verbose: bool, force_all: bool = False) -> str:

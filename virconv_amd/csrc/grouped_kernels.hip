@@ -189,16 +189,21 @@ struct Tile {
       stage8(lds, plane_bytes, at, reg[i]);
     }
   }
-  // the 16 rows from r0 on, 32 summed indices from k0 on, as an operand of v_mfma_f32_16x16x32: lane l holds row l % 16, eight indices
-  static __device__ __forceinline__ v8s fragment(const char* lds, int plane, int r0, int k0) {
+  // The 16 rows from r0 on (a multiple of 16), 32 summed indices from k0 on (a multiple of 32), as an operand of v_mfma_f32_16x16x32: lane l
+  // holds row l % 16, the eight indices from 8 (l / 16) on.  `lane_place` is the lane's part of the address, to be made once per tile row.
+  static __device__ __forceinline__ int lane_place(int r0) {
     const int lane = threadIdx.x & 63;
+    if constexpr (ALONG) return place(r0 + (lane & 15), (lane >> 4) * 8);
+    else return place(r0 + (lane & 3) * 4, (lane >> 4) * 8 + ((lane & 15) >> 2));
+  }
+  static __device__ __forceinline__ v8s fragment(const char* lds, int plane, int at, int k0) {
     if constexpr (ALONG) {
-      return *reinterpret_cast<const v8s*>(lds + plane * plane_bytes + place(r0 + (lane & 15), k0 + (lane >> 4) * 8));
+      return *reinterpret_cast<const v8s*>(lds + plane * plane_bytes + (at ^ (k0 << 1)));   // (32 indices on: bit 6 of the exchanged piece)
     } else {
-      const int k = k0 + (lane >> 4) * 8 + ((lane & 15) >> 2), c = r0 + (lane & 3) * 4;
       typedef __attribute__((address_space(3))) v4s lds4;
-      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(lds + plane * plane_bytes + place(c, k)));
-      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(lds + plane * plane_bytes + place(c, k + 4)));
+      const char* p = lds + at + plane * plane_bytes + k0 * ROWS * 2;
+      const v4s lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)p);
+      const v4s hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4*)(p + 4 * ROWS * 2));
       return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
@@ -239,7 +244,7 @@ template <typename T> __device__ __forceinline__ void store4(T* p, int valid, co
 
 // ------------------------------------------------------------------------------------------------ the kernel
 template <typename T, int BM, int BN, int MODE>
-__global__ void __launch_bounds__(256) grouped_kernel(GroupArgs a) {
+__global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
   typedef typename OperandOf<T>::type O;
   constexpr int BK = OperandOf<T>::bk, P = OperandOf<T>::planes;
   typedef Tile<T, BM, MODE != kBackWeight> TileA;
@@ -329,6 +334,11 @@ __global__ void __launch_bounds__(256) grouped_kernel(GroupArgs a) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
   }
+  int at_a[FM], at_b[FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) at_a[i] = TileA::lane_place(wm * (BM / WM) + i * 16);
+#pragma unroll
+  for (int j = 0; j < FN; ++j) at_b[j] = TileB::lane_place(wn * (BN / WN) + j * 16);
   TileA ta;
   TileB tb;
   ta.fetch(pa, lda, rows_a, depth);
@@ -349,12 +359,12 @@ __global__ void __launch_bounds__(256) grouped_kernel(GroupArgs a) {
 #pragma unroll
       for (int j = 0; j < FN; ++j)
 #pragma unroll
-        for (int q = 0; q < P; ++q) fb[j][q] = TileB::fragment(lb, q, wn * (BN / WN) + j * 16, kk);
+        for (int q = 0; q < P; ++q) fb[j][q] = TileB::fragment(lb, q, at_b[j], kk);
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
         v8s fa[P];
 #pragma unroll
-        for (int q = 0; q < P; ++q) fa[q] = TileA::fragment(la, q, wm * (BM / WM) + i * 16, kk);
+        for (int q = 0; q < P; ++q) fa[q] = TileA::fragment(la, q, at_a[i], kk);
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
           // the lane's four results are neighbours along n: the n side is the instruction's row operand
@@ -407,13 +417,25 @@ __global__ void __launch_bounds__(256) grouped_kernel(GroupArgs a) {
   }
 }
 
-// row products: the splits' sums added in order (+ bias)
+// the sum of `count` values `stride` apart, in order: a chain, its loads four at a time
+__device__ __forceinline__ float sum_along(const float* p, unsigned count, int64_t stride) {
+  float s = 0.f;
+  unsigned q = 0;
+  for (; q + 4 <= count; q += 4, p += 4 * stride) {
+    const float v0 = p[0], v1 = p[stride], v2 = p[2 * stride], v3 = p[3 * stride];
+    s += v0; s += v1; s += v2; s += v3;
+  }
+  for (; q < count; ++q, p += stride) s += *p;
+  return s;
+}
+
+// row products: the splits' sums added in order (+ bias); a wave takes 64 columns of a row
 template <typename T>
 __global__ void __launch_bounds__(256) grouped_row_sum_kernel(GroupArgs a) {
-  // one row a wave at a time; its group: the last one that begins at or before it
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, chunks = (a.n + 63) / 64;
+  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row = id / chunks;
   if (row >= a.rows) return;
-  const int lane = threadIdx.x & 63;
+  // the row's group: the first one whose end lies behind it
   int group = -1;
   int64_t high = 0;
   for (int g0 = 0; g0 < a.groups && group < 0; g0 += 64) {
@@ -430,20 +452,19 @@ __global__ void __launch_bounds__(256) grouped_row_sum_kernel(GroupArgs a) {
     if (hit) group = g0 + __builtin_ctzll(hit);
     high = shfl64(end, 63);
   }
-  T* out = (T*)a.out + row * a.n;
-  if (group < 0) return;   // rows of no group: written by the tiles' kernel
-  for (int n = lane; n < a.n; n += 64) {
-    float s = 0.f;
-    for (int q = 0; q < a.splits; ++q) s += a.partial[((int64_t)q * a.rows + row) * a.n + n];
-    if (a.bias) s += (float)((const T*)a.bias)[(int64_t)group * a.n + n];
-    out[n] = (T)s;
-  }
+  const int n = (int)(id % chunks) * 64 + lane;
+  if (group < 0 || n >= a.n) return;   // (rows of no group: written by the tiles' kernel)
+  float s = sum_along(a.partial + row * a.n + n, a.splits, a.rows * a.n);
+  if (a.bias) s += (float)((const T*)a.bias)[(int64_t)group * a.n + n];
+  ((T*)a.out)[row * a.n + n] = (T)s;
 }
 
-// weight product: the pieces' sums of each group added in order
+// weight product: the pieces' sums of each group.  64 elements a block; its four waves add a quarter of the pieces each, in order, and the four
+// sums are added in order.
 template <typename T>
 __global__ void __launch_bounds__(256) grouped_weight_sum_kernel(GroupArgs a) {
-  const int group = blockIdx.y, lane = threadIdx.x & 63;
+  __shared__ float part[4][64];
+  const int group = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // pieces in front of the group, and its own
   int64_t high = 0;
   unsigned before = 0, mine = 0;
@@ -464,18 +485,20 @@ __global__ void __launch_bounds__(256) grouped_weight_sum_kernel(GroupArgs a) {
     if (group - g0 < 64) mine = __shfl(pieces, group - g0, 64);
     high = shfl64(end, 63);
   }
-  const int64_t size = (int64_t)a.m * a.n;
-  for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < size; e += (int64_t)gridDim.x * 256) {
-    float s = 0.f;
-    for (unsigned q = 0; q < mine; ++q) s += a.partial[(int64_t)(before + q) * size + e];
-    ((T*)a.out)[group * size + e] = (T)s;
-  }
-  if (a.dbias)
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < a.m; e += (int64_t)gridDim.x * 256) {
-      float s = 0.f;
-      for (unsigned q = 0; q < mine; ++q) s += a.partial_bias[(int64_t)(before + q) * a.m + e];
-      ((T*)a.dbias)[group * (int64_t)a.m + e] = (T)s;
+  const int64_t weights = (int64_t)a.m * a.n, size = weights + (a.dbias ? a.m : 0);
+  const unsigned per = (mine + 3) / 4, q0 = min(wave * per, mine), q1 = min(q0 + per, mine);
+  for (int64_t e0 = (int64_t)blockIdx.x * 64; e0 < size; e0 += (int64_t)gridDim.x * 64) {
+    const int64_t e = e0 + lane, i = e - weights;
+    if (e < weights) part[wave][lane] = sum_along(a.partial + (int64_t)(before + q0) * weights + e, q1 - q0, weights);
+    else if (e < size) part[wave][lane] = sum_along(a.partial_bias + (int64_t)(before + q0) * a.m + i, q1 - q0, a.m);
+    __syncthreads();
+    if (wave == 0 && e < size) {
+      const float s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+      if (e < weights) ((T*)a.out)[group * weights + e] = (T)s;
+      else ((T*)a.dbias)[group * (int64_t)a.m + i] = (T)s;
     }
+    __syncthreads();
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ launch rules
@@ -489,9 +512,10 @@ static GroupPlan plan_rows(int64_t rows, int64_t groups, int64_t n, int64_t k, i
   p.bm = average > 96 && n > 64 ? 128 : average > 24 ? 64 : 16;
   p.bn = p.bm == 64 ? 64 : 128;
   p.mtiles_most = rows / p.bm + groups + 2;
-  const int64_t tiles = cdiv(rows, p.bm) * cdiv(n, p.bn), steps = cdiv(k, bk);
+  // tiles there will be: full ones, and one that is cut short for every group that has rows
+  const int64_t tiles = (rows / p.bm + (groups < rows ? groups : rows)) * cdiv(n, p.bn), steps = cdiv(k, bk);
   int64_t splits = 1;
-  if (tiles < 256 && steps >= 16) splits = cdiv(512, tiles);
+  if (tiles < 256 && steps >= 16) splits = 512 / tiles;
   if (splits > steps / 8) splits = steps / 8 > 0 ? steps / 8 : 1;
   p.per_split = (int)(cdiv(steps, splits) * bk);
   p.splits = (int)cdiv(k, p.per_split);
@@ -542,7 +566,7 @@ static int launch_rows(const char* who, GroupArgs a, int mode, int dtype, const 
 #define VC_GO(T, BM, BN)                                                                                                          \
   if (mode == kForward) hipLaunchKernelGGL((grouped_kernel<T, BM, BN, kForward>), dim3(a.total), dim3(256), 0, st, a);            \
   else hipLaunchKernelGGL((grouped_kernel<T, BM, BN, kBackInput>), dim3(a.total), dim3(256), 0, st, a);                           \
-  if (p.splits > 1) hipLaunchKernelGGL(grouped_row_sum_kernel<T>, dim3((unsigned)cdiv(a.rows, 4)), dim3(256), 0, st, a)
+  if (p.splits > 1) hipLaunchKernelGGL(grouped_row_sum_kernel<T>, dim3((unsigned)cdiv(a.rows * cdiv(a.n, 64), 4)), dim3(256), 0, st, a)
 #define VC_TILES(T)                                       \
   if (p.bm == 128) { VC_GO(T, 128, 128); }                \
   else if (p.bm == 64) { VC_GO(T, 64, 64); }              \
@@ -619,12 +643,12 @@ int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const voi
   VC_REQUIRE(total < (1LL << 31), "%s: %lld tiles", who, (long long)total);
   a.total = (unsigned)total;
   hipStream_t st = (hipStream_t)stream;
-  const int64_t sum_blocks = cdiv(out * in, 256 * 4);
+  const int64_t sum_blocks = cdiv(out * in + out, 64);
 #define VC_GO(T)                                                                                                                              \
   if (p.bm == 128) hipLaunchKernelGGL((grouped_kernel<T, 128, 128, kBackWeight>), dim3(a.total), dim3(256), 0, st, a);                        \
   else hipLaunchKernelGGL((grouped_kernel<T, 64, 64, kBackWeight>), dim3(a.total), dim3(256), 0, st, a);                                      \
   if (p.splits > 1)                                                                                                                           \
-    hipLaunchKernelGGL(grouped_weight_sum_kernel<T>, dim3((unsigned)(sum_blocks < 1024 ? sum_blocks : 1024), (unsigned)groups), dim3(256), 0, st, a)
+    hipLaunchKernelGGL(grouped_weight_sum_kernel<T>, dim3((unsigned)(sum_blocks < 16384 ? sum_blocks : 16384), (unsigned)groups), dim3(256), 0, st, a)
   if (dtype == VC_F32) { VC_GO(float); } else if (dtype == VC_F16) { VC_GO(_Float16); } else { VC_GO(__bf16); }
 #undef VC_GO
   VC_CHECK_LAUNCH(who);

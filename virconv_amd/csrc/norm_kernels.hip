@@ -294,28 +294,31 @@ __global__ void __launch_bounds__(256) norm_column_sums_kernel(NormBackArgs a) {
   out[a.c + c] = db;
 }
 
-// dw and db from the blocks' rows: 64 columns a block, four slices of the rows, added in a fixed order
+// dw and db from the blocks' rows: 16 columns a block, 16 slices of the rows, four loads in flight a thread; added in a fixed order
 __global__ void __launch_bounds__(256) norm_param_grad_kernel(const float* __restrict__ partial, int rows, int64_t c, void* dw, int wtype, void* db,
                                                               int btype) {
-  __shared__ float lds[4][64];
-  const int64_t col = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int slice = threadIdx.x >> 6;
-  const int per = (rows + 3) / 4, r0 = slice * per, r1 = min(r0 + per, rows);
+  __shared__ float lds[16][17];
+  const int x = threadIdx.x & 15, slice = threadIdx.x >> 4;
+  const int64_t col = (int64_t)blockIdx.x * 16 + x;
+  const int per = (rows + 15) / 16, r0 = slice * per, r1 = min(r0 + per, rows);
   float s0 = 0.f, s1 = 0.f, s2 = 0.f, s3 = 0.f;
   if (col < 2 * c) {
+    const float* p = partial + col + (int64_t)r0 * 2 * c;
     int r = r0;
-    for (; r + 4 <= r1; r += 4) {
-      s0 += partial[(int64_t)r * 2 * c + col];
-      s1 += partial[(int64_t)(r + 1) * 2 * c + col];
-      s2 += partial[(int64_t)(r + 2) * 2 * c + col];
-      s3 += partial[(int64_t)(r + 3) * 2 * c + col];
+    for (; r + 4 <= r1; r += 4, p += 8 * c) {
+      s0 += p[0];
+      s1 += p[2 * c];
+      s2 += p[4 * c];
+      s3 += p[6 * c];
     }
-    for (; r < r1; ++r) s0 += partial[(int64_t)r * 2 * c + col];
+    for (; r < r1; ++r, p += 2 * c) s0 += *p;
   }
-  lds[slice][threadIdx.x & 63] = (s0 + s1) + (s2 + s3);
+  lds[slice][x] = (s0 + s1) + (s2 + s3);
   __syncthreads();
   if (slice || col >= 2 * c) return;
-  const float s = (lds[0][threadIdx.x] + lds[1][threadIdx.x]) + (lds[2][threadIdx.x] + lds[3][threadIdx.x]);
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s += lds[i][x];
   void* out = col < c ? dw : db;
   const int type = col < c ? wtype : btype;
   const int64_t i = col < c ? col : col - c;
@@ -440,7 +443,7 @@ int vc_layer_norm_backward(const void* x, int64_t x_stride, const void* dy, int6
     }
   }
   if (sums) {
-    hipLaunchKernelGGL(norm_param_grad_kernel, dim3((unsigned)cdiv(2 * c, 64)), dim3(256), 0, st, (const float*)workspace, n > 0 ? (int)blocks : 0, c,
+    hipLaunchKernelGGL(norm_param_grad_kernel, dim3((unsigned)cdiv(2 * c, 16)), dim3(256), 0, st, (const float*)workspace, n > 0 ? (int)blocks : 0, c,
                        dweight, weight_dtype, dbias, bias_dtype);
     VC_CHECK_LAUNCH("norm_param_grad_kernel");
   }

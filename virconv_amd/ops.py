@@ -619,74 +619,13 @@ def bn_relu(x: torch.Tensor, bn: torch.nn.BatchNorm1d, relu: bool) -> torch.Tens
     return outs[0] if len(outs) == 1 else torch.cat(outs, 1)
 
 
-class LayerNormFunction(torch.autograd.Function):
-    """Layer norm over the last axis of (N, C) rows; the backward pass returns dx and the sums dweight, dbias in one walk over x and dy."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = get_backend().layer_norm_forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        return y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        need = ctx.needs_input_grad
-        return (*get_backend().layer_norm_backward(x, grad_out, weight, bias, mean, rstd, need[0], need[1], need[2]), None)
-
-
-def _wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """Layer norm over the last axis: y = (x - mean) / sqrt(var + eps) * weight + bias, statistics per row in fp32.
 
     x: (..., C) in float32, float16 or bfloat16 on the GPU; the result has its shape and type and is dense.  Rows may be strided (a column
-    slice of a wider matrix is not copied).  weight, bias: (C,) in x's type or float32, or None; their gradients have their own types."""
-    if x.dim() < 1 or x.shape[-1] < 1:
-        raise ValueError(f"layer_norm: wants rows of at least one channel, got a tensor of shape {tuple(x.shape)}")
-    c = x.shape[-1]
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is None:
-            continue
-        if t.shape != (c,):
-            raise ValueError(f"layer_norm: {name} has shape {tuple(t.shape)}, expected ({c},)")
-        if t.dtype != x.dtype and t.dtype != torch.float32:
-            raise ValueError(f"layer_norm: {name} is {t.dtype}; with {x.dtype} rows it has to be {x.dtype} or torch.float32")
-    eps = float(eps)
-    if not eps >= 0.0:
-        raise ValueError(f"layer_norm: eps = {eps}")
-    weight = weight if weight is None or weight.is_contiguous() else weight.contiguous()
-    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    rows = x if x.dim() == 2 else x.reshape(-1, c)
-    if _wants_grad(x, weight, bias):
-        y = LayerNormFunction.apply(rows, weight, bias, eps)
-    else:
-        y, _, _ = get_backend().layer_norm_forward(rows, weight, bias, eps, False)
-    return y if x.dim() == 2 else y.view(x.shape)
-
-
-class GroupedLinearFunction(torch.autograd.Function):
-    """y_r = weight[g] x_r + bias[g] for the rows r of group g; backward: the two transposed products."""
-
-    @staticmethod
-    def forward(ctx, x, weight, offsets, bias):
-        ctx.save_for_backward(x, weight, offsets)
-        return get_backend().grouped_linear_forward(x, weight, offsets, bias)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, grad_out):
-        x, weight, offsets = ctx.saved_tensors
-        be = get_backend()
-        need_dx, need_dw, _, need_db = ctx.needs_input_grad
-        dx = be.grouped_linear_backward_input(grad_out, weight, offsets) if need_dx else None
-        dw = db = None
-        if need_dw or need_db:
-            dw, db = be.grouped_linear_backward_weight(x, grad_out, offsets, need_db)
-        return dx, dw if need_dw else None, None, db
+    slice of a wider matrix is not copied).  weight, bias: (C,) in x's type or float32, or None; their gradients have their own types and a
+    fixed order of additions.  First-order gradients."""
+    return get_backend().host.layer_norm(x, weight, bias, eps)
 
 
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -695,21 +634,8 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     x: (N, in) rows sorted by group, in float32 (products accurate to fp32), float16 or bfloat16, on the GPU; rows may be strided.
     weight: (G, out, in), bias: (G, out) or None, in x's type.  offsets: (G + 1,) int32 or int64 on the GPU, rising within [0, N]: they are
     never read on the host, so what a router counted needs no synchronisation.  A group may have no rows; rows of no group (before
-    offsets[0], from offsets[G] on) give zeros and zero gradients.  -> (N, out)"""
-    if x.dim() != 2 or weight.dim() != 3 or x.shape[1] != weight.shape[2] or weight.shape[1] < 1 or weight.shape[2] < 1:
-        raise ValueError(f"grouped_linear: wants x (N, in) and weight (G, out, in), got {tuple(x.shape)} and {tuple(weight.shape)}")
-    if weight.dtype != x.dtype or (bias is not None and bias.dtype != x.dtype):
-        raise ValueError(f"grouped_linear: x, weight and bias have to be of one type, got {x.dtype}, {weight.dtype}, {None if bias is None else bias.dtype}")
-    if offsets.dim() != 1 or offsets.shape[0] != weight.shape[0] + 1 or offsets.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"grouped_linear: offsets have to be {weight.shape[0] + 1} int32 or int64 values, got {tuple(offsets.shape)} {offsets.dtype}")
-    if bias is not None and bias.shape != weight.shape[:2]:
-        raise ValueError(f"grouped_linear: bias has shape {tuple(bias.shape)}, expected {tuple(weight.shape[:2])}")
-    weight = weight if weight.is_contiguous() else weight.contiguous()
-    offsets = offsets if offsets.is_contiguous() else offsets.contiguous()
-    bias = bias if bias is None or bias.is_contiguous() else bias.contiguous()
-    if _wants_grad(x, weight, bias):
-        return GroupedLinearFunction.apply(x, weight, offsets, bias)
-    return get_backend().grouped_linear_forward(x, weight, offsets, bias)
+    offsets[0], from offsets[G] on) give zeros and zero gradients.  First-order gradients.  -> (N, out)"""
+    return get_backend().host.grouped_linear(x, weight, offsets, bias)
 
 
 def project_uv(indices, calib, trans, batch_size, stride):

@@ -143,15 +143,18 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: states in {state_bits} bits (8 or 32)")
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
         self.state_bits, self.seed = int(state_bits), int(seed)
-        self._seen = {}
-        self._lib = ops.get_backend().lib    # raises without libvirconv_hip.so
+        self._attach()
         for g in self.param_groups:
             self._check_group(g)
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._seen = {}
-        self._lib = ops.get_backend().lib
+        self._attach()
+
+    def _attach(self):
+        be = ops.get_backend()               # raises without libvirconv_hip.so
+        self._lib, self._host = be.lib, be.host
+        self._seen, self._order, self._lists = {}, [], {}
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed}
@@ -242,9 +245,18 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: a step counts on the host (bias correction, random numbers): it cannot be captured into a graph")
         place = 0
-        for g in self.param_groups:
+        for k, g in enumerate(self.param_groups):
             ps = g["params"]
+            b1, b2 = g["betas"]
+            states = self._states_of(k, ps)
+            if states is not None and self._host.adamw(ps, states, place, self.state_bits, float(g["lr"]), float(b1), float(b2), float(g["eps"]),
+                                                       float(g["weight_decay"]), self.seed & 0xffffffff) >= 0:
+                place += len(ps)
+                continue
+            # the first step, parameters without gradients, of several types or orders, or something to refuse
             grads = [p.grad for p in ps]
             if any(x is None for x in grads):
                 live = [k for k, x in enumerate(grads) if x is not None]
@@ -255,13 +267,21 @@ class AdamW(torch.optim.Optimizer):
             place += len(ps)
         return loss
 
+    def _states_of(self, k, ps):
+        """The state dicts of group k's parameters, in order; None before all of them have one.  The list is kept as long as self.state holds
+        the same dicts and the group the same parameters."""
+        if not self._host.same_values(self.state, self._order):
+            self._order, self._lists = list(self.state.values()), {}
+        known = self._lists.get(k)
+        if known is None or not self._host.same_objects(ps, known[0]):
+            known = self._lists[k] = (list(ps), [self.state[p] for p in ps] if all(p in self.state for p in ps) else None)
+        return known[1]
+
     def _step_tensors(self, g, ps, grads, places):
         if not ps:
             return
         first = ps[0]
         index = first.get_device()
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW: a step counts on the host (bias correction, random numbers): it cannot be captured into a graph")
         state = self.state
         states = [state[p] if p in state else self._new_state(p) for p in ps]
         second = "exp_avg_sq" if self.state_bits == 32 else "exp_avg_rms"
