@@ -329,8 +329,8 @@ typedef struct vc_adamw_tensor {
   void* exp_avg_sq;    /* n floats, or n e4m3 codes of the square root */
   int8_t* exponents;   /* 8-bit states */
   int64_t n;
-  uint32_t key;        /* the tensor's place in the model: tells its random numbers from another tensor's */
-  int32_t vec_;        /* not read */
+  uint32_t key;        /* the tensor's place in the model (< 2^20): tells its random numbers from another tensor's */
+  int32_t reserved_;
 } vc_adamw_tensor;
 int vc_adamw(const vc_adamw_tensor* tensors, int64_t n_tensors, int dtype, int state_bits, double lr, double beta1, double beta2, double eps,
              double weight_decay, int64_t step, uint32_t seed, void* stream);

@@ -81,8 +81,9 @@ def encode_blocks(x, bits16):
     finite = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x))
     e = torch.clamp(((finite.amax(1).view(torch.int32) >> 23) - 127), min=-119)
     y = x.abs() * power(7 - e)[:, None]
-    low = torch.where(y < 2.0 ** -6, torch.full_like(y, 2.0 ** -6), torch.zeros_like(y))
-    z = (((y + low).view(torch.int32) + (bits16 << 4).to(torch.int32)) & -(1 << 20)).view(torch.float32) - low
+    # above 2^-6: the 20 bits behind e4m3's three mantissa bits, carried into them; below, where the values are 2^-9 apart: the exact sum
+    z = ((y.view(torch.int32) + (bits16 << 4).to(torch.int32)) & -(1 << 20)).view(torch.float32)
+    z = torch.where(y < 2.0 ** -6, (torch.floor(y.double() * 512 + bits16.double() / 65536) / 512).float(), z)
     z = torch.where(y < 256, z, torch.full_like(z, math.nan))
     return torch.copysign(z, x).to(torch.float8_e4m3fn), e.to(torch.int8)
 
@@ -113,6 +114,7 @@ class Adam8:
         r = v.double().sqrt().float()      # correctly rounded (the CPU's fp32 root is not); 53 bits are enough for that
         scale = 1.0 / math.sqrt(1.0 - b2 ** self.step_)
         p = p * (1.0 - lr * wd) - lr / (1.0 - b1 ** self.step_) * (m / (r * scale + eps))
+        self.ratio = (m / (r * scale + eps)).reshape(-1)[:self.n].double()
         self.p = p.reshape(-1)[:self.n].to(self.p.dtype)
         key = mix32((mix32((mix32(self.seed) + self.step_) & 0xFFFFFFFF) + self.key) & 0xFFFFFFFF)
         bits = mix32(torch.arange(m.numel()).view(-1, BLOCK) ^ key)

@@ -89,6 +89,7 @@ def test_adamw_abi_refusals():
     refused(go(table((0x1000, 0x2000, 0x3000, 0x4000, 0, 16, 0)), bits=8), b"NULL")
     refused(go(table((0x1002, 0x2000, 0x3000, 0x4000, 0, 16, 0))), b"aligned")
     refused(go(table((0x1000, 0x2000, 0x3000, 0x4000, 0, -1, 0))), b"n = -1")
+    refused(go(table((0x1000, 0x2000, 0x3000, 0x4000, 0, 16, 1 << 20))), b"place")
     refused(go(table((0x1000, 0x2000, 0x3000, 0x3020, 0, 16, 0))), b"overlap")
     refused(go(table(ok, (0x103c, 0x2000, 0x6000, 0x7000, 0, 16, 0)), n=2), b"overlap")
     assert go(table((0, 0, 0, 0, 0, 0, 0))) == _lib.VC_OK and go(None, n=0) == _lib.VC_OK

@@ -12,7 +12,7 @@
 // steps (6 to 12 per cent of a value) are far wider than what one step changes of a moment (1 - b2 = 1 per cent of v), so rounding to the
 // nearest value would leave a moment where it is for good; it is rounded up with the probability of its distance from the lower
 // neighbour instead, which keeps every moment's mean.  The random numbers are a function of (seed, step, tensor, element), so a run can be
-// repeated, and resumed, bit for bit.  An infinite or undefined moment is held as NaN; it does not take part in its block's exponent.
+// repeated, and resumed, bit for bit.  An infinite or undefined moment is held as NaN and has no part in its block's exponent.
 #include "common.h"
 
 #include <math.h>
@@ -22,18 +22,34 @@
 
 namespace vc {
 
-static constexpr int kAdamwTensors = 48;    // per launch: the table travels in the kernel's arguments (48 x 56 + 49 x 4 bytes < 4 KB)
+static constexpr int kAdamwTensors = 64;    // per launch: the table travels in the kernel's arguments (64 x 48 + 64 x 4 bytes < 4 KB)
 static constexpr int kAdamwChunk = 2048;    // elements of one block: 256 threads x 8
 static constexpr int kStateBlock = 128;     // elements that share an exponent: 16 lanes x 8
 
+struct AdamwTensor {
+  void* param;
+  const void* grad;
+  void *exp_avg, *exp_avg_sq;
+  int8_t* exponents;
+  uint64_t n_place;      // elements (44 bits), place in the model (20 bits)
+};
+
 struct AdamwTable {
-  vc_adamw_tensor t[kAdamwTensors];
-  unsigned block0[kAdamwTensors + 1];
+  AdamwTensor t[kAdamwTensors];
+  unsigned block0[kAdamwTensors];
+  uint64_t vec;          // a bit a tensor: its pointers allow 16-byte accesses (8-byte ones of the 8-bit states)
   int n;
 };
+static_assert(sizeof(AdamwTable) < 3600, "kernel arguments are limited to 4 KB");
+
+__host__ __device__ static inline uint32_t mix32(uint32_t x) {   // the finalizer of MurmurHash3
+  x ^= x >> 16; x *= 0x85ebca6bu; x ^= x >> 13; x *= 0xc2b2ae35u; x ^= x >> 16;
+  return x;
+}
 
 struct AdamwArgs {
   float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, keep, step_size, inv_bc2_sqrt;
+  uint32_t key;          // of the seed and the step
 };
 
 template <typename T> struct Elem;
@@ -89,10 +105,10 @@ __device__ __forceinline__ int adamw_find(const AdamwTable& B) {
 template <typename T>
 __global__ void __launch_bounds__(256) adamw32_kernel(AdamwTable B, AdamwArgs a) {
   const int s = adamw_find(B);
-  const vc_adamw_tensor& S = B.t[s];
-  const int64_t n = S.n, i = (int64_t)(blockIdx.x - B.block0[s]) * kAdamwChunk + threadIdx.x * 8;
+  const AdamwTensor& S = B.t[s];
+  const int64_t n = (int64_t)(S.n_place & ((1ull << 44) - 1)), i = (int64_t)(blockIdx.x - B.block0[s]) * kAdamwChunk + threadIdx.x * 8;
   if (i >= n) return;
-  const bool vec = S.vec_;
+  const bool vec = B.vec >> s & 1;
   float p[8], g[8], m[8], v[8];
   load8((const T*)S.grad, i, n, vec, g);
   load8((const float*)S.exp_avg, i, n, vec, m);
@@ -107,11 +123,6 @@ __global__ void __launch_bounds__(256) adamw32_kernel(AdamwTable B, AdamwArgs a)
   store8((float*)S.exp_avg, i, n, vec, m);
   store8((float*)S.exp_avg_sq, i, n, vec, v);
   store8((T*)S.param, i, n, vec, p);
-}
-
-__device__ __forceinline__ uint32_t mix32(uint32_t x) {   // the finalizer of MurmurHash3
-  x ^= x >> 16; x *= 0x85ebca6bu; x ^= x >> 13; x *= 0xc2b2ae35u; x ^= x >> 16;
-  return x;
 }
 
 template <int CTRL>
@@ -144,87 +155,96 @@ __device__ __forceinline__ void decode8(const void* codes, int64_t i, int64_t n,
   }
 }
 
-// the magnitude's bits where it is finite, 0 otherwise: what the block's exponent is taken from
-__device__ __forceinline__ uint32_t finite_bits(float x) {
-  const uint32_t b = __float_as_uint(x) & 0x7fffffffu;
-  return b < 0x7f800000u ? b : 0u;
+// the magnitude's bits where it is finite, 0 otherwise
+__device__ __forceinline__ uint32_t finite_bits(uint32_t magnitude) { return magnitude < 0x7f800000u ? magnitude : 0u; }
+
+// The root of v >= 0: v_rsq_f32 with one correction by the exact residual, 8 issue slots where the library's correctly rounded root takes 17
+// (the last bit differs for one value in 280).  Below 2^-126, where v itself has lost bits, it falls with v instead of its root, to 0 at 0.
+__device__ __forceinline__ float root(float v) {
+  const float y = __builtin_amdgcn_rsqf(fmaxf(v, 0x1p-126f)), s = v * y;
+  return __builtin_fmaf(__builtin_fmaf(-s, s, v), 0.5f * y, s);
 }
 
-// one value onto the e4m3 grid: up with the probability of its distance from the lower neighbour (`r20`: 20 random bits).  Below 2^-6 the
-// grid's step is 2^-9, as in the binade above: there 2^-6 is added before and taken off after.
-__device__ __forceinline__ float round_e4m3(float x, float scale, uint32_t r20) {
-  const float y = fabsf(x) * scale;
-  const float low = y < 0x1p-6f ? 0x1p-6f : 0.f;
-  float z = __uint_as_float((__float_as_uint(y + low) + r20) & 0xfff00000u) - low;
-  z = y < 256.f ? z : __uint_as_float(0x7fc00000u);
-  return copysignf(z, x);
-}
-
-__device__ __forceinline__ void encode8(void* codes, int64_t i, int64_t n, bool vec, int exponent, const float (&x)[8], const uint32_t (&r20)[8]) {
-  const float scale = __uint_as_float((uint32_t)(134 - exponent) << 23);   // 2^(7 - exponent)
-  uint32_t w[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float z[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) z[k] = round_e4m3(x[4 * h + k], scale, r20[4 * h + k]);
-    int c = __builtin_amdgcn_cvt_pk_fp8_f32(z[0], z[1], 0, false);
-    w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(z[2], z[3], c, true);
-  }
+__device__ __forceinline__ void put8(void* codes, int64_t i, int64_t n, bool vec, const int (&w)[2]) {
   uint8_t* c = (uint8_t*)codes;
   if (vec && i + 8 <= n) {
-    *reinterpret_cast<uint2*>(c + i) = make_uint2(w[0], w[1]);
+    *reinterpret_cast<int2*>(c + i) = make_int2(w[0], w[1]);
   } else {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (i + k < n) c[i + k] = (uint8_t)(w[k >> 2] >> (8 * (k & 3)));
+      if (i + k < n) c[i + k] = (uint8_t)((uint32_t)w[k >> 2] >> (8 * (k & 3)));
   }
 }
 
+// What bounds this kernel is issue slots as much as HBM: at 16 (fp32) or 10 bytes (bf16 parameters) an element the memory leaves about 105 or 65
+// slots for one.  Hence v_cvt_sr_fp8_f32, which is the rounding that the states are defined with (16 random bits on top of the ones it takes),
+// v_rsq and v_rcp in place of the library's root and quotient, and the first product of the mixing function from its neighbour's: the eight
+// arguments of a lane differ in three bits, so their products differ by +-1, +-2, +-4 times the factor.
 template <typename T>
 __global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable B, AdamwArgs a) {
   const int s = adamw_find(B);
-  const vc_adamw_tensor& S = B.t[s];
-  const int64_t n = S.n, i = (int64_t)(blockIdx.x - B.block0[s]) * kAdamwChunk + threadIdx.x * 8;
+  const AdamwTensor& S = B.t[s];
+  const int64_t n = (int64_t)(S.n_place & ((1ull << 44) - 1)), i = (int64_t)(blockIdx.x - B.block0[s]) * kAdamwChunk + threadIdx.x * 8;
   // 16 lanes share an exponent, and all 16 are here for the maximum: the lanes behind the last element carry zeros
-  const bool vec = S.vec_;
+  const bool vec = B.vec >> s & 1;
   const int64_t blk = i / kStateBlock;
   const bool live = blk * kStateBlock < n;
-  const int8_t* e = S.exponents + 2 * blk;
   float p[8], g[8], m[8], r[8];
   load8((const T*)S.grad, i, n, vec, g);
   load8((const T*)S.param, i, n, vec, p);
-  decode8(S.exp_avg, i, n, vec, live ? e[0] : 0, m);
-  decode8(S.exp_avg_sq, i, n, vec, live ? e[1] : 0, r);
-  uint32_t mtop = 0, rtop = 0, random[8], r20[8];
+  const int8_t em0 = live ? S.exponents[2 * blk] : 0, er0 = live ? S.exponents[2 * blk + 1] : 0;
+  decode8(S.exp_avg, i, n, vec, em0, m);
+  decode8(S.exp_avg_sq, i, n, vec, er0, r);
+  uint32_t mtop = 0, vtop = 0;
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
     m[k] = m[k] * a.beta1 + g[k] * a.one_minus_beta1;
     const float v = r[k] * r[k] * a.beta2 + g[k] * g[k] * a.one_minus_beta2;
-    r[k] = sqrtf(v);
-    p[k] = p[k] * a.keep - a.step_size * (m[k] / (r[k] * a.inv_bc2_sqrt + a.eps));
-    mtop = max(mtop, finite_bits(m[k]));
-    rtop = max(rtop, finite_bits(r[k]));
-    const uint64_t at = (uint64_t)(i + k);
-    random[k] = mix32(S.key ^ (uint32_t)at ^ (uint32_t)(at >> 32) * 0x9e3779b9u);
+    r[k] = root(v);
+    p[k] = p[k] * a.keep - a.step_size * (m[k] * __builtin_amdgcn_rcpf(r[k] * a.inv_bc2_sqrt + a.eps));
+    mtop = max(mtop, __float_as_uint(m[k]) & 0x7fffffffu);
+    vtop = max(vtop, __float_as_uint(v));
   }
   store8((T*)S.param, i, n, vec, p);
-  const int em = max((int)(max16(mtop) >> 23) - 127, -119), er = max((int)(max16(rtop) >> 23) - 127, -119);
+  if (max(mtop, vtop) >= 0x7f800000u) {   // something infinite or undefined: it has no part in the block's exponents
+    mtop = vtop = 0;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) r20[k] = (random[k] & 0xffffu) << 4;
-  encode8(S.exp_avg, i, n, vec, em, m, r20);
+    for (int k = 0; k < 8; ++k) {
+      mtop = max(mtop, finite_bits(__float_as_uint(m[k]) & 0x7fffffffu));
+      vtop = max(vtop, finite_bits(__float_as_uint(r[k] * r[k])));
+    }
+  }
+  // the root's exponent is half of v's, whatever the root's last bit
+  mtop = max16(mtop);
+  vtop = max16(vtop);
+  const int em = max((int)(mtop >> 23) - 127, -119), er = vtop ? ((int)(vtop >> 23) - 127) >> 1 : -119;
+  const float mscale = __uint_as_float((uint32_t)(134 - em) << 23), rscale = __uint_as_float((uint32_t)(134 - er) << 23);   // 2^(7 - e)
+  constexpr uint32_t kFirst = 0x85ebca6bu, kSecond = 0xc2b2ae35u;
+  uint32_t x0 = mix32(a.key + (uint32_t)(S.n_place >> 44)) ^ (uint32_t)i ^ (uint32_t)(i >> 32) * 0x9e3779b9u;
+  x0 ^= x0 >> 16;     // (i is a multiple of 8: the element's three bits come in unshifted)
+  const uint32_t p0 = x0 * kFirst, d1 = x0 & 1 ? 0u - kFirst : kFirst, d2 = x0 & 2 ? 0u - 2 * kFirst : 2 * kFirst,
+                 d4 = x0 & 4 ? 0u - 4 * kFirst : 4 * kFirst;
+  int wm[2] = {0, 0}, wr[2] = {0, 0};
 #pragma unroll
-  for (int k = 0; k < 8; ++k) r20[k] = (random[k] >> 16) << 4;
-  encode8(S.exp_avg_sq, i, n, vec, er, r, r20);
+  for (int k = 0; k < 8; ++k) {
+    uint32_t x = p0 + (k & 1 ? d1 : 0u) + (k & 2 ? d2 : 0u) + (k & 4 ? d4 : 0u);
+    x ^= x >> 13;
+    x *= kSecond;
+    const float ym = m[k] * mscale, yr = r[k] * rscale;
+    const int bm = (int)((x ^ (x >> 16)) << 16), br = (int)(x & 0xffff0000u);   // the low and the high half of x ^ (x >> 16), each on top
+    switch (k & 3) {
+      case 0: wm[k >> 2] = __builtin_amdgcn_cvt_sr_fp8_f32(ym, bm, wm[k >> 2], 0); wr[k >> 2] = __builtin_amdgcn_cvt_sr_fp8_f32(yr, br, wr[k >> 2], 0); break;
+      case 1: wm[k >> 2] = __builtin_amdgcn_cvt_sr_fp8_f32(ym, bm, wm[k >> 2], 1); wr[k >> 2] = __builtin_amdgcn_cvt_sr_fp8_f32(yr, br, wr[k >> 2], 1); break;
+      case 2: wm[k >> 2] = __builtin_amdgcn_cvt_sr_fp8_f32(ym, bm, wm[k >> 2], 2); wr[k >> 2] = __builtin_amdgcn_cvt_sr_fp8_f32(yr, br, wr[k >> 2], 2); break;
+      default: wm[k >> 2] = __builtin_amdgcn_cvt_sr_fp8_f32(ym, bm, wm[k >> 2], 3); wr[k >> 2] = __builtin_amdgcn_cvt_sr_fp8_f32(yr, br, wr[k >> 2], 3);
+    }
+  }
+  put8(S.exp_avg, i, n, vec, wm);
+  put8(S.exp_avg_sq, i, n, vec, wr);
   if (live && (threadIdx.x & 15) == 0) {
     S.exponents[2 * blk] = (int8_t)em;
     S.exponents[2 * blk + 1] = (int8_t)er;
   }
-}
-
-static uint32_t host_mix32(uint32_t x) {
-  x ^= x >> 16; x *= 0x85ebca6bu; x ^= x >> 13; x *= 0xc2b2ae35u; x ^= x >> 16;
-  return x;
 }
 
 struct Span {
@@ -246,7 +266,7 @@ int vc_adamw(const vc_adamw_tensor* tensors, int64_t n_tensors, int dtype, int s
   VC_REQUIRE(step >= 1, "vc_adamw: step = %lld (the first step is 1)", (long long)step);
   VC_REQUIRE(beta1 >= 0. && beta1 < 1. && beta2 >= 0. && beta2 < 1., "vc_adamw: betas (%g, %g) outside [0, 1)", beta1, beta2);
   const int64_t psize = dtype == VC_F32 ? 4 : 2, ssize = state_bits / 8;
-  const uintptr_t pmask = psize == 4 ? 15 : 15, smask = ssize == 4 ? 15 : 7;
+  const uintptr_t smask = ssize == 4 ? 15 : 7;
   hipStream_t st = (hipStream_t)stream;
   // what is written must not overlap: two blocks would race on it
   Span stack[256];
@@ -259,7 +279,8 @@ int vc_adamw(const vc_adamw_tensor* tensors, int64_t n_tensors, int dtype, int s
   size_t n_spans = 0;
   for (int64_t k = 0; k < n_tensors; ++k) {
     const vc_adamw_tensor& T = tensors[k];
-    VC_REQUIRE(T.n >= 0, "vc_adamw: tensor %lld has n = %lld", (long long)k, (long long)T.n);
+    VC_REQUIRE(T.n >= 0 && T.n < (1LL << 30) * kAdamwChunk, "vc_adamw: tensor %lld has n = %lld", (long long)k, (long long)T.n);
+    VC_REQUIRE(T.key < (1u << 20), "vc_adamw: tensor %lld has the place %u (at most 2^20 tensors)", (long long)k, T.key);
     if (T.n == 0) continue;
     VC_REQUIRE(T.param && T.grad && T.exp_avg && T.exp_avg_sq && (state_bits == 32 || T.exponents), "vc_adamw: tensor %lld has a NULL pointer", (long long)k);
     VC_REQUIRE((((uintptr_t)T.param | (uintptr_t)T.grad) & (psize - 1)) == 0 && (((uintptr_t)T.exp_avg | (uintptr_t)T.exp_avg_sq) & (ssize - 1)) == 0,
@@ -278,26 +299,24 @@ int vc_adamw(const vc_adamw_tensor* tensors, int64_t n_tensors, int dtype, int s
   a.keep = (float)(1.0 - lr * weight_decay);
   a.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
   a.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
-  const uint32_t key = host_mix32(host_mix32(seed) + (uint32_t)step);
+  a.key = mix32(mix32(seed) + (uint32_t)step);
   AdamwTable B;
   int64_t k = 0;
   while (k < n_tensors) {
     B.n = 0;
+    B.vec = 0;
     unsigned blocks = 0;
     for (; k < n_tensors && B.n < kAdamwTensors; ++k) {
-      if (tensors[k].n == 0) continue;
-      const int64_t need = cdiv(tensors[k].n, kAdamwChunk);
-      VC_REQUIRE(need < (1LL << 30), "vc_adamw: tensor %lld has %lld elements", (long long)k, (long long)tensors[k].n);
+      const vc_adamw_tensor& T = tensors[k];
+      if (T.n == 0) continue;
+      const int64_t need = cdiv(T.n, kAdamwChunk);
       if (B.n && (int64_t)blocks + need >= (1LL << 30)) break;
-      vc_adamw_tensor& T = B.t[B.n];
-      T = tensors[k];
-      T.vec_ = ((((uintptr_t)T.param | (uintptr_t)T.grad) & pmask) | (((uintptr_t)T.exp_avg | (uintptr_t)T.exp_avg_sq) & smask)) == 0;
-      T.key = host_mix32(key + T.key);
+      B.t[B.n] = {T.param, T.grad, T.exp_avg, T.exp_avg_sq, T.exponents, (uint64_t)T.n | (uint64_t)T.key << 44};
+      if (((((uintptr_t)T.param | (uintptr_t)T.grad) & 15) | (((uintptr_t)T.exp_avg | (uintptr_t)T.exp_avg_sq) & smask)) == 0) B.vec |= 1ull << B.n;
       B.block0[B.n++] = blocks;
       blocks += (unsigned)need;
     }
     if (B.n == 0) break;
-    B.block0[B.n] = blocks;
 #define VC_ADAMW_LAUNCH(T)                                                                                              \
   if (state_bits == 32) hipLaunchKernelGGL(adamw32_kernel<T>, dim3(blocks), dim3(256), 0, st, B, a);                    \
   else hipLaunchKernelGGL(adamw8_kernel<T>, dim3(blocks), dim3(256), 0, st, B, a)
