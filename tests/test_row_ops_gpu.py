@@ -257,6 +257,18 @@ def test_grouped_linear_long_groups(hip_backend, dtype, ends):
                   rnd((n, 40), 4, dtype, 0.1))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("inner,outer", [(64, 8192), (136, 4104), (1064, 2056), (2056, 1064)])
+def test_grouped_linear_large_tiles(hip_backend, inner, outer, dtype):
+    # enough aligned work for the large tiles in at least one direction: whole and partial tiles, whole and partial last steps, short and empty groups
+    ends = [3, 3, 1030, 1031, 2311, 2700, 2703]
+    if inner < 200:
+        ends = [e * 3 for e in ends]
+    n, groups = ends[-1] + 5, len(ends) - 1
+    check_grouped(rnd((n, inner), 1, dtype), rnd((groups, outer, inner), 2, dtype, inner ** -0.5), ends, rnd((groups, outer), 3, dtype),
+                  rnd((n, outer), 4, dtype, 0.1))
+
+
 def test_grouped_linear_many_groups(hip_backend):
     g = torch.Generator().manual_seed(3)
     sizes = torch.randint(0, 9, (200,), generator=g)

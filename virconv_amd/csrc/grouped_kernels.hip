@@ -15,6 +15,8 @@
 // [0, rows]; one that is not is cut to it, so no content of `offsets` leads out of the tensors.  Rows of no group come out as zeros.
 #include "common.h"
 
+#include <initializer_list>
+
 namespace vc {
 
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -37,58 +39,89 @@ struct GroupArgs {
   int64_t rows;
   int groups, off64, m, n, k;   // m: weight product only
   int ntiles, mtiles, splits, per_split;
-  unsigned total;
 };
 
-__device__ __forceinline__ int64_t offset_at(const GroupArgs& a, int g) {
+// ------------------------------------------------------------------------------------------------ the groups
+__device__ __forceinline__ int offset_at(const GroupArgs& a, int g) {   // (rows < 2^31)
   const int64_t o = a.off64 ? ((const int64_t*)a.offsets)[g] : (int64_t)((const int32_t*)a.offsets)[g];
-  return o < 0 ? 0 : o > a.rows ? a.rows : o;
+  return o < 0 ? 0 : o > a.rows ? (int)a.rows : (int)o;
 }
 
-__device__ __forceinline__ int64_t shfl_up64(int64_t x, int d) {
-  int lo = __shfl_up((int)(uint32_t)x, d, 64), hi = __shfl_up((int)(x >> 32), d, 64);
-  return ((int64_t)hi << 32) | (uint32_t)lo;
+// inclusive scans over the 64 lanes, of values >= 0: shifts within a row of 16, then the rows' last lanes handed on
+template <int CTRL, int ROWS> __device__ __forceinline__ int moved(int x) { return __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false); }
+__device__ __forceinline__ int scan_add(int x) {
+  x += moved<0x111, 0xf>(x); x += moved<0x112, 0xf>(x); x += moved<0x114, 0xf>(x); x += moved<0x118, 0xf>(x);
+  x += moved<0x142, 0xa>(x); x += moved<0x143, 0xc>(x);
+  return x;
 }
-__device__ __forceinline__ int64_t shfl64(int64_t x, int l) {
-  int lo = __shfl((int)(uint32_t)x, l, 64), hi = __shfl((int)(x >> 32), l, 64);
-  return ((int64_t)hi << 32) | (uint32_t)lo;
+__device__ __forceinline__ int scan_max(int x) {
+  x = max(x, moved<0x111, 0xf>(x)); x = max(x, moved<0x112, 0xf>(x)); x = max(x, moved<0x114, 0xf>(x)); x = max(x, moved<0x118, 0xf>(x));
+  x = max(x, moved<0x142, 0xa>(x)); x = max(x, moved<0x143, 0xc>(x));
+  return x;
 }
 
-// Tile `target` of the groups' tiles of `per` rows, group after group: its group, the group's rows and the tile's number within it.
-// group = groups: behind the groups' tiles; `target` is then what is left of it, [begin, end) the rows behind the last group.
-// Every wave of the block runs it for itself.
-struct Place { int group; int64_t begin, end, first_row; unsigned tile; };
-__device__ __forceinline__ Place find_tile(const GroupArgs& a, int64_t per, unsigned target) {
-  const int lane = threadIdx.x & 63;
-  int64_t high = 0, first_row = 0;      // rows handed out so far (the running maximum of the offsets), the first group's begin
-  for (int g0 = 0; g0 < a.groups; g0 += 64) {
-    const int g = g0 + lane;
-    int64_t end = g < a.groups ? offset_at(a, g + 1) : 0;
-    if (g0 == 0) first_row = high = offset_at(a, 0);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const int64_t o = shfl_up64(end, d); if (lane >= d && o > end) end = o; }
-    if (end < high) end = high;
-    int64_t begin = shfl_up64(end, 1);
-    if (lane == 0) begin = high;
-    unsigned tiles = g < a.groups ? (unsigned)((end - begin + per - 1) / per) : 0u, upto = tiles;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const unsigned o = __shfl_up(upto, d, 64); if (lane >= d) upto += o; }
-    const uint64_t hit = __ballot(target < upto);
-    if (hit) {
-      const int l = __builtin_ctzll(hit);
-      Place p;
-      p.group = g0 + l;
-      p.begin = shfl64(begin, l);
-      p.end = shfl64(end, l);
-      p.first_row = first_row;
-      p.tile = target - (__shfl(upto, l, 64) - __shfl(tiles, l, 64));
-      return p;
-    }
-    target -= __shfl(upto, 63, 64);
-    high = shfl64(end, 63);
+struct Place { int group, begin, end, tile; };   // group = groups: none
+
+// The groups as a wave sees them, 64 at a time, one a lane: their rows (the offsets as a rising sequence), their tiles of `per` rows and the
+// running count of those.  Every wave of a block holds them for itself; up to 64 groups they are read once.
+struct Groups {
+  int begin, end, tiles, upto;        // the lane's group
+  int first_row, last_end, total;     // rows in front of the groups, the groups' last end, their tiles
+
+  __device__ __forceinline__ void load(const GroupArgs& a, int per, int g0, int high) {
+    const int g = g0 + (threadIdx.x & 63);
+    end = max(scan_max(g < a.groups ? offset_at(a, g + 1) : 0), high);
+    begin = __builtin_amdgcn_update_dpp(high, end, 0x138, 0xf, 0xf, false);   // the neighbour's end
+    tiles = g < a.groups ? (int)(((int64_t)end - begin + per - 1) / per) : 0;
+    upto = scan_add(tiles);
   }
-  return {a.groups, high, a.rows, first_row, target};
-}
+  __device__ __forceinline__ Groups(const GroupArgs& a, int per) {
+    begin = end = tiles = upto = first_row = last_end = total = 0;
+    for (int g0 = 0; g0 < a.groups; g0 += 64) {
+      if (g0 == 0) first_row = last_end = offset_at(a, 0);
+      load(a, per, g0, last_end);
+      total += __builtin_amdgcn_readlane(upto, 63);
+      last_end = __builtin_amdgcn_readlane(end, 63);
+    }
+    first_row = __builtin_amdgcn_readfirstlane(first_row);
+  }
+  // the group of tile `target` (of the groups' tiles, `times` of them counted for one), and the tile's number in it
+  __device__ __forceinline__ Place of_tile(const GroupArgs& a, int per, unsigned target, unsigned times) {
+    int high = first_row;
+    for (int g0 = 0; g0 < a.groups; g0 += 64) {
+      if (a.groups > 64) load(a, per, g0, high);
+      const uint64_t hit = __ballot(target < (unsigned)upto * times);
+      if (hit) {
+        const int l = __builtin_ctzll(hit);
+        const unsigned before = (unsigned)(__builtin_amdgcn_readlane(upto, l) - __builtin_amdgcn_readlane(tiles, l)) * times;
+        return {g0 + l, __builtin_amdgcn_readlane(begin, l), __builtin_amdgcn_readlane(end, l), (int)(target - before)};
+      }
+      target -= (unsigned)__builtin_amdgcn_readlane(upto, 63) * times;
+      high = __builtin_amdgcn_readlane(end, 63);
+    }
+    return {a.groups, 0, 0, (int)target};
+  }
+  // the group with the r-th most rows (up to 64 groups; above, group r)
+  __device__ __forceinline__ Place of_rank(const GroupArgs& a, int per, int r) {
+    if (a.groups > 64) {
+      int high = first_row;
+      for (int g0 = 0; g0 < a.groups; g0 += 64) {
+        load(a, per, g0, high);
+        if (r < g0 + 64) return {r, __builtin_amdgcn_readlane(begin, r - g0), __builtin_amdgcn_readlane(end, r - g0), 0};
+        high = __builtin_amdgcn_readlane(end, 63);
+      }
+    }
+    const int lane = threadIdx.x & 63, size = end - begin;
+    int rank = 0;
+    for (int g = 0; g < a.groups; ++g) {
+      const int other = __builtin_amdgcn_readlane(size, g);
+      rank += other > size || (other == size && g < lane);
+    }
+    const uint64_t hit = __ballot(rank == r && lane < a.groups);
+    const int l = hit ? __builtin_ctzll(hit) : 0;
+    return {l, __builtin_amdgcn_readlane(begin, l), __builtin_amdgcn_readlane(end, l), 0};
+  }
+};
 
 // ------------------------------------------------------------------------------------------------ operands
 template <typename T> struct OperandOf { static constexpr int planes = 1, bk = 64; typedef T type; };
@@ -103,9 +136,15 @@ __device__ __forceinline__ void load8(const T* p, int valid, T (&out)[8]) {   //
     __builtin_memcpy(&e, p, sizeof(e));
 #pragma unroll
     for (int i = 0; i < 8; ++i) out[i] = e.v[i];
+  } else if (valid > 0) {   // eight loads side by side: the missing ones read the last element that there is
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = p[i < valid ? i : valid - 1];
+#pragma unroll
+    for (int i = 1; i < 8; ++i)
+      if (i >= valid) out[i] = (T)0.f;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) out[i] = i < valid ? p[i] : (T)0.f;
+    for (int i = 0; i < 8; ++i) out[i] = (T)0.f;
   }
 }
 
@@ -139,11 +178,11 @@ __device__ __forceinline__ void stage8(char* lds, int plane_bytes, int at, const
 }
 
 // A tile of one operand in LDS.  ALONG: [rows][BK], pieces of 8 along the summed axis; else [BK][cols], pieces of 8 across it.
-template <typename T, int ROWS, bool ALONG>
+template <typename T, int ROWS, bool ALONG, int THREADS = 256>
 struct Tile {
   static constexpr int BK = OperandOf<T>::bk, planes = OperandOf<T>::planes;
   static constexpr int plane_bytes = ROWS * BK * 2, bytes = plane_bytes * planes;
-  static constexpr int pieces = ROWS * BK / 8, per_thread = (pieces + 255) / 256;
+  static constexpr int pieces = ROWS * BK / 8, per_thread = (pieces + THREADS - 1) / THREADS;
 
   static __device__ __forceinline__ int place(int r, int k) {   // byte of element (row r, summed index k); r or k a multiple of 8
     if constexpr (ALONG) {
@@ -162,8 +201,8 @@ struct Tile {
   __device__ __forceinline__ void fetch(const T* p, int64_t ld, int rows, int depth) {
 #pragma unroll
     for (int i = 0; i < per_thread; ++i) {
-      const int q = i * 256 + threadIdx.x;
-      if (pieces % 256 && q >= pieces) continue;
+      const int q = i * THREADS + threadIdx.x;
+      if (pieces % THREADS && q >= pieces) continue;
       int valid;
       const T* s;
       if constexpr (ALONG) {
@@ -181,14 +220,43 @@ struct Tile {
   __device__ __forceinline__ void put(char* lds) {
 #pragma unroll
     for (int i = 0; i < per_thread; ++i) {
-      const int q = i * 256 + threadIdx.x;
-      if (pieces % 256 && q >= pieces) continue;
+      const int q = i * THREADS + threadIdx.x;
+      if (pieces % THREADS && q >= pieces) continue;
       int at;
       if constexpr (ALONG) at = place(q / (BK / 8), (q % (BK / 8)) * 8);
       else at = place((q % (ROWS / 8)) * 8, q / (ROWS / 8));
       stage8(lds, plane_bytes, at, reg[i]);
     }
   }
+  // The tile straight from memory into LDS, 16 bytes a lane (16-bit operands whose pieces are all aligned): the order of the lanes' pieces in
+  // LDS is given, so a lane reads the piece that belongs at its place.  Rows that are not there read one that is: they only enter results that
+  // are not written.  Every summed index of the tile has to exist.
+  // `from`: the byte offsets of the lane's pieces in the tensor's tile, to be made once per tile (256 rows of up to 2^22 elements: 32 bits).
+  static __device__ __forceinline__ void offsets(uint32_t (&from)[per_thread], int64_t ld, int rows) {
+#pragma unroll
+    for (int i = 0; i < per_thread; ++i) {
+      const int q = i * THREADS + threadIdx.x;
+      if constexpr (ALONG) {
+        constexpr int CH = BK / 8, R = 16 / CH;
+        const int r = q / CH, k = ((q ^ (r / R)) & (CH - 1)) * 8;
+        from[i] = ((uint32_t)min(r, rows - 1) * (uint32_t)ld + k) * 2;
+      } else {
+        const int k = q / (ROWS / 8), c0 = (q % (ROWS / 8)) * 8;
+        const int f = (k & 3) | ((k >> 1) & 4), c = ((((c0 >> 4) ^ f) & (ROWS / 16 - 1)) << 4) | (c0 & 8);
+        from[i] = ((uint32_t)k * (uint32_t)ld + (c < rows ? c : 0)) * 2;
+      }
+    }
+  }
+  static __device__ __forceinline__ void copy(char* lds, const T* p, const uint32_t (&from)[per_thread]) {
+    static_assert(pieces % THREADS == 0 && planes == 1, "whole waves of pieces");
+    typedef __attribute__((address_space(1))) const void global_void;
+    typedef __attribute__((address_space(3))) void lds_void;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < per_thread; ++i)
+      __builtin_amdgcn_global_load_lds((global_void*)((const char*)p + from[i]), (lds_void*)(lds + (i * THREADS + wave * 64) * 16), 16, 0, 0);
+  }
+
   // The 16 rows from r0 on (a multiple of 16), 32 summed indices from k0 on (a multiple of 32), as an operand of v_mfma_f32_16x16x32: lane l
   // holds row l % 16, the eight indices from 8 (l / 16) on.  `lane_place` is the lane's part of the address, to be made once per tile row.
   static __device__ __forceinline__ int lane_place(int r0) {
@@ -217,16 +285,12 @@ __device__ __forceinline__ v4f mfma(v8s a, v8s b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
+// Ones in row i of a 16-row operand, zeros in the others: its product with an operand adds that one up along the summed axis, into row i of an
+// accumulator that the sums of sixteen operands fit in.
 template <typename T>
-__device__ __forceinline__ v8s ones() {
-  const short one = __is_same(T, _Float16) ? (short)0x3c00 : (short)0x3f80;
+__device__ __forceinline__ v8s ones_in_row(int i) {
+  const short one = (threadIdx.x & 15) != (unsigned)i ? (short)0 : __is_same(T, _Float16) ? (short)0x3c00 : (short)0x3f80;
   return v8s{one, one, one, one, one, one, one, one};
-}
-
-// blocks of one XCD (consecutive blocks go to the eight XCDs in turn) take consecutive tiles: neighbours share an operand in its L2
-__device__ __forceinline__ unsigned xcd_order(unsigned b, unsigned total) {
-  const unsigned per = total / 8, rest = total % 8, x = b % 8, i = b / 8;
-  return x * per + (x < rest ? x : rest) + i;
 }
 
 template <typename T> __device__ __forceinline__ void store4(T* p, int valid, const float (&x)[4]) {
@@ -242,7 +306,157 @@ template <typename T> __device__ __forceinline__ void store4(T* p, int valid, co
   }
 }
 
-// ------------------------------------------------------------------------------------------------ the kernel
+// ------------------------------------------------------------------------------------------------ tiles of a block
+// What a block computes: where its operands begin, how much of them there is, where its results go.
+template <typename T> struct Work {
+  const T *pa, *pb;
+  int64_t lda, ldb, m0;
+  int rows_a, rows_b, depth, group, n0;
+  unsigned piece;
+  float* partial;
+  bool none;
+};
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ int64_t uniform(int64_t x) { return (int64_t)(((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x)); }
+template <typename P> __device__ __forceinline__ P* uniform(P* p) { return (P*)uniform((int64_t)p); }
+template <typename T> __device__ __forceinline__ Work<T> uniform(const Work<T>& w) {   // into scalar registers
+  return {uniform(w.pa), uniform(w.pb), uniform(w.lda), uniform(w.ldb), uniform(w.m0), uniform(w.rows_a), uniform(w.rows_b), uniform(w.depth),
+          uniform(w.group), uniform(w.n0), (unsigned)uniform((int)w.piece), uniform(w.partial), (bool)uniform((int)w.none)};
+}
+
+// Consecutive blocks go to the eight XCDs in turn; the blocks of one XCD take neighbouring items, which share operands in its L2.
+//
+// Row products: the items are the tiles (x splits) that the groups really have, each XCD an eighth of them, within a group in bands of four
+// column tiles.  Weight products without splits: the groups by their size, the largest first (their tiles take longest), and each group's
+// tiles dealt out over all XCDs.
+struct Items {
+  unsigned count;      // of an XCD: the local items [0, count), item l of XCD x
+  unsigned first;      // row products: the XCD's first item
+};
+template <int MODE>
+__device__ __forceinline__ Items items_of(const GroupArgs& a, const Groups& g, int bm, unsigned x) {
+  if (MODE == kBackWeight && a.splits == 1) {
+    const unsigned tiles = (unsigned)a.mtiles * a.ntiles;
+    return {tiles >= 8 ? (tiles + 7) / 8 * a.groups : (tiles * a.groups + 7 - x) / 8, 0u};
+  }
+  unsigned all;
+  if (MODE == kBackWeight) all = (unsigned)g.total * a.mtiles * a.ntiles;
+  else all = (unsigned)(g.total + (g.first_row + bm - 1) / bm + (int)((a.rows - g.last_end + bm - 1) / bm)) * a.ntiles * a.splits;
+  const unsigned per = all / 8, rest = all % 8;
+  return {per + (x < rest ? 1u : 0u), x * per + (x < rest ? x : rest)};
+}
+
+template <typename T, int BM, int BN, int MODE, int THREADS>
+__device__ __forceinline__ Work<T> find_work(const GroupArgs& a, Groups& g, const Items& items, unsigned x, unsigned l) {
+  Work<T> w;
+  w.none = true;
+  w.partial = nullptr;
+  w.piece = 0;
+  if constexpr (MODE != kBackWeight) {
+    unsigned id = items.first + l;
+    const int split = (int)(id % a.splits);
+    id /= a.splits;
+    const Place at = g.of_tile(a, BM, id, a.ntiles);
+    if (at.group == a.groups) {   // rows of no group: in front of the first and behind the last
+      if (split) return w;
+      const int t = at.tile / a.ntiles, front_tiles = (g.first_row + BM - 1) / BM;
+      w.n0 = at.tile % a.ntiles * BN;
+      const int64_t lo = t < front_tiles ? (int64_t)t * BM : g.last_end + (int64_t)(t - front_tiles) * BM;
+      const int64_t hi = min(lo + BM, t < front_tiles ? (int64_t)g.first_row : a.rows);
+      for (int64_t e = threadIdx.x; lo < hi && e < (hi - lo) * BN; e += THREADS) {
+        const int n = w.n0 + (int)(e % BN);
+        if (n < a.n) ((T*)a.out)[(lo + e / BN) * a.n + n] = (T)0.f;
+      }
+      return w;
+    }
+    const int mtiles = (at.end - at.begin + BM - 1) / BM, band = at.tile / (4 * mtiles), wide = min(4, a.ntiles - 4 * band), in = at.tile - 4 * band * mtiles;
+    w.n0 = (4 * band + in % wide) * BN;
+    w.group = at.group;
+    w.m0 = at.begin + (int64_t)(in / wide) * BM;
+    const int k0 = split * a.per_split;
+    w.depth = min(a.per_split, a.k - k0);
+    w.rows_a = (int)min((int64_t)BM, at.end - w.m0);
+    w.lda = a.lda;
+    w.pa = (const T*)a.a + w.m0 * a.lda + k0;
+    const T* weights = (const T*)a.b + (int64_t)w.group * a.n * a.k;
+    w.ldb = MODE == kForward ? a.k : a.n;
+    w.pb = MODE == kForward ? weights + (int64_t)w.n0 * a.k + k0 : weights + (int64_t)k0 * a.n + w.n0;
+    if (a.splits > 1) w.partial = a.partial + ((int64_t)split * a.rows + w.m0) * a.n + w.n0;
+  } else {
+    const unsigned tiles = (unsigned)a.mtiles * a.ntiles;
+    unsigned t;
+    int64_t r0, r1;
+    if (a.splits > 1) {          // pieces of per_split rows, their sums added by grouped_weight_sum_kernel
+      const unsigned id = items.first + l;
+      t = id % tiles;
+      w.piece = id / tiles;
+      const Place at = g.of_tile(a, a.per_split, w.piece, 1);
+      if (at.group == a.groups) return w;
+      w.group = at.group;
+      r0 = at.begin + (int64_t)at.tile * a.per_split;
+      r1 = min(r0 + a.per_split, (int64_t)at.end);
+    } else {
+      const unsigned share = (tiles + 7) / 8;
+      const unsigned r = tiles >= 8 ? l / share : (l * 8 + x) / tiles;
+      t = tiles >= 8 ? x * share + l % share : (l * 8 + x) % tiles;
+      if (t >= tiles) return w;
+      const Place at = g.of_rank(a, a.per_split, (int)r);
+      w.group = at.group;
+      r0 = at.begin;
+      r1 = at.end;
+    }
+    w.n0 = (int)(t % a.ntiles) * BN;
+    w.m0 = (int64_t)(t / a.ntiles) * BM;
+    if (a.splits > 1) w.partial = a.partial + ((int64_t)w.piece * a.m + w.m0) * a.n + w.n0;
+    w.depth = (int)(r1 - r0);
+    w.rows_a = (int)min((int64_t)BM, (int64_t)a.m - w.m0);
+    w.lda = a.lda;
+    w.ldb = a.ldb;
+    w.pa = (const T*)a.a + r0 * a.lda + w.m0;
+    w.pb = (const T*)a.b + r0 * a.ldb + w.n0;
+  }
+  w.rows_b = min(BN, a.n - w.n0);
+  w.none = false;
+  return w;
+}
+
+// Results of a wave: lane l holds row m = l % 16 and the columns n = 4 (l / 16) .. + 3 of each 16 x 16 tile; (wm0, wn0): the wave's place.
+template <typename T, int FM, int FN, int MODE>
+__device__ __forceinline__ void write_results(const GroupArgs& a, const Work<T>& w, int wm0, int wn0, const v4f (&acc)[FM][FN], const v4f& accb, bool sum_bias) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = wm0 + i * 16 + (lane & 15);
+    if (m >= w.rows_a) continue;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+      const int n = wn0 + j * 16 + (lane >> 4) * 4;
+      if (n >= w.rows_b) continue;
+      float r[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+      if (w.partial) {
+        store4(w.partial + (int64_t)m * a.n + n, w.rows_b - n, r);
+        continue;
+      }
+      if (MODE == kForward && a.bias) {
+        const T* bias = (const T*)a.bias + (int64_t)w.group * a.n + w.n0 + n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n + e < w.rows_b) r[e] += (float)bias[e];
+      }
+      T* out = (T*)a.out;
+      if constexpr (MODE == kBackWeight) out += ((int64_t)w.group * a.m + w.m0 + m) * a.n + w.n0 + n;
+      else out += (w.m0 + m) * a.n + w.n0 + n;
+      store4(out, w.rows_b - n, r);
+    }
+    if (MODE == kBackWeight && sum_bias && lane >> 4 == i >> 2) {
+      if (w.partial) a.partial_bias[(int64_t)w.piece * a.m + w.m0 + m] = accb[i & 3];
+      else ((T*)a.dbias)[(int64_t)w.group * a.m + w.m0 + m] = (T)accb[i & 3];
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ the kernel for every case
 template <typename T, int BM, int BN, int MODE>
 __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
   typedef typename OperandOf<T>::type O;
@@ -254,86 +468,24 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
   __shared__ __align__(16) char lds[TileA::bytes + TileB::bytes];
   char* const la = lds;
   char* const lb = lds + TileA::bytes;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+  const int wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
 
-  unsigned id = xcd_order(blockIdx.x, a.total);
-  const T *pa, *pb;
-  int rows_a, rows_b, depth, group;
-  int64_t m0, mend;
-  int n0, split = 0;
-  float* partial = nullptr;
-  if constexpr (MODE != kBackWeight) {
-    n0 = (int)(id % a.ntiles) * BN;
-    id /= a.ntiles;
-    split = (int)(id % a.splits);
-    const Place w = find_tile(a, BM, id / a.splits);
-    if (w.group == a.groups) {   // rows of no group: in front of the first and behind the last
-      if (split) return;
-      int64_t r = (int64_t)w.tile * BM, front = w.first_row;
-      const int64_t front_tiles = (front + BM - 1) / BM;
-      const int64_t lo = (int64_t)w.tile < front_tiles ? r : w.begin + (r - front_tiles * BM);
-      const int64_t hi = min(lo + BM, (int64_t)w.tile < front_tiles ? front : a.rows);
-      for (int64_t e = threadIdx.x; lo < hi && e < (hi - lo) * BN; e += 256) {
-        const int n = n0 + (int)(e % BN);
-        if (n < a.n) ((T*)a.out)[(lo + e / BN) * a.n + n] = (T)0.f;
-      }
-      return;
-    }
-    group = w.group;
-    m0 = w.begin + (int64_t)w.tile * BM;
-    mend = w.end;
-    const int k0 = split * a.per_split;
-    depth = min(a.per_split, a.k - k0);
-    rows_a = (int)min((int64_t)BM, mend - m0);
-    rows_b = min(BN, a.n - n0);
-    pa = (const T*)a.a + m0 * a.lda + k0;
-    const T* weights = (const T*)a.b + (int64_t)group * a.n * a.k;
-    if constexpr (MODE == kForward) pb = weights + (int64_t)n0 * a.k + k0;
-    else pb = weights + (int64_t)k0 * a.n + n0;
-    if (a.splits > 1) partial = a.partial + ((int64_t)split * a.rows + m0) * a.n + n0;
-  } else {
-    n0 = (int)(id % a.ntiles) * BN;
-    id /= a.ntiles;
-    m0 = (int64_t)(id % a.mtiles) * BM;
-    mend = a.m;
-    id /= a.mtiles;
-    int64_t r0, r1;
-    if (a.splits > 1) {          // pieces of per_split rows, their sums added by grouped_weight_sum_kernel
-      const Place w = find_tile(a, a.per_split, id);
-      if (w.group == a.groups) return;
-      group = w.group;
-      r0 = w.begin + (int64_t)w.tile * a.per_split;
-      r1 = min(r0 + a.per_split, w.end);
-      partial = a.partial + ((int64_t)id * a.m + m0) * a.n + n0;
-    } else {
-      group = (int)id;
-      r0 = r1 = 0;
-      // the group's rows: the running maximum of the offsets up to it
-      for (int g0 = 0; g0 <= group; g0 += 64) {
-        const int g = g0 + lane;
-        int64_t o = g <= group ? offset_at(a, g) : 0;
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1) { const int64_t q = shfl64(o, lane ^ d); if (q > o) o = q; }
-        if (o > r0) r0 = o;
-      }
-      r1 = max(offset_at(a, group + 1), r0);
-    }
-    depth = (int)(r1 - r0);
-    rows_a = (int)min((int64_t)BM, (int64_t)a.m - m0);
-    rows_b = min(BN, a.n - n0);
-    pa = (const T*)a.a + r0 * a.lda + m0;
-    pb = (const T*)a.b + r0 * a.ldb + n0;
-  }
-  const int64_t lda = a.lda, ldb = MODE == kForward ? a.k : MODE == kBackInput ? a.n : a.ldb;
-  const bool sum_bias = MODE == kBackWeight && a.dbias && n0 == 0 && wn == 0;
+  Groups groups(a, MODE == kBackWeight ? a.per_split : BM);
+  const unsigned xcd = blockIdx.x % 8, item = blockIdx.x / 8;
+  const Items items = items_of<MODE>(a, groups, BM, xcd);
+  if (item >= items.count) return;
+  const Work<T> w = find_work<T, BM, BN, MODE, 256>(a, groups, items, xcd, item);
+  if (w.none) return;
+  const T *const pa = w.pa, *const pb = w.pb;
+  const int64_t lda = w.lda, ldb = w.ldb;
+  const int rows_a = w.rows_a, rows_b = w.rows_b, depth = w.depth;
+  const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && wn == 0;
 
-  v4f acc[FM][FN], accb[FM];
+  v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    accb[i] = v4f{0.f, 0.f, 0.f, 0.f};
+  for (int i = 0; i < FM; ++i)
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-  }
   int at_a[FM], at_b[FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i) at_a[i] = TileA::lane_place(wm * (BM / WM) + i * 16);
@@ -379,41 +531,112 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
         }
         if (MODE == kBackWeight && sum_bias) {
 #pragma unroll
-          for (int q = P - 1; q >= 0; --q) accb[i] = mfma<O>(ones<O>(), fa[q], accb[i]);
+          for (int q = P - 1; q >= 0; --q) accb = mfma<O>(ones_in_row<O>(i), fa[q], accb);
         }
       }
     }
   }
 
-  // results: lane l holds row m = l % 16 and the columns n = 4 (l / 16) .. + 3 of each 16 x 16 tile
+  write_results<T, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc, accb, sum_bias);
+}
+
+// ------------------------------------------------------------------------------------------------ large tiles of aligned 16-bit operands
+// 256 x 256 results a block of eight waves, 128 x 64 a wave: of the tiles that registers allow the one whose fragment reads (24 KB a wave and
+// step of 64) stay below what its products take (a 128 x 128 tile of four waves keeps LDS exactly as busy as the matrix units and reached 570
+// TFLOP/s).  The next step's operands come by LDS-direct loads into the other buffer while this one is multiplied: no registers, one barrier a
+// step.  What is left of the summed axis behind the last whole step goes through registers, with zeros behind its end.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
+  constexpr int BM = 256, BN = 256, BK = 64, WN = 4, FM = 8, FN = 4;
+  typedef Tile<T, BM, MODE != kBackWeight, 512> TileA;
+  typedef Tile<T, BN, MODE == kForward, 512> TileB;
+  __shared__ __align__(16) char even[TileA::bytes + TileB::bytes];
+  __shared__ __align__(16) char odd[TileA::bytes + TileB::bytes];
+  const int wave = threadIdx.x >> 6, wm0 = (wave / WN) * (FM * 16), wn0 = (wave % WN) * (FN * 16);
+  int at_a[FM], at_b[FN];
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = wm * (BM / WM) + i * 16 + (lane & 15);
-    if (m >= rows_a) continue;
+  for (int i = 0; i < FM; ++i) at_a[i] = TileA::lane_place(wm0 + i * 16);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int n = wn * (BN / WN) + j * 16 + (lane >> 4) * 4;
-      if (n >= rows_b) continue;
-      float r[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-      if (partial) {
-        store4(partial + (int64_t)m * a.n + n, rows_b - n, r);
-        continue;
+  for (int j = 0; j < FN; ++j) at_b[j] = TileB::lane_place(wn0 + j * 16);
+
+  Groups groups(a, MODE == kBackWeight ? a.per_split : BM);
+  const unsigned xcd = blockIdx.x % 8, blocks = gridDim.x / 8;
+  const Items items = items_of<MODE>(a, groups, BM, xcd);
+  unsigned item = blockIdx.x / 8;
+  auto next = [&](Work<T>& w) {
+    for (w.none = true; w.none && item < items.count; item += blocks) w = uniform(find_work<T, BM, BN, MODE, 512>(a, groups, items, xcd, item));
+  };
+  uint32_t from_a[TileA::per_thread], from_b[TileB::per_thread];
+  auto copy = [&](char* lds, const Work<T>& w, int t) {
+    TileA::copy(lds, w.pa + t * (MODE == kBackWeight ? BK * w.lda : BK), from_a);
+    TileB::copy(lds + TileA::bytes, w.pb + t * (MODE == kForward ? BK : BK * w.ldb), from_b);
+  };
+  auto begin = [&](const Work<T>& w) {
+    if (w.none) return;
+    TileA::offsets(from_a, w.lda, w.rows_a);
+    TileB::offsets(from_b, w.ldb, w.rows_b);
+    if (w.depth >= BK) copy(even, w, 0);
+  };
+  auto arrived = [&] {     // this wave's loads have landed, and every wave is done with the buffer that is filled next
+    __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+    __syncthreads();
+  };
+
+  Work<T> w;
+  next(w);
+  begin(w);
+  while (!w.none) {
+    const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && wn0 == 0;
+    v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    auto multiply = [&](const char* lds) {
+#pragma unroll
+      for (int kk = 0; kk < BK; kk += 32) {
+        v8s fb[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) fb[j] = TileB::fragment(lds + TileA::bytes, 0, at_b[j], kk);
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          const v8s fa = TileA::fragment(lds, 0, at_a[i], kk);
+#pragma unroll
+          for (int j = 0; j < FN; ++j) acc[i][j] = mfma<T>(fb[j], fa, acc[i][j]);
+          if (MODE == kBackWeight && sum_bias) accb = mfma<T>(ones_in_row<T>(i), fa, accb);
+        }
       }
-      if (MODE == kForward && a.bias) {
-        const T* bias = (const T*)a.bias + (int64_t)group * a.n + n0 + n;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (n + e < rows_b) r[e] += (float)bias[e];
+    };
+    const int steps = w.depth / BK, rest = w.depth % BK;
+    for (int t = 0; t < steps; t += 2) {
+      arrived();
+      if (t + 1 < steps) copy(odd, w, t + 1);
+      multiply(even);
+      if (t + 1 < steps) {
+        arrived();
+        if (t + 2 < steps) copy(even, w, t + 2);
+        multiply(odd);
       }
-      T* out = (T*)a.out;
-      if constexpr (MODE == kBackWeight) out += ((int64_t)group * a.m + m0 + m) * a.n + n0 + n;
-      else out += (m0 + m) * a.n + n0 + n;
-      store4(out, rows_b - n, r);
     }
-    if (MODE == kBackWeight && sum_bias && lane < 16) {
-      if (partial) a.partial_bias[(int64_t)id * a.m + m0 + m] = accb[i][0];
-      else ((T*)a.dbias)[(int64_t)group * a.m + m0 + m] = (T)accb[i][0];
+    if (rest) {
+      char* lds = steps & 1 ? odd : even;
+      {
+        TileA ta;
+        ta.fetch(w.pa + (int64_t)steps * (MODE == kBackWeight ? BK * w.lda : BK), w.lda, w.rows_a, rest);
+        ta.put(lds);
+        TileB tb;
+        tb.fetch(w.pb + (int64_t)steps * (MODE == kForward ? BK : BK * w.ldb), w.ldb, w.rows_b, rest);
+        tb.put(lds + TileA::bytes);
+      }
+      __syncthreads();
+      multiply(lds);
     }
+    Work<T> after;
+    next(after);
+    __syncthreads();       // every wave is done with both buffers:
+    begin(after);          // the next tile is under way while this one's results are written
+    write_results<T, FM, FN, MODE>(a, w, wm0, wn0, acc, accb, sum_bias);
+    w = after;
   }
 }
 
@@ -435,25 +658,11 @@ __global__ void __launch_bounds__(256) grouped_row_sum_kernel(GroupArgs a) {
   const int lane = threadIdx.x & 63, chunks = (a.n + 63) / 64;
   const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6), row = id / chunks;
   if (row >= a.rows) return;
-  // the row's group: the first one whose end lies behind it
-  int group = -1;
-  int64_t high = 0;
-  for (int g0 = 0; g0 < a.groups && group < 0; g0 += 64) {
-    const int g = g0 + lane;
-    int64_t end = g < a.groups ? offset_at(a, g + 1) : 0;
-    if (g0 == 0) {
-      high = offset_at(a, 0);
-      if (row < high) break;
-    }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const int64_t o = shfl_up64(end, d); if (lane >= d && o > end) end = o; }
-    if (end < high) end = high;
-    const uint64_t hit = __ballot(g < a.groups && row < end);
-    if (hit) group = g0 + __builtin_ctzll(hit);
-    high = shfl64(end, 63);
-  }
+  Groups groups(a, 1);     // tiles of one row: the row's group is that of the tile `row`
+  int group = a.groups;
+  if (row >= groups.first_row && row < groups.last_end) group = groups.of_tile(a, 1, (unsigned)(row - groups.first_row), 1).group;
   const int n = (int)(id % chunks) * 64 + lane;
-  if (group < 0 || n >= a.n) return;   // (rows of no group: written by the tiles' kernel)
+  if (group == a.groups || n >= a.n) return;   // (rows of no group: written by the tiles' kernel)
   float s = sum_along(a.partial + row * a.n + n, a.splits, a.rows * a.n);
   if (a.bias) s += (float)((const T*)a.bias)[(int64_t)group * a.n + n];
   ((T*)a.out)[row * a.n + n] = (T)s;
@@ -466,24 +675,15 @@ __global__ void __launch_bounds__(256) grouped_weight_sum_kernel(GroupArgs a) {
   __shared__ float part[4][64];
   const int group = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // pieces in front of the group, and its own
-  int64_t high = 0;
   unsigned before = 0, mine = 0;
+  Groups groups(a, a.per_split);
+  int high = groups.first_row;
   for (int g0 = 0; g0 <= group; g0 += 64) {
-    const int g = g0 + lane;
-    int64_t end = g < a.groups ? offset_at(a, g + 1) : 0;
-    if (g0 == 0) high = offset_at(a, 0);
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) { const int64_t o = shfl_up64(end, d); if (lane >= d && o > end) end = o; }
-    if (end < high) end = high;
-    int64_t begin = shfl_up64(end, 1);
-    if (lane == 0) begin = high;
-    const unsigned pieces = (unsigned)((end - begin + a.per_split - 1) / a.per_split);
-    unsigned s = g < group ? pieces : 0u;
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) s += __shfl_xor(s, d, 64);
-    before += s;
-    if (group - g0 < 64) mine = __shfl(pieces, group - g0, 64);
-    high = shfl64(end, 63);
+    if (a.groups > 64) groups.load(a, a.per_split, g0, high);
+    const int l = min(group - g0, 63);
+    mine = (unsigned)__builtin_amdgcn_readlane(groups.tiles, l);
+    before += (unsigned)__builtin_amdgcn_readlane(groups.upto, l) - (group - g0 < 64 ? mine : 0u);
+    high = __builtin_amdgcn_readlane(groups.end, 63);
   }
   const int64_t weights = (int64_t)a.m * a.n, size = weights + (a.dbias ? a.m : 0);
   const unsigned per = (mine + 3) / 4, q0 = min(wave * per, mine), q1 = min(q0 + per, mine);
@@ -542,6 +742,16 @@ static GroupPlan plan_weight(int64_t rows, int64_t groups, int64_t m, int64_t n,
   return p;
 }
 
+// The large tiles take over where every piece of both operands is aligned and there are about enough of them for the compute units: below
+// that the finer cut of the 128-row tiles is worth more than the higher rate.
+static constexpr unsigned kLargeBlocks = 256;   // one a compute unit, each taking tiles until there are none
+static bool large_tiles(int dtype, int64_t m_average, int64_t n, int64_t tiles, int64_t longest, std::initializer_list<uintptr_t> aligned) {
+  if (longest >= (1 << 22) || dtype == VC_F32 || m_average < 192 || n < 192 || tiles < 160) return false;
+  for (uintptr_t v : aligned)
+    if (v & 15) return false;
+  return true;
+}
+
 static bool grouped_dtype(int t) { return t == VC_F32 || t == VC_F16 || t == VC_BF16; }
 
 static int grouped_check(const char* who, int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype, int offset_bits, const void* offsets) {
@@ -559,19 +769,28 @@ static int launch_rows(const char* who, GroupArgs a, int mode, int dtype, const 
   a.partial = (float*)ws;
   a.splits = p.splits;
   a.per_split = p.per_split;
-  a.ntiles = (int)cdiv(a.n, p.bn);
-  const int64_t total = p.mtiles_most * a.ntiles * p.splits;
-  VC_REQUIRE(total < (1LL << 31), "%s: %lld tiles", who, (long long)total);
-  a.total = (unsigned)total;
+  const uintptr_t size = 2;
+  const bool large = p.splits == 1 && large_tiles(dtype, a.groups ? a.rows / a.groups : 0, a.n, cdiv(a.rows, 256) * cdiv(a.n, 256), a.lda > a.n ? a.lda : a.n,
+                                                  {(uintptr_t)a.a, (uintptr_t)a.b, a.lda * size, a.k * size, a.n * size});
+  a.ntiles = (int)cdiv(a.n, large ? 256 : p.bn);
+  const int64_t total = (large ? a.rows / 256 + a.groups + 2 : p.mtiles_most) * a.ntiles * p.splits;
+  VC_REQUIRE(total < (1LL << 30), "%s: %lld tiles", who, (long long)total);
+  const unsigned blocks = large ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
 #define VC_GO(T, BM, BN)                                                                                                          \
-  if (mode == kForward) hipLaunchKernelGGL((grouped_kernel<T, BM, BN, kForward>), dim3(a.total), dim3(256), 0, st, a);            \
-  else hipLaunchKernelGGL((grouped_kernel<T, BM, BN, kBackInput>), dim3(a.total), dim3(256), 0, st, a);                           \
+  if (mode == kForward) hipLaunchKernelGGL((grouped_kernel<T, BM, BN, kForward>), dim3(blocks), dim3(256), 0, st, a);            \
+  else hipLaunchKernelGGL((grouped_kernel<T, BM, BN, kBackInput>), dim3(blocks), dim3(256), 0, st, a);                           \
   if (p.splits > 1) hipLaunchKernelGGL(grouped_row_sum_kernel<T>, dim3((unsigned)cdiv(a.rows * cdiv(a.n, 64), 4)), dim3(256), 0, st, a)
 #define VC_TILES(T)                                       \
   if (p.bm == 128) { VC_GO(T, 128, 128); }                \
   else if (p.bm == 64) { VC_GO(T, 64, 64); }              \
   else { VC_GO(T, 16, 128); }
-  if (dtype == VC_F32) { VC_TILES(float) } else if (dtype == VC_F16) { VC_TILES(_Float16) } else { VC_TILES(__bf16) }
+#define VC_LARGE(T)                                                                                                               \
+  if (mode == kForward) hipLaunchKernelGGL((grouped_large_kernel<T, kForward>), dim3(blocks), dim3(512), 0, st, a);              \
+  else hipLaunchKernelGGL((grouped_large_kernel<T, kBackInput>), dim3(blocks), dim3(512), 0, st, a)
+  if (large && dtype == VC_F16) { VC_LARGE(_Float16); }
+  else if (large) { VC_LARGE(__bf16); }
+  else if (dtype == VC_F32) { VC_TILES(float) } else if (dtype == VC_F16) { VC_TILES(_Float16) } else { VC_TILES(__bf16) }
+#undef VC_LARGE
 #undef VC_TILES
 #undef VC_GO
   VC_CHECK_LAUNCH(who);
@@ -636,20 +855,27 @@ int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const voi
   a.a = dy; a.lda = dy_stride; a.b = x; a.ldb = x_stride; a.offsets = offsets; a.off64 = offset_bits == 64; a.out = dweight; a.dbias = dbias;
   a.rows = rows; a.groups = (int)groups; a.m = (int)out; a.n = (int)in;
   a.splits = p.splits; a.per_split = p.per_split;
-  a.mtiles = (int)cdiv(out, p.bm); a.ntiles = (int)cdiv(in, p.bn);
+  const uintptr_t size = 2;
+  const bool large = p.splits == 1 && large_tiles(dtype, out, in, groups * cdiv(out, 256) * cdiv(in, 256), x_stride > dy_stride ? x_stride : dy_stride,
+                                                  {(uintptr_t)x, (uintptr_t)dy, x_stride * size, dy_stride * size, in * size, out * size});
+  a.mtiles = (int)cdiv(out, large ? 256 : p.bm); a.ntiles = (int)cdiv(in, large ? 256 : p.bn);
   a.partial = (float*)workspace;
   a.partial_bias = a.partial + p.mtiles_most * out * in;
-  const int64_t total = p.mtiles_most * a.mtiles * a.ntiles;
-  VC_REQUIRE(total < (1LL << 31), "%s: %lld tiles", who, (long long)total);
-  a.total = (unsigned)total;
+  const int64_t tiles = (int64_t)a.mtiles * a.ntiles;
+  // without splits every XCD takes an eighth of each group's tiles
+  const int64_t total = p.splits == 1 && tiles >= 8 ? cdiv(tiles, 8) * 8 * groups : p.mtiles_most * tiles;
+  VC_REQUIRE(total < (1LL << 30), "%s: %lld tiles", who, (long long)total);
+  const unsigned blocks = large ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
   hipStream_t st = (hipStream_t)stream;
   const int64_t sum_blocks = cdiv(out * in + out, 64);
 #define VC_GO(T)                                                                                                                              \
-  if (p.bm == 128) hipLaunchKernelGGL((grouped_kernel<T, 128, 128, kBackWeight>), dim3(a.total), dim3(256), 0, st, a);                        \
-  else hipLaunchKernelGGL((grouped_kernel<T, 64, 64, kBackWeight>), dim3(a.total), dim3(256), 0, st, a);                                      \
+  if (p.bm == 128) hipLaunchKernelGGL((grouped_kernel<T, 128, 128, kBackWeight>), dim3(blocks), dim3(256), 0, st, a);                        \
+  else hipLaunchKernelGGL((grouped_kernel<T, 64, 64, kBackWeight>), dim3(blocks), dim3(256), 0, st, a);                                      \
   if (p.splits > 1)                                                                                                                           \
     hipLaunchKernelGGL(grouped_weight_sum_kernel<T>, dim3((unsigned)(sum_blocks < 16384 ? sum_blocks : 16384), (unsigned)groups), dim3(256), 0, st, a)
-  if (dtype == VC_F32) { VC_GO(float); } else if (dtype == VC_F16) { VC_GO(_Float16); } else { VC_GO(__bf16); }
+  if (large && dtype == VC_F16) hipLaunchKernelGGL((grouped_large_kernel<_Float16, kBackWeight>), dim3(blocks), dim3(512), 0, st, a);
+  else if (large) hipLaunchKernelGGL((grouped_large_kernel<__bf16, kBackWeight>), dim3(blocks), dim3(512), 0, st, a);
+  else if (dtype == VC_F32) { VC_GO(float); } else if (dtype == VC_F16) { VC_GO(_Float16); } else { VC_GO(__bf16); }
 #undef VC_GO
   VC_CHECK_LAUNCH(who);
   return VC_OK;
