@@ -309,7 +309,7 @@ template <typename T> __device__ __forceinline__ void store4(T* p, int valid, co
 // ------------------------------------------------------------------------------------------------ tiles of a block
 // What a block computes: where its operands begin, how much of them there is, where its results go.
 template <typename T> struct Work {
-  const T *pa, *pb;
+  int64_t pa, pb;          // elements behind a.a and a.b
   int64_t lda, ldb, m0;
   int rows_a, rows_b, depth, group, n0;
   unsigned piece;
@@ -319,10 +319,9 @@ template <typename T> struct Work {
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int64_t uniform(int64_t x) { return (int64_t)(((uint64_t)(uint32_t)uniform((int)(x >> 32)) << 32) | (uint32_t)uniform((int)x)); }
-template <typename P> __device__ __forceinline__ P* uniform(P* p) { return (P*)uniform((int64_t)p); }
 template <typename T> __device__ __forceinline__ Work<T> uniform(const Work<T>& w) {   // into scalar registers
   return {uniform(w.pa), uniform(w.pb), uniform(w.lda), uniform(w.ldb), uniform(w.m0), uniform(w.rows_a), uniform(w.rows_b), uniform(w.depth),
-          uniform(w.group), uniform(w.n0), (unsigned)uniform((int)w.piece), uniform(w.partial), (bool)uniform((int)w.none)};
+          uniform(w.group), uniform(w.n0), (unsigned)uniform((int)w.piece), w.partial, (bool)uniform((int)w.none)};
 }
 
 // Consecutive blocks go to the eight XCDs in turn; the blocks of one XCD take neighbouring items, which share operands in its L2.
@@ -378,8 +377,8 @@ __device__ __forceinline__ Work<T> find_work(const GroupArgs& a, Groups& g, cons
     w.depth = min(a.per_split, a.k - k0);
     w.rows_a = (int)min((int64_t)BM, at.end - w.m0);
     w.lda = a.lda;
-    w.pa = (const T*)a.a + w.m0 * a.lda + k0;
-    const T* weights = (const T*)a.b + (int64_t)w.group * a.n * a.k;
+    w.pa = w.m0 * a.lda + k0;
+    const int64_t weights = (int64_t)w.group * a.n * a.k;
     w.ldb = MODE == kForward ? a.k : a.n;
     w.pb = MODE == kForward ? weights + (int64_t)w.n0 * a.k + k0 : weights + (int64_t)k0 * a.n + w.n0;
     if (a.splits > 1) w.partial = a.partial + ((int64_t)split * a.rows + w.m0) * a.n + w.n0;
@@ -413,8 +412,8 @@ __device__ __forceinline__ Work<T> find_work(const GroupArgs& a, Groups& g, cons
     w.rows_a = (int)min((int64_t)BM, (int64_t)a.m - w.m0);
     w.lda = a.lda;
     w.ldb = a.ldb;
-    w.pa = (const T*)a.a + r0 * a.lda + w.m0;
-    w.pb = (const T*)a.b + r0 * a.ldb + w.n0;
+    w.pa = r0 * a.lda + w.m0;
+    w.pb = r0 * a.ldb + w.n0;
   }
   w.rows_b = min(BN, a.n - w.n0);
   w.none = false;
@@ -476,7 +475,7 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
   if (item >= items.count) return;
   const Work<T> w = find_work<T, BM, BN, MODE, 256>(a, groups, items, xcd, item);
   if (w.none) return;
-  const T *const pa = w.pa, *const pb = w.pb;
+  const T *const pa = (const T*)a.a + w.pa, *const pb = (const T*)a.b + w.pb;
   const int64_t lda = w.lda, ldb = w.ldb;
   const int rows_a = w.rows_a, rows_b = w.rows_b, depth = w.depth;
   const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && wn == 0;
@@ -562,19 +561,34 @@ __global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
   Groups groups(a, MODE == kBackWeight ? a.per_split : BM);
   const unsigned xcd = blockIdx.x % 8, blocks = gridDim.x / 8;
   const Items items = items_of<MODE>(a, groups, BM, xcd);
-  unsigned item = blockIdx.x / 8;
+  const unsigned block = blockIdx.x / 8;
+  unsigned round = 0;
   auto next = [&](Work<T>& w) {
-    for (w.none = true; w.none && item < items.count; item += blocks) w = uniform(find_work<T, BM, BN, MODE, 512>(a, groups, items, xcd, item));
+    // (there and back: a block that had one of the larger items of a round gets one of the smaller of the next)
+    for (w.none = true; w.none && round * blocks < items.count; ++round) {
+      const unsigned item = round * blocks + (round & 1 ? blocks - 1 - block : block);
+      if (item < items.count) w = uniform(find_work<T, BM, BN, MODE, 512>(a, groups, items, xcd, item));
+    }
   };
   uint32_t from_a[TileA::per_thread], from_b[TileB::per_thread];
+  struct alignas(8) Four { T v[4]; };
+  Four bias[FN];           // of the tile to come: asked for before the stores of the one that ends, which later loads queue behind
   auto copy = [&](char* lds, const Work<T>& w, int t) {
-    TileA::copy(lds, w.pa + t * (MODE == kBackWeight ? BK * w.lda : BK), from_a);
-    TileB::copy(lds + TileA::bytes, w.pb + t * (MODE == kForward ? BK : BK * w.ldb), from_b);
+    TileA::copy(lds, (const T*)a.a + (w.pa + t * (MODE == kBackWeight ? BK * w.lda : BK)), from_a);
+    TileB::copy(lds + TileA::bytes, (const T*)a.b + (w.pb + t * (MODE == kForward ? BK : BK * w.ldb)), from_b);
   };
   auto begin = [&](const Work<T>& w) {
     if (w.none) return;
     TileA::offsets(from_a, w.lda, w.rows_a);
     TileB::offsets(from_b, w.ldb, w.rows_b);
+    if (MODE == kForward && a.bias) {
+      const T* p = (const T*)a.bias + (int64_t)w.group * a.n + w.n0;
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int n = wn0 + j * 16 + ((threadIdx.x & 63) >> 4) * 4;
+        bias[j] = *reinterpret_cast<const Four*>(p + (n < w.rows_b ? n : 0));   // (sizes and pointers are multiples of eight elements)
+      }
+    }
     if (w.depth >= BK) copy(even, w, 0);
   };
   auto arrived = [&] {     // this wave's loads have landed, and every wave is done with the buffer that is filled next
@@ -589,9 +603,12 @@ __global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
     const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && wn0 == 0;
     v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < FM; ++i)
+    for (int j = 0; j < FN; ++j) {
+      v4f start = accb;
+      if (MODE == kForward && a.bias) start = v4f{(float)bias[j].v[0], (float)bias[j].v[1], (float)bias[j].v[2], (float)bias[j].v[3]};
 #pragma unroll
-      for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+      for (int i = 0; i < FM; ++i) acc[i][j] = start;
+    }
     auto multiply = [&](const char* lds) {
 #pragma unroll
       for (int kk = 0; kk < BK; kk += 32) {
@@ -622,10 +639,10 @@ __global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
       char* lds = steps & 1 ? odd : even;
       {
         TileA ta;
-        ta.fetch(w.pa + (int64_t)steps * (MODE == kBackWeight ? BK * w.lda : BK), w.lda, w.rows_a, rest);
+        ta.fetch((const T*)a.a + w.pa + (int64_t)steps * (MODE == kBackWeight ? BK * w.lda : BK), w.lda, w.rows_a, rest);
         ta.put(lds);
         TileB tb;
-        tb.fetch(w.pb + (int64_t)steps * (MODE == kForward ? BK : BK * w.ldb), w.ldb, w.rows_b, rest);
+        tb.fetch((const T*)a.b + w.pb + (int64_t)steps * (MODE == kForward ? BK : BK * w.ldb), w.ldb, w.rows_b, rest);
         tb.put(lds + TileA::bytes);
       }
       __syncthreads();
@@ -635,7 +652,21 @@ __global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
     next(after);
     __syncthreads();       // every wave is done with both buffers:
     begin(after);          // the next tile is under way while this one's results are written
-    write_results<T, FM, FN, MODE>(a, w, wm0, wn0, acc, accb, sum_bias);
+    const int lane = threadIdx.x & 63, m0 = wm0 + (lane & 15), nb = wn0 + (lane >> 4) * 4;
+    T* out = (T*)a.out + ((MODE == kBackWeight ? (int64_t)w.group * a.m : 0) + w.m0) * a.n + w.n0 + (int64_t)m0 * a.n + nb;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        Four e;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) e.v[k] = (T)acc[i][j][k];
+        if (m0 + i * 16 < w.rows_a && nb + j * 16 < w.rows_b) *reinterpret_cast<Four*>(out + j * 16) = e;
+      }
+      out += (int64_t)16 * a.n;
+      if (MODE == kBackWeight && sum_bias && lane >> 4 == i >> 2 && m0 + i * 16 < w.rows_a)
+        ((T*)a.dbias)[(int64_t)w.group * a.m + w.m0 + m0 + i * 16] = (T)accb[i & 3];
+    }
     w = after;
   }
 }
@@ -771,7 +802,7 @@ static int launch_rows(const char* who, GroupArgs a, int mode, int dtype, const 
   a.per_split = p.per_split;
   const uintptr_t size = 2;
   const bool large = p.splits == 1 && large_tiles(dtype, a.groups ? a.rows / a.groups : 0, a.n, cdiv(a.rows, 256) * cdiv(a.n, 256), a.lda > a.n ? a.lda : a.n,
-                                                  {(uintptr_t)a.a, (uintptr_t)a.b, a.lda * size, a.k * size, a.n * size});
+                                                  {(uintptr_t)a.a, (uintptr_t)a.b, (uintptr_t)a.out, (uintptr_t)a.bias, a.lda * size, a.k * size, a.n * size});
   a.ntiles = (int)cdiv(a.n, large ? 256 : p.bn);
   const int64_t total = (large ? a.rows / 256 + a.groups + 2 : p.mtiles_most) * a.ntiles * p.splits;
   VC_REQUIRE(total < (1LL << 30), "%s: %lld tiles", who, (long long)total);
@@ -857,7 +888,7 @@ int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const voi
   a.splits = p.splits; a.per_split = p.per_split;
   const uintptr_t size = 2;
   const bool large = p.splits == 1 && large_tiles(dtype, out, in, groups * cdiv(out, 256) * cdiv(in, 256), x_stride > dy_stride ? x_stride : dy_stride,
-                                                  {(uintptr_t)x, (uintptr_t)dy, x_stride * size, dy_stride * size, in * size, out * size});
+                                                  {(uintptr_t)x, (uintptr_t)dy, (uintptr_t)dweight, x_stride * size, dy_stride * size, in * size, out * size});
   a.mtiles = (int)cdiv(out, large ? 256 : p.bm); a.ntiles = (int)cdiv(in, large ? 256 : p.bn);
   a.partial = (float*)workspace;
   a.partial_bias = a.partial + p.mtiles_most * out * in;
