@@ -230,7 +230,7 @@ def check_grouped(x, w, ends, b=None, dy=None, index=torch.int32):
 GROUPED = [  # ends, inner, outer
     ([0, 1], 1, 1), ([0, 3], 8, 8), ([0, 5, 5, 9], 7, 5), ([0, 0, 0, 17], 16, 24), ([0, 40, 130], 33, 65), ([0, 130, 131, 400], 64, 64),
     ([0, 200, 457], 100, 250), ([0, 517], 250, 129), ([0, 300, 300, 900], 130, 192), ([0, 1, 2, 3, 4, 5, 6, 7, 8], 256, 144),
-    ([0, 16, 33, 47], 520, 40), ([0, 1000], 27, 16), ([0, 128, 256, 384], 128, 128),
+    ([0, 16, 33, 47], 520, 40), ([0, 1000], 27, 16), ([0, 128, 256, 384], 128, 128), ([0, 150, 170, 480], 300, 200), ([0, 0, 192, 330], 65, 129),
 ]
 
 
@@ -257,7 +257,7 @@ def test_grouped_linear_long_groups(hip_backend, dtype, ends):
                   rnd((n, 40), 4, dtype, 0.1))
 
 
-@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=str)
 @pytest.mark.parametrize("inner,outer", [(64, 8192), (136, 4104), (1064, 2056), (2056, 1064)])
 def test_grouped_linear_large_tiles(hip_backend, inner, outer, dtype):
     # enough aligned work for the large tiles in at least one direction: whole and partial tiles, whole and partial last steps, short and empty groups

@@ -151,26 +151,24 @@ __device__ __forceinline__ void load8(const T* p, int valid, T (&out)[8]) {   //
 // the top 16 bits of x as a bf16 (cut, not rounded: x - top is exact and so is what is left of it)
 __device__ __forceinline__ uint32_t top16(float x) { return __float_as_uint(x) & 0xffff0000u; }
 
+__device__ __forceinline__ uint32_t top_halves(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
+
 // eight elements into their place(s) in LDS: one 16-byte piece, or three planes of it
 template <typename T>
 __device__ __forceinline__ void stage8(char* lds, int plane_bytes, int at, const T (&x)[8]) {
   if constexpr (sizeof(T) == 2) {
     *reinterpret_cast<v8s*>(lds + at) = *reinterpret_cast<const v8s*>(&x);
   } else {
+    // four operations an element, and a byte exchange that packs two of them for each plane
     uint32_t w[3][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint32_t h[2][3];
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float v = x[2 * i + j];
-        h[j][0] = top16(v);
-        const float r = v - __uint_as_float(h[j][0]);
-        h[j][1] = top16(r);
-        h[j][2] = top16(r - __uint_as_float(h[j][1]));
-      }
-#pragma unroll
-      for (int q = 0; q < 3; ++q) w[q][i] = (h[0][q] >> 16) | h[1][q];
+      const float v0 = x[2 * i], v1 = x[2 * i + 1];
+      const float r0 = v0 - __uint_as_float(top16(v0)), r1 = v1 - __uint_as_float(top16(v1));
+      const float s0 = r0 - __uint_as_float(top16(r0)), s1 = r1 - __uint_as_float(top16(r1));
+      w[0][i] = top_halves(v0, v1);
+      w[1][i] = top_halves(r0, r1);
+      w[2][i] = top_halves(s0, s1);
     }
 #pragma unroll
     for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(lds + q * plane_bytes + at) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);
@@ -187,7 +185,10 @@ struct Tile {
   static __device__ __forceinline__ int place(int r, int k) {   // byte of element (row r, summed index k); r or k a multiple of 8
     if constexpr (ALONG) {
       constexpr int CH = BK / 8, R = 16 / CH;                   // pieces a row, rows per 256 bytes
-      return r * BK * 2 + ((((k >> 3) ^ (r / R)) & (CH - 1)) << 4);
+      // ds_read_b128 serves lanes 0-3, 12-15, 20-23, 24-27 (and so on) together: with four pieces a row the plain order would let rows 0-3
+      // and 4-7 meet, so the four row groups exchange by 0, 2, 3, 1
+      const int f = CH == 4 ? 0x78 >> ((r / R & 3) << 1) : r / R;
+      return r * BK * 2 + ((((k >> 3) ^ f) & (CH - 1)) << 4);
     } else {
       constexpr int SLOTS = ROWS / 16;                          // 32-byte slots a row (of the summed axis)
       const int f = SLOTS >= 8 ? ((k & 3) | ((k >> 1) & 4)) : SLOTS == 4 ? (((k >> 1) & 1) | ((k >> 2) & 2)) : SLOTS == 2 ? ((k >> 3) & 1) : 0;
@@ -215,6 +216,26 @@ struct Tile {
         s = p + k * ld + c;
       }
       load8(s, valid, reg[i]);
+    }
+  }
+  // The same where every summed index of the tile exists and, for an operand across it, every row: no checks, offsets made once (rows that are
+  // not there read one that is: they only enter results that are not written).  `whole`: may a tile of these sizes be read so?
+  static __device__ __forceinline__ bool whole(int64_t ld, int rows) { return (ALONG || rows == ROWS) && ld < (1 << 22); }
+  static __device__ __forceinline__ void plain_offsets(uint32_t (&from)[per_thread], int64_t ld, int rows) {
+#pragma unroll
+    for (int i = 0; i < per_thread; ++i) {
+      const int q = min(i * THREADS + (int)threadIdx.x % THREADS, pieces - 1);
+      if constexpr (ALONG) from[i] = ((uint32_t)min(q / (BK / 8), rows - 1) * (uint32_t)ld + (q % (BK / 8)) * 8) * sizeof(T);
+      else from[i] = ((uint32_t)(q / (ROWS / 8)) * (uint32_t)ld + (q % (ROWS / 8)) * 8) * sizeof(T);
+    }
+  }
+  __device__ __forceinline__ void fetch_whole(const T* p, const uint32_t (&from)[per_thread]) {
+#pragma unroll
+    for (int i = 0; i < per_thread; ++i) {
+      Eight<T> e;
+      __builtin_memcpy(&e, (const char*)p + from[i], sizeof(e));
+#pragma unroll
+      for (int k = 0; k < 8; ++k) reg[i][k] = e.v[k];
     }
   }
   __device__ __forceinline__ void put(char* lds) {
@@ -424,6 +445,23 @@ __device__ __forceinline__ Work<T> find_work(const GroupArgs& a, Groups& g, cons
 template <typename T, int FM, int FN, int MODE>
 __device__ __forceinline__ void write_results(const GroupArgs& a, const Work<T>& w, int wm0, int wn0, const v4f (&acc)[FM][FN], const v4f& accb, bool sum_bias) {
   const int lane = threadIdx.x & 63;
+  if (MODE != kForward && !sum_bias && w.rows_a >= wm0 + FM * 16 && w.rows_b >= wn0 + FN * 16) {   // the wave's part of the tile is whole
+    const int64_t at = (int64_t)(wm0 + (lane & 15)) * a.n + wn0 + (lane >> 4) * 4;
+    float* part = w.partial ? w.partial + at : nullptr;
+    T* out = (T*)a.out + ((MODE == kBackWeight ? (int64_t)w.group * a.m : 0) + w.m0) * a.n + w.n0 + at;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const float r[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if (part) store4(part + j * 16, 4, r);
+        else store4(out + j * 16, 4, r);
+      }
+      if (part) part += (int64_t)16 * a.n;
+      out += (int64_t)16 * a.n;
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
     const int m = wm0 + i * 16 + (lane & 15);
@@ -456,17 +494,17 @@ __device__ __forceinline__ void write_results(const GroupArgs& a, const Work<T>&
 }
 
 // ------------------------------------------------------------------------------------------------ the kernel for every case
-template <typename T, int BM, int BN, int MODE>
+// WM of the four waves lie along m.  STAGES tiles are under way in registers ahead of the one that is multiplied (a short summed axis is asked
+// for as a whole, a long one keeps that many times a tile in flight).
+template <typename T, int BM, int BN, int WM, int STAGES, int MODE>
 __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
   typedef typename OperandOf<T>::type O;
   constexpr int BK = OperandOf<T>::bk, P = OperandOf<T>::planes;
   typedef Tile<T, BM, MODE != kBackWeight> TileA;
   typedef Tile<T, BN, MODE == kForward> TileB;
-  constexpr int WM = BM >= 64 ? 2 : 1, WN = 4 / WM;            // waves along m and n
-  constexpr int FM = BM / WM / 16, FN = BN / WN / 16;          // fragments of a wave
-  __shared__ __align__(16) char lds[TileA::bytes + TileB::bytes];
-  char* const la = lds;
-  char* const lb = lds + TileA::bytes;
+  constexpr int WN = 4 / WM, FM = BM / WM / 16, FN = BN / WN / 16;   // waves along n, fragments of a wave
+  constexpr int kBuffer = TileA::bytes + TileB::bytes;
+  __shared__ __align__(16) char lds[2 * kBuffer];
   const int wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
 
   Groups groups(a, MODE == kBackWeight ? a.per_split : BM);
@@ -480,6 +518,26 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
   const int rows_a = w.rows_a, rows_b = w.rows_b, depth = w.depth;
   const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && wn == 0;
 
+  TileA ta[STAGES];
+  TileB tb[STAGES];
+  const bool whole = TileA::whole(lda, rows_a) && TileB::whole(ldb, rows_b);
+  uint32_t from_a[TileA::per_thread], from_b[TileB::per_thread];
+  TileA::plain_offsets(from_a, lda, rows_a);
+  TileB::plain_offsets(from_b, ldb, rows_b);
+  auto fetch = [&](int stage, int k0) {
+    if (k0 >= depth) return;
+    const int64_t k = k0;
+    const T *p = pa + (MODE == kBackWeight ? k * lda : k), *q = pb + (MODE == kForward ? k : k * ldb);
+    if (whole && k0 + BK <= depth) {
+      ta[stage].fetch_whole(p, from_a);
+      tb[stage].fetch_whole(q, from_b);
+    } else {
+      ta[stage].fetch(p, lda, rows_a, depth - k0);
+      tb[stage].fetch(q, ldb, rows_b, depth - k0);
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < STAGES; ++d) fetch(d, d * BK);
   v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -490,53 +548,184 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
   for (int i = 0; i < FM; ++i) at_a[i] = TileA::lane_place(wm * (BM / WM) + i * 16);
 #pragma unroll
   for (int j = 0; j < FN; ++j) at_b[j] = TileB::lane_place(wn * (BN / WN) + j * 16);
-  TileA ta;
-  TileB tb;
-  ta.fetch(pa, lda, rows_a, depth);
-  tb.fetch(pb, ldb, rows_b, depth);
-  for (int k0 = 0; k0 < depth; k0 += BK) {
-    __syncthreads();
-    ta.put(la);
-    tb.put(lb);
-    __syncthreads();
-    if (k0 + BK < depth) {   // the next tile is under way while this one is multiplied
-      const int64_t k1 = k0 + BK;
-      ta.fetch(MODE == kBackWeight ? pa + k1 * lda : pa + k1, lda, rows_a, depth - (int)k1);
-      tb.fetch(MODE == kForward ? pb + k1 : pb + k1 * ldb, ldb, rows_b, depth - (int)k1);
-    }
+
+  // One barrier a step: the two halves of LDS take turns, so that a wave may put the next tile while another still multiplies this one.
+  int half = 0;
+  for (int kb = 0; kb < depth; kb += STAGES * BK) {
 #pragma unroll
-    for (int kk = 0; kk < BK; kk += 32) {
-      v8s fb[FN][P];
+    for (int d = 0; d < STAGES; ++d) {
+      const int k0 = kb + d * BK;
+      if (k0 >= depth) break;
+      char* const la = lds + half;
+      char* const lb = la + TileA::bytes;
+      half ^= kBuffer;
+      ta[d].put(la);
+      tb[d].put(lb);
+      __syncthreads();
+      fetch(d, k0 + STAGES * BK);
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
+      for (int kk = 0; kk < BK; kk += 32) {
+        v8s fb[FN][P];
 #pragma unroll
-        for (int q = 0; q < P; ++q) fb[j][q] = TileB::fragment(lb, q, at_b[j], kk);
+        for (int j = 0; j < FN; ++j)
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        v8s fa[P];
+          for (int q = 0; q < P; ++q) fb[j][q] = TileB::fragment(lb, q, at_b[j], kk);
 #pragma unroll
-        for (int q = 0; q < P; ++q) fa[q] = TileA::fragment(la, q, at_a[i], kk);
+        for (int i = 0; i < FM; ++i) {
+          v8s fa[P];
 #pragma unroll
-        for (int j = 0; j < FN; ++j) {
-          // the lane's four results are neighbours along n: the n side is the instruction's row operand
-          if constexpr (P == 3) {
-            acc[i][j] = mfma<O>(fb[j][2], fa[0], acc[i][j]);
-            acc[i][j] = mfma<O>(fb[j][0], fa[2], acc[i][j]);
-            acc[i][j] = mfma<O>(fb[j][1], fa[1], acc[i][j]);
-            acc[i][j] = mfma<O>(fb[j][1], fa[0], acc[i][j]);
-            acc[i][j] = mfma<O>(fb[j][0], fa[1], acc[i][j]);
+          for (int q = 0; q < P; ++q) fa[q] = TileA::fragment(la, q, at_a[i], kk);
+#pragma unroll
+          for (int j = 0; j < FN; ++j) {
+            // the lane's four results are neighbours along n: the n side is the instruction's row operand
+            if constexpr (P == 3) {
+              acc[i][j] = mfma<O>(fb[j][2], fa[0], acc[i][j]);
+              acc[i][j] = mfma<O>(fb[j][0], fa[2], acc[i][j]);
+              acc[i][j] = mfma<O>(fb[j][1], fa[1], acc[i][j]);
+              acc[i][j] = mfma<O>(fb[j][1], fa[0], acc[i][j]);
+              acc[i][j] = mfma<O>(fb[j][0], fa[1], acc[i][j]);
+            }
+            acc[i][j] = mfma<O>(fb[j][0], fa[0], acc[i][j]);
           }
-          acc[i][j] = mfma<O>(fb[j][0], fa[0], acc[i][j]);
-        }
-        if (MODE == kBackWeight && sum_bias) {
+          if (MODE == kBackWeight && sum_bias) {
 #pragma unroll
-          for (int q = P - 1; q >= 0; --q) accb = mfma<O>(ones_in_row<O>(i), fa[q], accb);
+            for (int q = P - 1; q >= 0; --q) accb = mfma<O>(ones_in_row<O>(i), fa[q], accb);
+          }
         }
       }
     }
   }
 
   write_results<T, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc, accb, sum_bias);
+}
+
+// ------------------------------------------------------------------------------------------------ large tiles of fp32 operands
+// Cutting fp32 operands into three bf16 pieces takes half as many issue slots as their six products take matrix cycles, and in a wave that does
+// both the two come one after the other (28 to 40 per cent of the matrix rate).  So each SIMD has one wave that loads, cuts and stores tiles and
+// one that multiplies them: four waves of each kind, two halves of LDS, one barrier a step.  The block takes tiles until there are none, and
+// the first kind is already at the next tile while the second writes its results.
+template <int BM, int BN, int MODE>
+__global__ void __launch_bounds__(512, 2) grouped_f32_kernel(GroupArgs a) {
+  constexpr int BK = 32, P = 3, STAGES = 2, WM = 2, WN = 2, FM = BM / WM / 16, FN = BN / WN / 16;
+  typedef Tile<float, BM, MODE != kBackWeight> TileA;
+  typedef Tile<float, BN, MODE == kForward> TileB;
+  constexpr int kBuffer = TileA::bytes + TileB::bytes;
+  __shared__ __align__(16) char lds[2 * kBuffer];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  Groups groups(a, MODE == kBackWeight ? a.per_split : BM);
+  const unsigned xcd = blockIdx.x % 8, blocks = gridDim.x / 8, block = blockIdx.x / 8;
+  const Items items = items_of<MODE>(a, groups, BM, xcd);
+  unsigned round = 0;
+  auto next = [&](Work<float>& w) {
+    for (w.none = true; w.none && round * blocks < items.count; ++round) {
+      const unsigned item = round * blocks + (round & 1 ? blocks - 1 - block : block);
+      if (item < items.count) w = uniform(find_work<float, BM, BN, MODE, 512>(a, groups, items, xcd, item));
+    }
+  };
+  auto meet = [] {           // what this wave wrote is there for the others, and they have come as far
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  };
+  int half = 0;
+  Work<float> w;
+  next(w);
+  if (wave < 4) {
+    // The steps of all tiles are one stream: the loads run two steps ahead of the stores, into the next tile where this one ends.
+    TileA ta[STAGES];
+    TileB tb[STAGES];
+    bool there[STAGES], whole = false;
+    uint32_t from_a[TileA::per_thread], from_b[TileB::per_thread];
+    int k0 = 0;
+    auto settle = [&](bool fresh) {      // (k0 is a step of w, or there is none left)
+      while (!w.none && k0 >= w.depth) { next(w); k0 = 0; fresh = true; }
+      if (!fresh || w.none) return;
+      whole = TileA::whole(w.lda, w.rows_a) && TileB::whole(w.ldb, w.rows_b);
+      TileA::plain_offsets(from_a, w.lda, w.rows_a);
+      TileB::plain_offsets(from_b, w.ldb, w.rows_b);
+    };
+    auto fetch = [&](int stage) {
+      there[stage] = !w.none;
+      if (w.none) return;
+      const int64_t k = k0;
+      const float* pa = (const float*)a.a + (w.pa + (MODE == kBackWeight ? k * w.lda : k));
+      const float* pb = (const float*)a.b + (w.pb + (MODE == kForward ? k : k * w.ldb));
+      if (whole && k0 + BK <= w.depth) {
+        ta[stage].fetch_whole(pa, from_a);
+        tb[stage].fetch_whole(pb, from_b);
+      } else {
+        ta[stage].fetch(pa, w.lda, w.rows_a, w.depth - k0);
+        tb[stage].fetch(pb, w.ldb, w.rows_b, w.depth - k0);
+      }
+      k0 += BK;
+      settle(false);
+    };
+    settle(true);
+#pragma unroll
+    for (int d = 0; d < STAGES; ++d) fetch(d);
+    for (bool more = true; more;) {
+#pragma unroll
+      for (int d = 0; d < STAGES; ++d) {
+        if (!there[d]) { more = false; break; }
+        ta[d].put(lds + half);
+        tb[d].put(lds + half + TileA::bytes);
+        half ^= kBuffer;
+        fetch(d);
+        meet();
+      }
+    }
+    return;
+  }
+  const int wm = (wave - 4) / WN, wn = (wave - 4) % WN;
+  int at_a[FM], at_b[FN];
+#pragma unroll
+  for (int i = 0; i < FM; ++i) at_a[i] = TileA::lane_place(wm * (BM / WM) + i * 16);
+#pragma unroll
+  for (int j = 0; j < FN; ++j) at_b[j] = TileB::lane_place(wn * (BN / WN) + j * 16);
+  while (!w.none) {
+    const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && wn == 0;
+    v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+      for (int j = 0; j < FN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+    for (int k0 = 0; k0 < w.depth; k0 += BK) {
+      meet();
+      const char *la = lds + half, *lb = la + TileA::bytes;
+      half ^= kBuffer;
+      v8s fb[FN][P];
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int q = 0; q < P; ++q) fb[j][q] = TileB::fragment(lb, q, at_b[j], 0);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        v8s fa[P];
+#pragma unroll
+        for (int q = 0; q < P; ++q) fa[q] = TileA::fragment(la, q, at_a[i], 0);
+        // the smallest terms first, each over all columns: neighbouring products do not wait for one another
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma<__bf16>(fb[j][2], fa[0], acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma<__bf16>(fb[j][0], fa[2], acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma<__bf16>(fb[j][1], fa[1], acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma<__bf16>(fb[j][1], fa[0], acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma<__bf16>(fb[j][0], fa[1], acc[i][j]);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma<__bf16>(fb[j][0], fa[0], acc[i][j]);
+        if (MODE == kBackWeight && sum_bias) {
+#pragma unroll
+          for (int q = P - 1; q >= 0; --q) accb = mfma<__bf16>(ones_in_row<__bf16>(i), fa[q], accb);
+        }
+      }
+    }
+    write_results<float, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc, accb, sum_bias);
+    next(w);
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ large tiles of aligned 16-bit operands
@@ -733,20 +922,24 @@ __global__ void __launch_bounds__(256) grouped_weight_sum_kernel(GroupArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ launch rules
-struct GroupPlan { int bm, bn, splits, per_split; int64_t partial_floats, mtiles_most; };
+struct GroupPlan { int bm, bn, splits, per_split; bool two_kinds; int64_t partial_floats, mtiles_most; };
 
-// Row products.  Tiles of 128 rows where the groups have that many on average, of 64 or 16 where they have fewer (a tile of a short group is
-// mostly padding); the inner axis is split where there are too few tiles to fill 256 compute units.
+// Row products.  Tiles of 128 x 128 where the groups have several of them on average, of 64 x 128 or 16 x 128 where they are shorter (a tile of a
+// short group is mostly padding), of 64 x 64 where there are no more than 64 columns; the inner axis is split where there are too few
+// tiles to fill 256 compute units.
 static GroupPlan plan_rows(int64_t rows, int64_t groups, int64_t n, int64_t k, int dtype) {
   GroupPlan p;
   const int64_t average = groups > 0 ? rows / groups : rows, bk = dtype == VC_F32 ? 32 : 64;
-  p.bm = average > 96 && n > 64 ? 128 : average > 24 ? 64 : 16;
-  p.bn = p.bm == 64 ? 64 : 128;
+  p.two_kinds = dtype == VC_F32 && average > 64 && n > 64;
+  if (p.two_kinds) { p.bm = average > 128 && average <= 192 ? 192 : 128; p.bn = 128; }
+  else if (average <= 24) { p.bm = 16; p.bn = 128; }
+  else if (n <= 64) { p.bm = 64; p.bn = 64; }
+  else { p.bm = average >= 256 ? 128 : 64; p.bn = 128; }
   p.mtiles_most = rows / p.bm + groups + 2;
   // tiles there will be: full ones, and one that is cut short for every group that has rows
   const int64_t tiles = (rows / p.bm + (groups < rows ? groups : rows)) * cdiv(n, p.bn), steps = cdiv(k, bk);
   int64_t splits = 1;
-  if (tiles < 256 && steps >= 16) splits = 512 / tiles;
+  if (tiles < 256 && steps >= 16) splits = (p.two_kinds ? 256 : 512) / tiles;   // (one block of the two-kind kernel a compute unit)
   if (splits > steps / 8) splits = steps / 8 > 0 ? steps / 8 : 1;
   p.per_split = (int)(cdiv(steps, splits) * bk);
   p.splits = (int)cdiv(k, p.per_split);
@@ -759,6 +952,7 @@ static GroupPlan plan_rows(int64_t rows, int64_t groups, int64_t n, int64_t k, i
 // (and read once more) stay small beside the rows that it reads.
 static GroupPlan plan_weight(int64_t rows, int64_t groups, int64_t m, int64_t n, int dtype) {
   GroupPlan p;
+  p.two_kinds = dtype == VC_F32 && m > 64 && n > 64;
   p.bm = m > 64 && n > 64 ? 128 : 64;
   p.bn = p.bm;
   const int64_t tiles = cdiv(m, p.bm) * cdiv(n, p.bn);
@@ -806,21 +1000,29 @@ static int launch_rows(const char* who, GroupArgs a, int mode, int dtype, const 
   a.ntiles = (int)cdiv(a.n, large ? 256 : p.bn);
   const int64_t total = (large ? a.rows / 256 + a.groups + 2 : p.mtiles_most) * a.ntiles * p.splits;
   VC_REQUIRE(total < (1LL << 30), "%s: %lld tiles", who, (long long)total);
-  const unsigned blocks = large ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
-#define VC_GO(T, BM, BN)                                                                                                          \
-  if (mode == kForward) hipLaunchKernelGGL((grouped_kernel<T, BM, BN, kForward>), dim3(blocks), dim3(256), 0, st, a);            \
-  else hipLaunchKernelGGL((grouped_kernel<T, BM, BN, kBackInput>), dim3(blocks), dim3(256), 0, st, a);                           \
+  const unsigned blocks = large || p.two_kinds ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
+#define VC_GO(T, ...)                                                                                                             \
+  if (mode == kForward) hipLaunchKernelGGL((grouped_kernel<T, __VA_ARGS__, kForward>), dim3(blocks), dim3(256), 0, st, a);        \
+  else hipLaunchKernelGGL((grouped_kernel<T, __VA_ARGS__, kBackInput>), dim3(blocks), dim3(256), 0, st, a);                       \
   if (p.splits > 1) hipLaunchKernelGGL(grouped_row_sum_kernel<T>, dim3((unsigned)cdiv(a.rows * cdiv(a.n, 64), 4)), dim3(256), 0, st, a)
 #define VC_TILES(T)                                       \
-  if (p.bm == 128) { VC_GO(T, 128, 128); }                \
-  else if (p.bm == 64) { VC_GO(T, 64, 64); }              \
-  else { VC_GO(T, 16, 128); }
+  if (p.bm == 128) { if constexpr (sizeof(T) == 2) { VC_GO(T, 128, 128, 2, 2); } }    \
+  else if (p.bm == 64 && p.bn == 64) { VC_GO(T, 64, 64, 2, 3); }    \
+  else if (p.bm == 64) { VC_GO(T, 64, 128, 2, 2); }                 \
+  else { VC_GO(T, 16, 128, 1, 3); }
 #define VC_LARGE(T)                                                                                                               \
   if (mode == kForward) hipLaunchKernelGGL((grouped_large_kernel<T, kForward>), dim3(blocks), dim3(512), 0, st, a);              \
   else hipLaunchKernelGGL((grouped_large_kernel<T, kBackInput>), dim3(blocks), dim3(512), 0, st, a)
+#define VC_PIECES(BM)                                                                                                                \
+  if (mode == kForward) hipLaunchKernelGGL((grouped_f32_kernel<BM, 128, kForward>), dim3(blocks), dim3(512), 0, st, a);           \
+  else hipLaunchKernelGGL((grouped_f32_kernel<BM, 128, kBackInput>), dim3(blocks), dim3(512), 0, st, a);                          \
+  if (p.splits > 1) hipLaunchKernelGGL(grouped_row_sum_kernel<float>, dim3((unsigned)cdiv(a.rows * cdiv(a.n, 64), 4)), dim3(256), 0, st, a)
   if (large && dtype == VC_F16) { VC_LARGE(_Float16); }
   else if (large) { VC_LARGE(__bf16); }
+  else if (p.two_kinds && p.bm == 192) { VC_PIECES(192); }
+  else if (p.two_kinds) { VC_PIECES(128); }
   else if (dtype == VC_F32) { VC_TILES(float) } else if (dtype == VC_F16) { VC_TILES(_Float16) } else { VC_TILES(__bf16) }
+#undef VC_PIECES
 #undef VC_LARGE
 #undef VC_TILES
 #undef VC_GO
@@ -896,12 +1098,13 @@ int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const voi
   // without splits every XCD takes an eighth of each group's tiles
   const int64_t total = p.splits == 1 && tiles >= 8 ? cdiv(tiles, 8) * 8 * groups : p.mtiles_most * tiles;
   VC_REQUIRE(total < (1LL << 30), "%s: %lld tiles", who, (long long)total);
-  const unsigned blocks = large ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
+  const unsigned blocks = large || p.two_kinds ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
   hipStream_t st = (hipStream_t)stream;
   const int64_t sum_blocks = cdiv(out * in + out, 64);
 #define VC_GO(T)                                                                                                                              \
-  if (p.bm == 128) hipLaunchKernelGGL((grouped_kernel<T, 128, 128, kBackWeight>), dim3(blocks), dim3(256), 0, st, a);                        \
-  else hipLaunchKernelGGL((grouped_kernel<T, 64, 64, kBackWeight>), dim3(blocks), dim3(256), 0, st, a);                                      \
+  if (p.two_kinds) hipLaunchKernelGGL((grouped_f32_kernel<128, 128, kBackWeight>), dim3(blocks), dim3(512), 0, st, a);                        \
+  else if (p.bm == 128) { if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((grouped_kernel<T, 128, 128, 2, 2, kBackWeight>), dim3(blocks), dim3(256), 0, st, a); } \
+  else hipLaunchKernelGGL((grouped_kernel<T, 64, 64, 2, 3, kBackWeight>), dim3(blocks), dim3(256), 0, st, a);                                      \
   if (p.splits > 1)                                                                                                                           \
     hipLaunchKernelGGL(grouped_weight_sum_kernel<T>, dim3((unsigned)(sum_blocks < 16384 ? sum_blocks : 16384), (unsigned)groups), dim3(256), 0, st, a)
   if (large && dtype == VC_F16) hipLaunchKernelGGL((grouped_large_kernel<_Float16, kBackWeight>), dim3(blocks), dim3(512), 0, st, a);
