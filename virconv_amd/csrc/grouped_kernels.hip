@@ -153,17 +153,52 @@ __device__ __forceinline__ uint32_t top16(float x) { return __float_as_uint(x) &
 
 __device__ __forceinline__ uint32_t top_halves(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
 
+// eight elements, as 32-bit words
+template <typename T> struct Words { static constexpr int n = sizeof(T) * 2; uint32_t w[n]; };
+
+template <typename T>
+__device__ __forceinline__ Words<T> load_words(const void* p) {   // all eight, at any alignment that the elements have
+  struct __attribute__((packed, aligned(sizeof(T)))) Raw { uint32_t w[Words<T>::n]; };
+  Words<T> x;
+  const Raw r = *reinterpret_cast<const Raw*>(p);
+#pragma unroll
+  for (int i = 0; i < Words<T>::n; ++i) x.w[i] = r.w[i];
+  return x;
+}
+
+// (by value: a choice between two array elements would be made between their addresses, and put the array into memory)
+__device__ __forceinline__ uint32_t choose(bool first, uint32_t x, uint32_t y) { return first ? x : y; }
+
+// the elements `shift` places on (to the front), zeros from the `valid`-th on
+template <typename T>
+__device__ __forceinline__ void shift_words(Words<T>& x, int shift, int valid) {
+  constexpr int n = Words<T>::n, per = 4 / sizeof(T);     // elements a word
+#pragma unroll
+  for (int step = 4; step >= per; step >>= 1)
+#pragma unroll
+    for (int k = 0; k + step / per < n; ++k) x.w[k] = choose(shift & step, x.w[k + step / per], x.w[k]);
+  if constexpr (per == 2) {
+#pragma unroll
+    for (int k = 0; k < n; ++k) x.w[k] = choose(shift & 1, __builtin_amdgcn_alignbyte(k + 1 < n ? x.w[k + 1] : 0u, x.w[k], 2), x.w[k]);
+  }
+#pragma unroll
+  for (int k = 0; k < n; ++k) {
+    const int left = valid - k * per;
+    x.w[k] &= left <= 0 ? 0u : per == 2 && left == 1 ? 0xffffu : 0xffffffffu;
+  }
+}
+
 // eight elements into their place(s) in LDS: one 16-byte piece, or three planes of it
 template <typename T>
-__device__ __forceinline__ void stage8(char* lds, int plane_bytes, int at, const T (&x)[8]) {
+__device__ __forceinline__ void stage8(char* lds, int plane_bytes, int at, const Words<T>& x) {
   if constexpr (sizeof(T) == 2) {
-    *reinterpret_cast<v8s*>(lds + at) = *reinterpret_cast<const v8s*>(&x);
+    *reinterpret_cast<uint4*>(lds + at) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
   } else {
     // four operations an element, and a byte exchange that packs two of them for each plane
     uint32_t w[3][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float v0 = x[2 * i], v1 = x[2 * i + 1];
+      const float v0 = __uint_as_float(x.w[2 * i]), v1 = __uint_as_float(x.w[2 * i + 1]);
       const float r0 = v0 - __uint_as_float(top16(v0)), r1 = v1 - __uint_as_float(top16(v1));
       const float s0 = r0 - __uint_as_float(top16(r0)), s1 = r1 - __uint_as_float(top16(r1));
       w[0][i] = top_halves(v0, v1);
@@ -196,7 +231,7 @@ struct Tile {
     }
   }
 
-  T reg[per_thread][8];
+  Words<T> reg[per_thread];
 
   // rows [0, rows) and summed indices [0, depth) of the tile exist; p: the tile's first element, ld: the stride of its slow axis
   __device__ __forceinline__ void fetch(const T* p, int64_t ld, int rows, int depth) {
@@ -215,27 +250,44 @@ struct Tile {
         valid = k < depth ? rows - c : 0;
         s = p + k * ld + c;
       }
-      load8(s, valid, reg[i]);
+      T e[8];
+      load8(s, valid, e);
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) reg[i].w[j] = __builtin_bit_cast(uint32_t, e[j]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          reg[i].w[j] = (uint32_t)__builtin_bit_cast(uint16_t, e[2 * j]) | (uint32_t)__builtin_bit_cast(uint16_t, e[2 * j + 1]) << 16;
+      }
     }
   }
-  // The same where every summed index of the tile exists and, for an operand across it, every row: no checks, offsets made once (rows that are
-  // not there read one that is: they only enter results that are not written).  `whole`: may a tile of these sizes be read so?
-  static __device__ __forceinline__ bool whole(int64_t ld, int rows) { return (ALONG || rows == ROWS) && ld < (1 << 22); }
-  static __device__ __forceinline__ void plain_offsets(uint32_t (&from)[per_thread], int64_t ld, int rows) {
+  // The same with as many loads whatever exists (a load in a branch would have to be waited for at its end): a piece that reaches behind the
+  // operand is read from where it just fits, a row that is not there as one that is, and `mend` puts the elements in their places and zeros
+  // behind the ends.  For operands of at least eight elements either way and ld < 2^22.  `rest`: summed indices from the tile's first on.
+  static constexpr int kBias = BK > ROWS ? BK : ROWS;          // keeps the 32-bit offsets positive where a piece begins in front of the tile
+  static __device__ __forceinline__ void offsets_for(uint32_t (&from)[per_thread], int64_t ld, int rows, int rest) {
 #pragma unroll
     for (int i = 0; i < per_thread; ++i) {
       const int q = min(i * THREADS + (int)threadIdx.x % THREADS, pieces - 1);
-      if constexpr (ALONG) from[i] = ((uint32_t)min(q / (BK / 8), rows - 1) * (uint32_t)ld + (q % (BK / 8)) * 8) * sizeof(T);
-      else from[i] = ((uint32_t)(q / (ROWS / 8)) * (uint32_t)ld + (q % (ROWS / 8)) * 8) * sizeof(T);
+      if constexpr (ALONG) from[i] = ((uint32_t)min(q / (BK / 8), rows - 1) * (uint32_t)ld + (kBias + min(q % (BK / 8) * 8, rest - 8))) * sizeof(T);
+      else from[i] = ((uint32_t)min(q / (ROWS / 8), rest - 1) * (uint32_t)ld + (kBias + min(q % (ROWS / 8) * 8, rows - 8))) * sizeof(T);
     }
   }
-  __device__ __forceinline__ void fetch_whole(const T* p, const uint32_t (&from)[per_thread]) {
+  __device__ __forceinline__ void load(const T* p, const uint32_t (&from)[per_thread]) {
+    const char* base = (const char*)(p - kBias);
+#pragma unroll
+    for (int i = 0; i < per_thread; ++i) reg[i] = load_words<T>(base + from[i]);
+  }
+  static __device__ __forceinline__ bool ragged(int rows, int rest) { return rest < BK || (!ALONG && rows < ROWS); }
+  __device__ __forceinline__ void mend(int rows, int rest) {
 #pragma unroll
     for (int i = 0; i < per_thread; ++i) {
-      Eight<T> e;
-      __builtin_memcpy(&e, (const char*)p + from[i], sizeof(e));
-#pragma unroll
-      for (int k = 0; k < 8; ++k) reg[i][k] = e.v[k];
+      const int q = i * THREADS + (int)threadIdx.x % THREADS;
+      int valid;
+      if constexpr (ALONG) valid = rest - q % (BK / 8) * 8;
+      else valid = q / (ROWS / 8) < rest ? rows - q % (ROWS / 8) * 8 : 0;
+      shift_words<T>(reg[i], valid >= 8 ? 0 : 8 - valid, valid);
     }
   }
   __device__ __forceinline__ void put(char* lds) {
@@ -246,7 +298,7 @@ struct Tile {
       int at;
       if constexpr (ALONG) at = place(q / (BK / 8), (q % (BK / 8)) * 8);
       else at = place((q % (ROWS / 8)) * 8, q / (ROWS / 8));
-      stage8(lds, plane_bytes, at, reg[i]);
+      stage8<T>(lds, plane_bytes, at, reg[i]);
     }
   }
   // The tile straight from memory into LDS, 16 bytes a lane (16-bit operands whose pieces are all aligned): the order of the lanes' pieces in
@@ -496,7 +548,8 @@ __device__ __forceinline__ void write_results(const GroupArgs& a, const Work<T>&
 // ------------------------------------------------------------------------------------------------ the kernel for every case
 // WM of the four waves lie along m.  STAGES tiles are under way in registers ahead of the one that is multiplied (a short summed axis is asked
 // for as a whole, a long one keeps that many times a tile in flight).
-template <typename T, int BM, int BN, int WM, int STAGES, int MODE>
+// SMALL: operands of fewer than eight elements one way or the other, or with longer strides than 32-bit offsets reach.
+template <typename T, int BM, int BN, int WM, int STAGES, bool SMALL, int MODE>
 __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
   typedef typename OperandOf<T>::type O;
   constexpr int BK = OperandOf<T>::bk, P = OperandOf<T>::planes;
@@ -520,24 +573,31 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
 
   TileA ta[STAGES];
   TileB tb[STAGES];
-  const bool whole = TileA::whole(lda, rows_a) && TileB::whole(ldb, rows_b);
   uint32_t from_a[TileA::per_thread], from_b[TileB::per_thread];
-  TileA::plain_offsets(from_a, lda, rows_a);
-  TileB::plain_offsets(from_b, ldb, rows_b);
-  auto fetch = [&](int stage, int k0) {
-    if (k0 >= depth) return;
+  if (!SMALL && depth > 0) {
+    TileA::offsets_for(from_a, lda, rows_a, min(depth, BK));
+    TileB::offsets_for(from_b, ldb, rows_b, min(depth, BK));
+  }
+  auto load = [&](int stage, int k0) {
     const int64_t k = k0;
     const T *p = pa + (MODE == kBackWeight ? k * lda : k), *q = pb + (MODE == kForward ? k : k * ldb);
-    if (whole && k0 + BK <= depth) {
-      ta[stage].fetch_whole(p, from_a);
-      tb[stage].fetch_whole(q, from_b);
-    } else {
+    if constexpr (SMALL) {
       ta[stage].fetch(p, lda, rows_a, depth - k0);
       tb[stage].fetch(q, ldb, rows_b, depth - k0);
+    } else {
+      if (k0 && depth - k0 < BK) {
+        TileA::offsets_for(from_a, lda, rows_a, depth - k0);
+        TileB::offsets_for(from_b, ldb, rows_b, depth - k0);
+      }
+      ta[stage].load(p, from_a);
+      tb[stage].load(q, from_b);
     }
   };
+  const bool deep = depth > (2 * STAGES - 1) * BK;
+  if (deep) {                  // (in the loop that runs on from here every load exists; one that might not would make each wait one for all)
 #pragma unroll
-  for (int d = 0; d < STAGES; ++d) fetch(d, d * BK);
+    for (int d = 0; d < STAGES; ++d) load(d, d * BK);
+  }
   v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int i = 0; i < FM; ++i)
@@ -551,51 +611,75 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
 
   // One barrier a step: the two halves of LDS take turns, so that a wave may put the next tile while another still multiplies this one.
   int half = 0;
-  for (int kb = 0; kb < depth; kb += STAGES * BK) {
+  auto put = [&](int d, int k0) {
+    if constexpr (!SMALL) {
+      if (TileA::ragged(rows_a, depth - k0)) ta[d].mend(rows_a, min(depth - k0, BK));
+      if (TileB::ragged(rows_b, depth - k0)) tb[d].mend(rows_b, min(depth - k0, BK));
+    }
+    ta[d].put(lds + half);
+    tb[d].put(lds + half + TileA::bytes);
+  };
+  auto multiply = [&] {
+    const char *const la = lds + half, *const lb = la + TileA::bytes;
+    half ^= kBuffer;
+#pragma unroll
+    for (int kk = 0; kk < BK; kk += 32) {
+      v8s fb[FN][P];
+#pragma unroll
+      for (int j = 0; j < FN; ++j)
+#pragma unroll
+        for (int q = 0; q < P; ++q) fb[j][q] = TileB::fragment(lb, q, at_b[j], kk);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        v8s fa[P];
+#pragma unroll
+        for (int q = 0; q < P; ++q) fa[q] = TileA::fragment(la, q, at_a[i], kk);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          // the lane's four results are neighbours along n: the n side is the instruction's row operand
+          if constexpr (P == 3) {
+            acc[i][j] = mfma<O>(fb[j][2], fa[0], acc[i][j]);
+            acc[i][j] = mfma<O>(fb[j][0], fa[2], acc[i][j]);
+            acc[i][j] = mfma<O>(fb[j][1], fa[1], acc[i][j]);
+            acc[i][j] = mfma<O>(fb[j][1], fa[0], acc[i][j]);
+            acc[i][j] = mfma<O>(fb[j][0], fa[1], acc[i][j]);
+          }
+          acc[i][j] = mfma<O>(fb[j][0], fa[0], acc[i][j]);
+        }
+        if (MODE == kBackWeight && sum_bias) {
+#pragma unroll
+          for (int q = P - 1; q >= 0; --q) accb = mfma<O>(ones_in_row<O>(i), fa[q], accb);
+        }
+      }
+    }
+  };
+  int kb = 0;
+  if (deep) {
+    for (; kb + (2 * STAGES - 1) * BK < depth; kb += STAGES * BK) {
+#pragma unroll
+      for (int d = 0; d < STAGES; ++d) {
+        put(d, kb + d * BK);
+        __syncthreads();
+        load(d, kb + (d + STAGES) * BK);
+        multiply();
+      }
+    }
+  } else {
+#pragma unroll
+    for (int d = 0; d < STAGES; ++d)
+      if (d * BK < depth) load(d, d * BK);
+  }
+  for (; kb < depth; kb += STAGES * BK) {
 #pragma unroll
     for (int d = 0; d < STAGES; ++d) {
       const int k0 = kb + d * BK;
       if (k0 >= depth) break;
-      char* const la = lds + half;
-      char* const lb = la + TileA::bytes;
-      half ^= kBuffer;
-      ta[d].put(la);
-      tb[d].put(lb);
+      put(d, k0);
       __syncthreads();
-      fetch(d, k0 + STAGES * BK);
-#pragma unroll
-      for (int kk = 0; kk < BK; kk += 32) {
-        v8s fb[FN][P];
-#pragma unroll
-        for (int j = 0; j < FN; ++j)
-#pragma unroll
-          for (int q = 0; q < P; ++q) fb[j][q] = TileB::fragment(lb, q, at_b[j], kk);
-#pragma unroll
-        for (int i = 0; i < FM; ++i) {
-          v8s fa[P];
-#pragma unroll
-          for (int q = 0; q < P; ++q) fa[q] = TileA::fragment(la, q, at_a[i], kk);
-#pragma unroll
-          for (int j = 0; j < FN; ++j) {
-            // the lane's four results are neighbours along n: the n side is the instruction's row operand
-            if constexpr (P == 3) {
-              acc[i][j] = mfma<O>(fb[j][2], fa[0], acc[i][j]);
-              acc[i][j] = mfma<O>(fb[j][0], fa[2], acc[i][j]);
-              acc[i][j] = mfma<O>(fb[j][1], fa[1], acc[i][j]);
-              acc[i][j] = mfma<O>(fb[j][1], fa[0], acc[i][j]);
-              acc[i][j] = mfma<O>(fb[j][0], fa[1], acc[i][j]);
-            }
-            acc[i][j] = mfma<O>(fb[j][0], fa[0], acc[i][j]);
-          }
-          if (MODE == kBackWeight && sum_bias) {
-#pragma unroll
-            for (int q = P - 1; q >= 0; --q) accb = mfma<O>(ones_in_row<O>(i), fa[q], accb);
-          }
-        }
-      }
+      if (k0 + STAGES * BK < depth) load(d, k0 + STAGES * BK);
+      multiply();
     }
   }
-
   write_results<T, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc, accb, sum_bias);
 }
 
@@ -635,39 +719,41 @@ __global__ void __launch_bounds__(512, 2) grouped_f32_kernel(GroupArgs a) {
     // The steps of all tiles are one stream: the loads run two steps ahead of the stores, into the next tile where this one ends.
     TileA ta[STAGES];
     TileB tb[STAGES];
-    bool there[STAGES], whole = false;
+    int rest[STAGES], rows_a[STAGES], rows_b[STAGES];        // rest 0: the stream has ended
     uint32_t from_a[TileA::per_thread], from_b[TileB::per_thread];
     int k0 = 0;
     auto settle = [&](bool fresh) {      // (k0 is a step of w, or there is none left)
       while (!w.none && k0 >= w.depth) { next(w); k0 = 0; fresh = true; }
-      if (!fresh || w.none) return;
-      whole = TileA::whole(w.lda, w.rows_a) && TileB::whole(w.ldb, w.rows_b);
-      TileA::plain_offsets(from_a, w.lda, w.rows_a);
-      TileB::plain_offsets(from_b, w.ldb, w.rows_b);
+      if (w.none || !(fresh || w.depth - k0 < BK)) return;
+      TileA::offsets_for(from_a, w.lda, w.rows_a, min(w.depth - k0, BK));
+      TileB::offsets_for(from_b, w.ldb, w.rows_b, min(w.depth - k0, BK));
     };
-    auto fetch = [&](int stage) {
-      there[stage] = !w.none;
-      if (w.none) return;
-      const int64_t k = k0;
-      const float* pa = (const float*)a.a + (w.pa + (MODE == kBackWeight ? k * w.lda : k));
-      const float* pb = (const float*)a.b + (w.pb + (MODE == kForward ? k : k * w.ldb));
-      if (whole && k0 + BK <= w.depth) {
-        ta[stage].fetch_whole(pa, from_a);
-        tb[stage].fetch_whole(pb, from_b);
-      } else {
-        ta[stage].fetch(pa, w.lda, w.rows_a, w.depth - k0);
-        tb[stage].fetch(pb, w.ldb, w.rows_b, w.depth - k0);
+    int64_t at_pa = 0, at_pb = 0;
+    auto fetch = [&](int d) {
+      rest[d] = w.none ? 0 : min(w.depth - k0, BK);
+      if (!w.none) {
+        rows_a[d] = w.rows_a;
+        rows_b[d] = w.rows_b;
+        at_pa = w.pa + (MODE == kBackWeight ? (int64_t)k0 * w.lda : k0);
+        at_pb = w.pb + (MODE == kForward ? k0 : (int64_t)k0 * w.ldb);
       }
-      k0 += BK;
-      settle(false);
+      ta[d].load((const float*)a.a + at_pa, from_a);      // (behind the stream's end the last step once more: the number of loads under
+      tb[d].load((const float*)a.b + at_pb, from_b);      // way has to be the same on every path, or all of them would be waited for)
+      if (!w.none) {
+        k0 += BK;
+        settle(false);
+      }
     };
     settle(true);
+    if (w.none) return;
 #pragma unroll
     for (int d = 0; d < STAGES; ++d) fetch(d);
     for (bool more = true; more;) {
 #pragma unroll
       for (int d = 0; d < STAGES; ++d) {
-        if (!there[d]) { more = false; break; }
+        if (!rest[d]) { more = false; break; }
+        if (TileA::ragged(rows_a[d], rest[d])) ta[d].mend(rows_a[d], rest[d]);
+        if (TileB::ragged(rows_b[d], rest[d])) tb[d].mend(rows_b[d], rest[d]);
         ta[d].put(lds + half);
         tb[d].put(lds + half + TileA::bytes);
         half ^= kBuffer;
@@ -977,6 +1063,8 @@ static bool large_tiles(int dtype, int64_t m_average, int64_t n, int64_t tiles, 
   return true;
 }
 
+static bool small_operands(int64_t n, int64_t k, int64_t longest) { return n < 8 || k < 8 || longest >= (1 << 22) - 1 || n >= (1 << 22) - 1; }
+
 static bool grouped_dtype(int t) { return t == VC_F32 || t == VC_F16 || t == VC_BF16; }
 
 static int grouped_check(const char* who, int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype, int offset_bits, const void* offsets) {
@@ -997,19 +1085,22 @@ static int launch_rows(const char* who, GroupArgs a, int mode, int dtype, const 
   const uintptr_t size = 2;
   const bool large = p.splits == 1 && large_tiles(dtype, a.groups ? a.rows / a.groups : 0, a.n, cdiv(a.rows, 256) * cdiv(a.n, 256), a.lda > a.n ? a.lda : a.n,
                                                   {(uintptr_t)a.a, (uintptr_t)a.b, (uintptr_t)a.out, (uintptr_t)a.bias, a.lda * size, a.k * size, a.n * size});
-  a.ntiles = (int)cdiv(a.n, large ? 256 : p.bn);
-  const int64_t total = (large ? a.rows / 256 + a.groups + 2 : p.mtiles_most) * a.ntiles * p.splits;
+  const bool small = small_operands(a.n, a.k, a.lda);
+  const int bm = large ? 256 : small ? 64 : p.bm, bn = large ? 256 : small ? 64 : p.bn;
+  a.ntiles = (int)cdiv(a.n, bn);
+  const int64_t total = (a.rows / bm + a.groups + 2) * a.ntiles * p.splits;
   VC_REQUIRE(total < (1LL << 30), "%s: %lld tiles", who, (long long)total);
-  const unsigned blocks = large || p.two_kinds ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
+  const unsigned blocks = large || (p.two_kinds && !small) ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
 #define VC_GO(T, ...)                                                                                                             \
   if (mode == kForward) hipLaunchKernelGGL((grouped_kernel<T, __VA_ARGS__, kForward>), dim3(blocks), dim3(256), 0, st, a);        \
   else hipLaunchKernelGGL((grouped_kernel<T, __VA_ARGS__, kBackInput>), dim3(blocks), dim3(256), 0, st, a);                       \
   if (p.splits > 1) hipLaunchKernelGGL(grouped_row_sum_kernel<T>, dim3((unsigned)cdiv(a.rows * cdiv(a.n, 64), 4)), dim3(256), 0, st, a)
 #define VC_TILES(T)                                       \
-  if (p.bm == 128) { if constexpr (sizeof(T) == 2) { VC_GO(T, 128, 128, 2, 2); } }    \
-  else if (p.bm == 64 && p.bn == 64) { VC_GO(T, 64, 64, 2, 3); }    \
-  else if (p.bm == 64) { VC_GO(T, 64, 128, 2, 2); }                 \
-  else { VC_GO(T, 16, 128, 1, 3); }
+  if (small) { VC_GO(T, 64, 64, 2, 1, true); }                          \
+  else if (p.bm == 128) { if constexpr (sizeof(T) == 2) { VC_GO(T, 128, 128, 2, 2, false); } }    \
+  else if (p.bm == 64 && p.bn == 64) { VC_GO(T, 64, 64, 2, 3, false); }    \
+  else if (p.bm == 64) { VC_GO(T, 64, 128, 2, 2, false); }                 \
+  else { VC_GO(T, 16, 128, 1, 3, false); }
 #define VC_LARGE(T)                                                                                                               \
   if (mode == kForward) hipLaunchKernelGGL((grouped_large_kernel<T, kForward>), dim3(blocks), dim3(512), 0, st, a);              \
   else hipLaunchKernelGGL((grouped_large_kernel<T, kBackInput>), dim3(blocks), dim3(512), 0, st, a)
@@ -1019,8 +1110,8 @@ static int launch_rows(const char* who, GroupArgs a, int mode, int dtype, const 
   if (p.splits > 1) hipLaunchKernelGGL(grouped_row_sum_kernel<float>, dim3((unsigned)cdiv(a.rows * cdiv(a.n, 64), 4)), dim3(256), 0, st, a)
   if (large && dtype == VC_F16) { VC_LARGE(_Float16); }
   else if (large) { VC_LARGE(__bf16); }
-  else if (p.two_kinds && p.bm == 192) { VC_PIECES(192); }
-  else if (p.two_kinds) { VC_PIECES(128); }
+  else if (!small && p.two_kinds && p.bm == 192) { VC_PIECES(192); }
+  else if (!small && p.two_kinds) { VC_PIECES(128); }
   else if (dtype == VC_F32) { VC_TILES(float) } else if (dtype == VC_F16) { VC_TILES(_Float16) } else { VC_TILES(__bf16) }
 #undef VC_PIECES
 #undef VC_LARGE
@@ -1091,20 +1182,22 @@ int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const voi
   const uintptr_t size = 2;
   const bool large = p.splits == 1 && large_tiles(dtype, out, in, groups * cdiv(out, 256) * cdiv(in, 256), x_stride > dy_stride ? x_stride : dy_stride,
                                                   {(uintptr_t)x, (uintptr_t)dy, (uintptr_t)dweight, x_stride * size, dy_stride * size, in * size, out * size});
-  a.mtiles = (int)cdiv(out, large ? 256 : p.bm); a.ntiles = (int)cdiv(in, large ? 256 : p.bn);
+  const bool small = small_operands(out, in, x_stride > dy_stride ? x_stride : dy_stride);
+  a.mtiles = (int)cdiv(out, large ? 256 : small ? 64 : p.bm); a.ntiles = (int)cdiv(in, large ? 256 : small ? 64 : p.bn);
   a.partial = (float*)workspace;
   a.partial_bias = a.partial + p.mtiles_most * out * in;
   const int64_t tiles = (int64_t)a.mtiles * a.ntiles;
   // without splits every XCD takes an eighth of each group's tiles
   const int64_t total = p.splits == 1 && tiles >= 8 ? cdiv(tiles, 8) * 8 * groups : p.mtiles_most * tiles;
   VC_REQUIRE(total < (1LL << 30), "%s: %lld tiles", who, (long long)total);
-  const unsigned blocks = large || p.two_kinds ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
+  const unsigned blocks = large || (p.two_kinds && !small) ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
   hipStream_t st = (hipStream_t)stream;
   const int64_t sum_blocks = cdiv(out * in + out, 64);
 #define VC_GO(T)                                                                                                                              \
-  if (p.two_kinds) hipLaunchKernelGGL((grouped_f32_kernel<128, 128, kBackWeight>), dim3(blocks), dim3(512), 0, st, a);                        \
-  else if (p.bm == 128) { if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((grouped_kernel<T, 128, 128, 2, 2, kBackWeight>), dim3(blocks), dim3(256), 0, st, a); } \
-  else hipLaunchKernelGGL((grouped_kernel<T, 64, 64, 2, 3, kBackWeight>), dim3(blocks), dim3(256), 0, st, a);                                      \
+  if (small) hipLaunchKernelGGL((grouped_kernel<T, 64, 64, 2, 1, true, kBackWeight>), dim3(blocks), dim3(256), 0, st, a);                     \
+  else if (p.two_kinds) hipLaunchKernelGGL((grouped_f32_kernel<128, 128, kBackWeight>), dim3(blocks), dim3(512), 0, st, a);                        \
+  else if (p.bm == 128) { if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((grouped_kernel<T, 128, 128, 2, 2, false, kBackWeight>), dim3(blocks), dim3(256), 0, st, a); } \
+  else hipLaunchKernelGGL((grouped_kernel<T, 64, 64, 2, 3, false, kBackWeight>), dim3(blocks), dim3(256), 0, st, a);                                      \
   if (p.splits > 1)                                                                                                                           \
     hipLaunchKernelGGL(grouped_weight_sum_kernel<T>, dim3((unsigned)(sum_blocks < 16384 ? sum_blocks : 16384), (unsigned)groups), dim3(256), 0, st, a)
   if (large && dtype == VC_F16) hipLaunchKernelGGL((grouped_large_kernel<_Float16, kBackWeight>), dim3(blocks), dim3(512), 0, st, a);
