@@ -17,8 +17,6 @@
 
 namespace vc {
 
-template <typename T> __device__ __forceinline__ float up(T x) { return (float)x; }
-
 template <typename T, int VEC> struct __attribute__((packed, aligned(sizeof(T)))) Pack { T v[VEC]; };
 
 template <typename T, int VEC>
@@ -47,21 +45,52 @@ __device__ __forceinline__ void load_weight(const void* w, int wtype, int64_t c,
   else load_vec<__bf16, VEC>((const __bf16*)w + c, out);
 }
 
-// the sum over the LPR lanes of a row (LPR a power of two up to 64: within the wave; else over the block), the same in every lane
+template <int CTRL>
+__device__ __forceinline__ float plus_moved(float x) {
+  return x + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane_of(float x, int l) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), l)); }
+
+// the sum over min(LPR, 64) neighbouring lanes, the same in each of them: exchanges within a row of 16 lanes, then between the rows
 template <int LPR>
-__device__ __forceinline__ float row_sum(float x, float* lds) {
+__device__ __forceinline__ float lane_sum(float x) {
+  if constexpr (LPR >= 2) x = plus_moved<0xb1>(x);     // neighbours
+  if constexpr (LPR >= 4) x = plus_moved<0x4e>(x);     // pairs
+  if constexpr (LPR >= 8) x = plus_moved<0x141>(x);    // mirrored in eight
+  if constexpr (LPR >= 16) x = plus_moved<0x140>(x);   // mirrored in sixteen
+  if constexpr (LPR == 32) x += __shfl_xor(x, 16, 64);
+  if constexpr (LPR >= 64) x = (lane_of(x, 0) + lane_of(x, 16)) + (lane_of(x, 32) + lane_of(x, 48));
+  return x;
+}
+
+// N sums over the LPR lanes of a row, the same in each of them; rows of several waves meet in LDS: one barrier, the halves of `lds` in turn
+template <int LPR, int ROWS, int N>
+struct RowSums {
+  static constexpr int W = LPR > 64 ? LPR / 64 : 1;
+  float lds[2][ROWS][N][W];
+};
+template <int LPR, int ROWS, int N, int M>
+__device__ __forceinline__ void row_sums(float (&x)[M], RowSums<LPR, ROWS, N>& shared, int& half) {
+  static_assert(M <= N, "room for the sums");
 #pragma unroll
-  for (int off = 1; off < (LPR < 64 ? LPR : 64); off <<= 1) x += __shfl_xor(x, off, 64);
+  for (int i = 0; i < M; ++i) x[i] = lane_sum<LPR>(x[i]);
   if constexpr (LPR > 64) {
     constexpr int W = LPR / 64;
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = x;
-    __syncthreads();
-    x = 0.f;
+    const int r = threadIdx.x / LPR, w = threadIdx.x % LPR / 64;
+    if ((threadIdx.x & 63) == 0) {
 #pragma unroll
-    for (int i = 0; i < W; ++i) x += lds[i];
+      for (int i = 0; i < M; ++i) shared.lds[half][r][i][w] = x[i];
+    }
     __syncthreads();
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+      float s = 0.f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) s += shared.lds[half][r][i][j];
+      x[i] = s;
+    }
+    half ^= 1;
   }
-  return x;
 }
 
 struct NormArgs {
@@ -77,74 +106,87 @@ struct NormArgs {
 template <int VEC>
 __device__ __forceinline__ int vec_at(int j, int c, int& first) {
   const int at = min(j * VEC, c - VEC);
-  first = j * VEC - at;
+  first = j * VEC - at;         // VEC or more: the row has no such vector (it is read all the same, and counts for nothing)
   return at;
 }
 
-template <typename T, int VEC, int LPR, int ITER>
-__global__ void __launch_bounds__(LPR > 256 ? LPR : 256) norm_forward_kernel(NormArgs a) {
-  constexpr int kThreads = LPR > 256 ? LPR : 256, kRows = kThreads / LPR;
-  __shared__ float lds[LPR > 64 ? LPR / 64 : 1];
-  const int lane = threadIdx.x % LPR;
-  const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / LPR;
-  if (row >= a.n) return;   // (a whole block where a row is one; the lanes of a row leave together)
-  const T* x = (const T*)a.x + row * a.stride;
-  float v[ITER][VEC];
-  int at[ITER], first[ITER];
-  float s = 0.f;
+// A block takes rows until there are none: the weights are read once (a row of 4096 16-bit channels is 8 KB, its two fp32 weights 32 KB), and the
+// next row is under way while this one is summed.
+template <typename T, int VEC, int LPR, int ITER, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_forward_kernel(NormArgs a) {
+  constexpr int kRows = THREADS / LPR;
+  __shared__ RowSums<LPR, kRows, 1> shared;
+  const int lane = threadIdx.x % LPR, mine = threadIdx.x / LPR;
+  int at[ITER], first[ITER], half = 0;
+  float w[ITER][VEC], b[ITER][VEC];
+  Pack<T, VEC> next[ITER];
+  const int64_t step = (int64_t)gridDim.x * kRows;
+  auto ask = [&](int64_t row) {     // (behind the last row, that one again)
+    const T* x = (const T*)a.x + min(row, a.n - 1) * a.stride;
+#pragma unroll
+    for (int j = 0; j < ITER; ++j) __builtin_memcpy(&next[j], x + at[j], sizeof(next[j]));
+  };
 #pragma unroll
   for (int j = 0; j < ITER; ++j) {
     at[j] = vec_at<VEC>(j * LPR + lane, a.c, first[j]);
-    if (first[j] < VEC) load_vec<T, VEC>(x + at[j], v[j]);
+    load_weight<VEC>(a.w, a.wtype, at[j], 1.f, w[j]);
+    load_weight<VEC>(a.b, a.btype, at[j], 0.f, b[j]);
   }
+  ask((int64_t)blockIdx.x * kRows + mine);
+  for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.n; base += step) {
+    const int64_t row = base + mine;
+    float v[ITER][VEC], sum[1] = {0.f};
 #pragma unroll
-  for (int j = 0; j < ITER; ++j)
-    if (first[j] < VEC) {
+    for (int j = 0; j < ITER; ++j)
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) s += k >= first[j] ? v[j][k] : 0.f;
-    }
-  const float inv = 1.f / (float)a.c;
-  const float mean = row_sum<LPR>(s, lds) / (float)a.c;
-  float q = 0.f;
+      for (int k = 0; k < VEC; ++k) {
+        v[j][k] = (float)next[j].v[k];
+        sum[0] += k >= first[j] ? v[j][k] : 0.f;
+      }
+    ask(row + step);
+    row_sums(sum, shared, half);
+    const float mean = sum[0] / (float)a.c;
+    sum[0] = 0.f;
 #pragma unroll
-  for (int j = 0; j < ITER; ++j)
-    if (first[j] < VEC) {
+    for (int j = 0; j < ITER; ++j)
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         v[j][k] -= mean;
-        q += k >= first[j] ? v[j][k] * v[j][k] : 0.f;
+        sum[0] += k >= first[j] ? v[j][k] * v[j][k] : 0.f;
       }
-    }
-  const float rstd = 1.f / sqrtf(row_sum<LPR>(q, lds) * inv + a.eps);
-  T* y = (T*)a.y + row * a.c;
+    row_sums(sum, shared, half);
+    const float rstd = 1.f / sqrtf(sum[0] / (float)a.c + a.eps);
+    if (row >= a.n) continue;
+    T* y = (T*)a.y + row * a.c;
 #pragma unroll
-  for (int j = 0; j < ITER; ++j)
-    if (first[j] < VEC) {
-      float w[VEC], b[VEC];
-      load_weight<VEC>(a.w, a.wtype, at[j], 1.f, w);
-      load_weight<VEC>(a.b, a.btype, at[j], 0.f, b);
+    for (int j = 0; j < ITER; ++j)
+      if (first[j] < VEC) {
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) v[j][k] = v[j][k] * rstd * w[k] + b[k];
-      store_vec<T, VEC>(y + at[j], v[j]);
+        for (int k = 0; k < VEC; ++k) v[j][k] = v[j][k] * rstd * w[j][k] + b[j][k];
+        store_vec<T, VEC>(y + at[j], v[j]);
+      }
+    if (a.mean && lane == 0) {
+      a.mean[row] = mean;
+      a.rstd[row] = rstd;
     }
-  if (a.mean && lane == 0) {
-    a.mean[row] = mean;
-    a.rstd[row] = rstd;
   }
 }
 
 // rows wider than a block's registers: three walks over the row
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_forward_wide_kernel(NormArgs a) {
-  __shared__ float lds[16];
+  __shared__ RowSums<1024, 1, 1> shared;
   const int64_t row = blockIdx.x;
   const T* x = (const T*)a.x + row * a.stride;
-  float s = 0.f, q = 0.f;
-  for (int c = threadIdx.x; c < a.c; c += 1024) s += (float)x[c];
-  const float inv = 1.f / (float)a.c;
-  const float mean = row_sum<1024>(s, lds) / (float)a.c;
-  for (int c = threadIdx.x; c < a.c; c += 1024) { const float d = (float)x[c] - mean; q += d * d; }
-  const float rstd = 1.f / sqrtf(row_sum<1024>(q, lds) * inv + a.eps);
+  int half = 0;
+  float sum[1] = {0.f};
+  for (int c = threadIdx.x; c < a.c; c += 1024) sum[0] += (float)x[c];
+  row_sums(sum, shared, half);
+  const float mean = sum[0] / (float)a.c;
+  sum[0] = 0.f;
+  for (int c = threadIdx.x; c < a.c; c += 1024) { const float d = (float)x[c] - mean; sum[0] += d * d; }
+  row_sums(sum, shared, half);
+  const float rstd = 1.f / sqrtf(sum[0] / (float)a.c + a.eps);
   T* y = (T*)a.y + row * a.c;
   for (int c = threadIdx.x; c < a.c; c += 1024) {
     float w[1], b[1];
@@ -167,51 +209,58 @@ struct NormBackArgs {
   int c, wtype;
 };
 
-template <typename T, int VEC, int LPR, int ITER>
-__global__ void __launch_bounds__(LPR > 256 ? LPR : 256) norm_backward_kernel(NormBackArgs a) {
-  constexpr int kThreads = LPR > 256 ? LPR : 256, kRows = kThreads / LPR;
-  __shared__ float lds[LPR > 64 ? LPR / 64 : 1];
-  __shared__ float sums[LPR < kThreads ? kThreads * VEC * 2 : 1];
-  const int lane = threadIdx.x % LPR;
-  int at[ITER], first[ITER];
+template <typename T, int VEC, int LPR, int ITER, int THREADS>
+__global__ void __launch_bounds__(THREADS) norm_backward_kernel(NormBackArgs a) {
+  constexpr int kRows = THREADS / LPR;
+  __shared__ RowSums<LPR, kRows, 2> shared;
+  __shared__ float sums[kRows > 1 ? THREADS * VEC * 2 : 1];
+  const int lane = threadIdx.x % LPR, mine = threadIdx.x / LPR;
+  int at[ITER], first[ITER], half = 0;
   float w[ITER][VEC], dw[ITER][VEC], db[ITER][VEC];
+  Pack<T, VEC> nx[ITER], ny[ITER];
+  float nmean, nrstd;
 #pragma unroll
   for (int j = 0; j < ITER; ++j) {
     at[j] = vec_at<VEC>(j * LPR + lane, a.c, first[j]);
-    if (first[j] < VEC) load_weight<VEC>(a.w, a.wtype, at[j], 1.f, w[j]);
+    load_weight<VEC>(a.w, a.wtype, at[j], 1.f, w[j]);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) dw[j][k] = db[j][k] = 0.f;
   }
-  const float inv = 1.f / (float)a.c;
   const int64_t begin = (int64_t)blockIdx.x * a.rows_per_block, end = min(begin + a.rows_per_block, a.n);
-  for (int64_t row = begin + threadIdx.x / LPR; row < end; row += kRows) {
+  auto ask = [&](int64_t r) {     // (behind the last row, that one again)
+    const int64_t row = min(r, a.n - 1);
     const T* x = (const T*)a.x + row * a.stride;
     const T* dy = (const T*)a.dy + row * a.dystride;
-    const float mean = a.mean[row], rstd = a.rstd[row];
-    float h[ITER][VEC], g[ITER][VEC];
-    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int j = 0; j < ITER; ++j) {
+      __builtin_memcpy(&nx[j], x + at[j], sizeof(nx[j]));
+      __builtin_memcpy(&ny[j], dy + at[j], sizeof(ny[j]));
+    }
+    nmean = a.mean[row];
+    nrstd = a.rstd[row];
+  };
+  ask(begin + mine);
+  for (int64_t base = begin; base < end; base += kRows) {
+    const int64_t row = base + mine;
+    const bool live = row < end;
+    const float mean = nmean, rstd = nrstd;
+    float h[ITER][VEC], g[ITER][VEC], sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < ITER; ++j)
-      if (first[j] < VEC) {
-        load_vec<T, VEC>(x + at[j], h[j]);
-        load_vec<T, VEC>(dy + at[j], g[j]);
-      }
 #pragma unroll
-    for (int j = 0; j < ITER; ++j)
-      if (first[j] < VEC) {
-#pragma unroll
-        for (int k = 0; k < VEC; ++k) {
-          h[j][k] = (h[j][k] - mean) * rstd;
-          dw[j][k] += g[j][k] * h[j][k];
-          db[j][k] += g[j][k];
-          g[j][k] *= w[j][k];
-          s += k >= first[j] ? g[j][k] : 0.f;
-          q += k >= first[j] ? g[j][k] * h[j][k] : 0.f;
-        }
+      for (int k = 0; k < VEC; ++k) {
+        h[j][k] = ((float)nx[j].v[k] - mean) * rstd;
+        const float d = live ? (float)ny[j].v[k] : 0.f;
+        dw[j][k] += live ? d * h[j][k] : 0.f;      // (a row that is not there must not bring in 0 times something undefined)
+        db[j][k] += d;
+        g[j][k] = d * w[j][k];
+        sum[0] += k >= first[j] ? g[j][k] : 0.f;
+        sum[1] += k >= first[j] ? g[j][k] * h[j][k] : 0.f;
       }
-    s = row_sum<LPR>(s, lds) * inv;
-    q = row_sum<LPR>(q, lds) * inv;
-    if (a.dx) {
+    ask(row + kRows);
+    row_sums(sum, shared, half);
+    const float s = sum[0] / (float)a.c, q = sum[1] / (float)a.c;
+    if (a.dx && live) {
       T* dx = (T*)a.dx + row * a.c;
 #pragma unroll
       for (int j = 0; j < ITER; ++j)
@@ -239,14 +288,14 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256) norm_backward_kernel(No
       __syncthreads();
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
-        sums[(2 * k) * kThreads + threadIdx.x] = dw[j][k];
-        sums[(2 * k + 1) * kThreads + threadIdx.x] = db[j][k];
+        sums[(2 * k) * THREADS + threadIdx.x] = dw[j][k];
+        sums[(2 * k + 1) * THREADS + threadIdx.x] = db[j][k];
       }
       __syncthreads();
-      for (int i = threadIdx.x; i < LPR * VEC * 2; i += kThreads) {
+      for (int i = threadIdx.x; i < LPR * VEC * 2; i += THREADS) {
         const int l = i % LPR, k2 = i / LPR;
         float s = 0.f;
-        for (int r = 0; r < kRows; ++r) s += sums[k2 * kThreads + r * LPR + l];
+        for (int r = 0; r < kRows; ++r) s += sums[k2 * THREADS + r * LPR + l];
         int f;
         const int col = vec_at<VEC>(j * LPR + l, a.c, f);
         if ((k2 >> 1) >= f) out[(k2 & 1) * a.c + col + (k2 >> 1)] = s;
@@ -257,20 +306,21 @@ __global__ void __launch_bounds__(LPR > 256 ? LPR : 256) norm_backward_kernel(No
 
 template <typename T>
 __global__ void __launch_bounds__(1024) norm_backward_wide_kernel(NormBackArgs a) {   // dx only; the sums have a kernel of their own
-  __shared__ float lds[16];
+  __shared__ RowSums<1024, 1, 2> shared;
   const int64_t row = blockIdx.x;
   const T* x = (const T*)a.x + row * a.stride;
   const T* dy = (const T*)a.dy + row * a.dystride;
-  const float mean = a.mean[row], rstd = a.rstd[row], inv = 1.f / (float)a.c;
-  float s = 0.f, q = 0.f, w[1];
+  const float mean = a.mean[row], rstd = a.rstd[row];
+  int half = 0;
+  float sum[2] = {0.f, 0.f}, w[1];
   for (int c = threadIdx.x; c < a.c; c += 1024) {
     load_weight<1>(a.w, a.wtype, c, 1.f, w);
     const float g = (float)dy[c] * w[0];
-    s += g;
-    q += g * (((float)x[c] - mean) * rstd);
+    sum[0] += g;
+    sum[1] += g * (((float)x[c] - mean) * rstd);
   }
-  s = row_sum<1024>(s, lds) * inv;
-  q = row_sum<1024>(q, lds) * inv;
+  row_sums(sum, shared, half);
+  const float s = sum[0] / (float)a.c, q = sum[1] / (float)a.c;
   T* dx = (T*)a.dx + row * a.c;
   for (int c = threadIdx.x; c < a.c; c += 1024) {
     load_weight<1>(a.w, a.wtype, c, 1.f, w);
@@ -330,36 +380,42 @@ __global__ void __launch_bounds__(256) norm_param_grad_kernel(const float* __res
 
 // how a row of c elements is held: VEC elements a vector, LPR lanes, ITER vectors a lane; iter 0: wider than a block's registers
 struct NormShape { int vec, lpr, iter; };
-static NormShape norm_shape(int64_t c, int dtype) {
+static NormShape norm_shape(int64_t c, int dtype, bool backward) {
   const int full = dtype == VC_F32 ? 4 : 8;
   if (c < full) return {1, 8, 1};
   const int64_t vecs = cdiv(c, full);
   for (int lpr = 2; lpr <= 64; lpr *= 2)
     if (vecs <= lpr) return {full, lpr, 1};
   if (vecs <= 128) return {full, 64, 2};
+  // (two vectors a lane hide more latency in the forward pass; the backward pass, which holds five values an element, would spill)
   for (int lpr = 256; lpr <= 1024; lpr *= 2)
-    if (vecs <= 2 * lpr) return {full, lpr, vecs <= lpr ? 1 : 2};
+    if (vecs <= (backward ? 1 : 2) * lpr) return {full, lpr, vecs <= lpr ? 1 : 2};
+  if (vecs <= 2048) return {full, 1024, 2};
   if (dtype == VC_F32 && vecs <= 4096) return {full, 1024, 4};
   return {1, 1024, 0};
 }
 
-static int64_t norm_blocks(int64_t n, int64_t c, const NormShape& s) {   // blocks of the backward pass = rows of its partial sums
-  const int rows = s.iter ? (s.lpr > 256 ? 1 : 256 / s.lpr) : 1;
-  const int64_t most = s.lpr > 256 ? 512 : 1024;
-  int64_t b = cdiv(n, rows);
-  if (!s.iter) b = cdiv(n, 64);
+// Blocks of the backward pass = rows of its partial sums: one of 1024 threads a compute unit for rows of several waves (each block's column sums are
+// written and read once more: at 4096 channels 1024 blocks of 256 threads would add 67 MB to the 402 MB of 16381 rows), four of 256 for
+// shorter ones.
+static int back_threads(const NormShape& s) { return s.lpr > 64 ? 1024 : 256; }
+static int64_t norm_blocks(int64_t n, int64_t c, const NormShape& s) {
+  const int rows = s.iter ? back_threads(s) / s.lpr : 64;
+  const int64_t most = s.lpr > 64 ? (s.iter ? 256 : 512) : 1024, b = cdiv(n, rows);
   return b < most ? (b > 0 ? b : 1) : most;
 }
 
 template <typename T> struct FullVec { static constexpr int value = sizeof(T) == 4 ? 4 : 8; };
 
-#define VC_NORM_SHAPES(DO)                                                                                                                  \
+// DO: in both directions, ONE: in the backward pass, TWO: in the forward pass
+#define VC_NORM_SHAPES(DO, ONE, TWO)                                                                                                                  \
   if (s.vec == 1) { DO(1, 8, 1); }                                                                                                          \
   else if (s.lpr == 2) { DO(V, 2, 1); } else if (s.lpr == 4) { DO(V, 4, 1); } else if (s.lpr == 8) { DO(V, 8, 1); }                         \
   else if (s.lpr == 16) { DO(V, 16, 1); } else if (s.lpr == 32) { DO(V, 32, 1); }                                                           \
   else if (s.lpr == 64 && s.iter == 1) { DO(V, 64, 1); } else if (s.lpr == 64) { DO(V, 64, 2); }                                            \
-  else if (s.lpr == 256 && s.iter == 1) { DO(V, 256, 1); } else if (s.lpr == 256) { DO(V, 256, 2); }                                        \
-  else if (s.lpr == 512) { DO(V, 512, 2); } else if (s.iter <= 2) { DO(V, 1024, 2); } else if constexpr (V == 4) { DO(V, 1024, 4); }
+  else if (s.lpr == 256 && s.iter == 1) { DO(V, 256, 1); } else if (s.lpr == 256) { TWO(V, 256, 2); }                                       \
+  else if (s.lpr == 512 && s.iter == 1) { ONE(V, 512, 1); } else if (s.lpr == 512) { TWO(V, 512, 2); }                                      \
+  else if (s.iter == 1) { ONE(V, 1024, 1); } else if (s.iter == 2) { DO(V, 1024, 2); } else if constexpr (V == 4) { DO(V, 1024, 4); }
 
 template <typename T>
 static void norm_forward_launch(const NormArgs& a, const NormShape& s, hipStream_t st) {
@@ -368,10 +424,15 @@ static void norm_forward_launch(const NormArgs& a, const NormShape& s, hipStream
     hipLaunchKernelGGL(norm_forward_wide_kernel<T>, dim3((unsigned)a.n), dim3(1024), 0, st, a);
     return;
   }
+  // as many blocks as the chip holds (2048 threads a compute unit), or as there are rows for
   const int threads = s.lpr > 256 ? s.lpr : 256;
-  const unsigned blocks = (unsigned)cdiv(a.n, threads / s.lpr);
-#define VC_DO(VEC, LPR, ITER) hipLaunchKernelGGL((norm_forward_kernel<T, VEC, LPR, ITER>), dim3(blocks), dim3(threads), 0, st, a)
-  VC_NORM_SHAPES(VC_DO)
+  const int64_t most = 256 * (2048 / threads), need = cdiv(a.n, threads / s.lpr);
+  const unsigned blocks = (unsigned)(need < most ? need : most);
+#define VC_DO(VEC, LPR, ITER)                                                                                                               \
+  hipLaunchKernelGGL((norm_forward_kernel<T, VEC, LPR, ITER, (LPR > 256 ? LPR : 256)>), dim3(blocks), dim3(threads), 0, st, a)
+#define VC_NO(...)
+  VC_NORM_SHAPES(VC_DO, VC_NO, VC_DO)
+#undef VC_NO
 #undef VC_DO
 }
 
@@ -383,9 +444,11 @@ static void norm_backward_launch(const NormBackArgs& a, const NormShape& s, int6
     if (a.partial) hipLaunchKernelGGL(norm_column_sums_kernel<T>, dim3((unsigned)cdiv(a.c, 256), (unsigned)blocks), dim3(256), 0, st, a);
     return;
   }
-  const int threads = s.lpr > 256 ? s.lpr : 256;
-#define VC_DO(VEC, LPR, ITER) hipLaunchKernelGGL((norm_backward_kernel<T, VEC, LPR, ITER>), dim3((unsigned)blocks), dim3(threads), 0, st, a)
-  VC_NORM_SHAPES(VC_DO)
+#define VC_DO(VEC, LPR, ITER)                                                                                                               \
+  hipLaunchKernelGGL((norm_backward_kernel<T, VEC, LPR, ITER, (LPR > 64 ? 1024 : 256)>), dim3((unsigned)blocks), dim3(back_threads(s)), 0, st, a)
+#define VC_NO(...)
+  VC_NORM_SHAPES(VC_DO, VC_DO, VC_NO)
+#undef VC_NO
 #undef VC_DO
 }
 
@@ -406,7 +469,7 @@ int vc_layer_norm_forward(const void* x, int64_t x_stride, int64_t n, int64_t c,
   if (n == 0) return VC_OK;
   VC_REQUIRE(x && y, "vc_layer_norm_forward: NULL pointer");
   NormArgs a{x, weight, bias, y, mean, rstd, n, x_stride, (int)c, weight_dtype, bias_dtype, eps};
-  const NormShape s = norm_shape(c, dtype);
+  const NormShape s = norm_shape(c, dtype, false);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == VC_F32) norm_forward_launch<float>(a, s, st);
   else if (dtype == VC_F16) norm_forward_launch<_Float16>(a, s, st);
@@ -417,7 +480,7 @@ int vc_layer_norm_forward(const void* x, int64_t x_stride, int64_t n, int64_t c,
 
 size_t vc_layer_norm_backward_workspace_bytes(int64_t n, int64_t c, int dtype) {
   if (n <= 0 || c <= 0 || !known_dtype(dtype)) return 0;
-  return (size_t)norm_blocks(n, c, norm_shape(c, dtype)) * 2 * (size_t)c * sizeof(float);
+  return (size_t)norm_blocks(n, c, norm_shape(c, dtype, true)) * 2 * (size_t)c * sizeof(float);
 }
 
 int vc_layer_norm_backward(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, int64_t n, int64_t c, int dtype,
@@ -428,7 +491,7 @@ int vc_layer_norm_backward(const void* x, int64_t x_stride, const void* dy, int6
   VC_REQUIRE((x_stride >= c && dy_stride >= c) || n <= 1, "vc_layer_norm_backward: row stride below %lld columns", (long long)c);
   hipStream_t st = (hipStream_t)stream;
   const bool sums = dweight || dbias;
-  const NormShape s = norm_shape(c, dtype);
+  const NormShape s = norm_shape(c, dtype, true);
   const int64_t blocks = norm_blocks(n, c, s);
   if (n > 0) {
     VC_REQUIRE(x && dy && mean && rstd, "vc_layer_norm_backward: NULL pointer");
