@@ -22,6 +22,7 @@ namespace vc {
 typedef short v4s __attribute__((ext_vector_type(4)));
 typedef short v8s __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
@@ -358,12 +359,20 @@ __device__ __forceinline__ v4f mfma(v8s a, v8s b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-// Ones in row i of a 16-row operand, zeros in the others: its product with an operand adds that one up along the summed axis, into row i of an
-// accumulator that the sums of sixteen operands fit in.
-template <typename T>
-__device__ __forceinline__ v8s ones_in_row(int i) {
-  const short one = (threadIdx.x & 15) != (unsigned)i ? (short)0 : __is_same(T, _Float16) ? (short)0x3c00 : (short)0x3f80;
-  return v8s{one, one, one, one, one, one, one, one};
+// accb += the sums of FM operands of a tile along the summed axis (dbias from dy): operand i times ones in row i, so that the sums of sixteen
+// operands fit in one accumulator.  It reads its operands once more: between the other products it would cut those into pieces that wait for
+// their own reads (weight product with a bias or without, 8192^3: 1010 TFLOP/s so).
+template <typename T, typename Tile, int FM>
+__device__ __forceinline__ void add_bias_sums(const char* lds, const int (&at)[FM], v4f& accb) {
+#pragma unroll 1
+  for (int kk = 0; kk < Tile::BK; kk += 32)
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const short one = (threadIdx.x & 15) != (unsigned)i ? (short)0 : __is_same(T, _Float16) ? (short)0x3c00 : (short)0x3f80;
+#pragma unroll
+      for (int q = Tile::planes - 1; q >= 0; --q)
+        accb = mfma<T>(v8s{one, one, one, one, one, one, one, one}, Tile::fragment(lds, q, at[i], kk), accb);
+    }
 }
 
 template <typename T> __device__ __forceinline__ void store4(T* p, int valid, const float (&x)[4]) {
@@ -459,6 +468,7 @@ __device__ __forceinline__ Work<T> find_work(const GroupArgs& a, Groups& g, cons
     const unsigned tiles = (unsigned)a.mtiles * a.ntiles;
     unsigned t;
     int64_t r0, r1;
+    bool pieces = false;         // the sums of a group of one piece are its result
     if (a.splits > 1) {          // pieces of per_split rows, their sums added by grouped_weight_sum_kernel
       const unsigned id = items.first + l;
       t = id % tiles;
@@ -468,6 +478,7 @@ __device__ __forceinline__ Work<T> find_work(const GroupArgs& a, Groups& g, cons
       w.group = at.group;
       r0 = at.begin + (int64_t)at.tile * a.per_split;
       r1 = min(r0 + a.per_split, (int64_t)at.end);
+      pieces = at.end - at.begin > a.per_split;
     } else {
       const unsigned share = (tiles + 7) / 8;
       const unsigned r = tiles >= 8 ? l / share : (l * 8 + x) / tiles;
@@ -480,7 +491,7 @@ __device__ __forceinline__ Work<T> find_work(const GroupArgs& a, Groups& g, cons
     }
     w.n0 = (int)(t % a.ntiles) * BN;
     w.m0 = (int64_t)(t / a.ntiles) * BM;
-    if (a.splits > 1) w.partial = a.partial + ((int64_t)w.piece * a.m + w.m0) * a.n + w.n0;
+    if (pieces) w.partial = a.partial + ((int64_t)w.piece * a.m + w.m0) * a.n + w.n0;
     w.depth = (int)(r1 - r0);
     w.rows_a = (int)min((int64_t)BM, (int64_t)a.m - w.m0);
     w.lda = a.lda;
@@ -569,7 +580,7 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
   const T *const pa = (const T*)a.a + w.pa, *const pb = (const T*)a.b + w.pb;
   const int64_t lda = w.lda, ldb = w.ldb;
   const int rows_a = w.rows_a, rows_b = w.rows_b, depth = w.depth;
-  const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && wn == 0;
+  const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && __builtin_amdgcn_readfirstlane(wn) == 0;
 
   TileA ta[STAGES];
   TileB tb[STAGES];
@@ -646,12 +657,9 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
           }
           acc[i][j] = mfma<O>(fb[j][0], fa[0], acc[i][j]);
         }
-        if (MODE == kBackWeight && sum_bias) {
-#pragma unroll
-          for (int q = P - 1; q >= 0; --q) accb = mfma<O>(ones_in_row<O>(i), fa[q], accb);
-        }
       }
     }
+    if (MODE == kBackWeight && sum_bias) add_bias_sums<O, TileA>(la, at_a, accb);
   };
   int kb = 0;
   if (deep) {
@@ -803,11 +811,8 @@ __global__ void __launch_bounds__(512, 2) grouped_f32_kernel(GroupArgs a) {
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma<__bf16>(fb[j][0], fa[1], acc[i][j]);
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma<__bf16>(fb[j][0], fa[0], acc[i][j]);
-        if (MODE == kBackWeight && sum_bias) {
-#pragma unroll
-          for (int q = P - 1; q >= 0; --q) accb = mfma<__bf16>(ones_in_row<__bf16>(i), fa[q], accb);
-        }
       }
+      if (MODE == kBackWeight && sum_bias) add_bias_sums<__bf16, TileA>(la, at_a, accb);
     }
     write_results<float, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc, accb, sum_bias);
     next(w);
@@ -875,7 +880,7 @@ __global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
   next(w);
   begin(w);
   while (!w.none) {
-    const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && wn0 == 0;
+    const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && __builtin_amdgcn_readfirstlane(wn0) == 0;
     v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
@@ -885,19 +890,24 @@ __global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
       for (int i = 0; i < FM; ++i) acc[i][j] = start;
     }
     auto multiply = [&](const char* lds) {
+      v8s fb[2][FN], fa[2];
 #pragma unroll
-      for (int kk = 0; kk < BK; kk += 32) {
-        v8s fb[FN];
+      for (int j = 0; j < FN; ++j) fb[0][j] = TileB::fragment(lds + TileA::bytes, 0, at_b[j], 0);
+      fa[0] = TileA::fragment(lds, 0, at_a[0], 0);
 #pragma unroll
-        for (int j = 0; j < FN; ++j) fb[j] = TileB::fragment(lds + TileA::bytes, 0, at_b[j], kk);
+      for (int q = 0; q < BK / 32 * FM; ++q) {
+        const int i = q % FM, h = q / FM, kk = h * 32;
+        if (i + 1 < FM) fa[(q + 1) & 1] = TileA::fragment(lds, 0, at_a[i + 1], kk);
+        else if (kk + 32 < BK) {
+          fa[(q + 1) & 1] = TileA::fragment(lds, 0, at_a[0], kk + 32);
 #pragma unroll
-        for (int i = 0; i < FM; ++i) {
-          const v8s fa = TileA::fragment(lds, 0, at_a[i], kk);
-#pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = mfma<T>(fb[j], fa, acc[i][j]);
-          if (MODE == kBackWeight && sum_bias) accb = mfma<T>(ones_in_row<T>(i), fa, accb);
+          for (int j = 0; j < FN; ++j) fb[h + 1][j] = TileB::fragment(lds + TileA::bytes, 0, at_b[j], kk + 32);
         }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) acc[i][j] = mfma<T>(fb[h][j], fa[q & 1], acc[i][j]);
       }
+      if (MODE == kBackWeight && sum_bias) add_bias_sums<T, TileA>(lds, at_a, accb);
     };
     const int steps = w.depth / BK, rest = w.depth % BK;
     for (int t = 0; t < steps; t += 2) {
@@ -927,16 +937,31 @@ __global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
     next(after);
     __syncthreads();       // every wave is done with both buffers:
     begin(after);          // the next tile is under way while this one's results are written
-    const int lane = threadIdx.x & 63, m0 = wm0 + (lane & 15), nb = wn0 + (lane >> 4) * 4;
+    // Two neighbouring column tiles at a time: a lane that holds four columns of either exchanges with its neighbour for eight of one, so that a
+    // row's 64 bytes go out together.  The rows' results, of which nothing is read again here, are marked so, which leaves the L2s to the operands
+    // (forward, 32768 x 1024 to 4096 columns in 16 groups: 350 us with 32 bytes a store, 333 with 64, 300 marked; 8192^3: 888, 875, 845.  The
+    // weight product lost 2 percent by the mark.)
+    const int lane = threadIdx.x & 63, m0 = wm0 + (lane & 15), nb = wn0 + (lane >> 4 & 1) * 16 + (lane >> 5) * 8;
     T* out = (T*)a.out + ((MODE == kBackWeight ? (int64_t)w.group * a.m : 0) + w.m0) * a.n + w.n0 + (int64_t)m0 * a.n + nb;
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        Four e;
+      for (int j = 0; j < FN; j += 2) {
+        uint2 e[2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) e.v[k] = (T)acc[i][j][k];
-        if (m0 + i * 16 < w.rows_a && nb + j * 16 < w.rows_b) *reinterpret_cast<Four*>(out + j * 16) = e;
+        for (int h = 0; h < 2; ++h) {
+          Four f;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) f.v[k] = (T)acc[i][j + h][k];
+          e[h] = __builtin_bit_cast(uint2, f);
+        }
+        const auto x = __builtin_amdgcn_permlane16_swap(e[0].x, e[1].x, false, false);   // lanes 16-31 of one with lanes 0-15 of the other,
+        const auto y = __builtin_amdgcn_permlane16_swap(e[0].y, e[1].y, false, false);   // and 48-63 with 32-47
+        const v4u eight = {x[0], y[0], x[1], y[1]};
+        if (m0 + i * 16 < w.rows_a && nb + j * 16 < w.rows_b) {
+          if (MODE == kBackWeight) *reinterpret_cast<v4u*>(out + j * 16) = eight;
+          else __builtin_nontemporal_store(eight, reinterpret_cast<v4u*>(out + j * 16));
+        }
       }
       out += (int64_t)16 * a.n;
       if (MODE == kBackWeight && sum_bias && lane >> 4 == i >> 2 && m0 + i * 16 < w.rows_a)
@@ -991,6 +1016,7 @@ __global__ void __launch_bounds__(256) grouped_weight_sum_kernel(GroupArgs a) {
     before += (unsigned)__builtin_amdgcn_readlane(groups.upto, l) - (group - g0 < 64 ? mine : 0u);
     high = __builtin_amdgcn_readlane(groups.end, 63);
   }
+  if (mine == 1) return;   // (written by the tiles' kernel; a group without rows is cleared here)
   const int64_t weights = (int64_t)a.m * a.n, size = weights + (a.dbias ? a.m : 0);
   const unsigned per = (mine + 3) / 4, q0 = min(wave * per, mine), q1 = min(q0 + per, mine);
   for (int64_t e0 = (int64_t)blockIdx.x * 64; e0 < size; e0 += (int64_t)gridDim.x * 64) {
