@@ -269,6 +269,31 @@ def test_grouped_linear_large_tiles(hip_backend, inner, outer, dtype):
                   rnd((n, outer), 4, dtype, 0.1))
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=str)
+@pytest.mark.parametrize("inner,outer,ends", [(72, 4096, [0, 1900, 1900, 4160]), (328, 2048, [2, 2500, 2520, 8000]), (256, 256, [0, 131072])])
+def test_grouped_linear_tall_and_low_large_tiles(hip_backend, inner, outer, ends, dtype):
+    # one column of blocks more than whole rounds of 256-row tiles, and sizes that fill them: either height of the large tiles
+    n, groups = ends[-1], len(ends) - 1
+    for i, o in ((inner, outer), (outer, inner)):
+        check_grouped(rnd((n, i), 1, dtype), rnd((groups, o, i), 2, dtype, i ** -0.5), ends, rnd((groups, o), 3, dtype), rnd((n, o), 4, dtype, 0.1))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("ends", [[0, 200, 456, 456, 9001], [8000, 8000, 8256, 8999, 9001], [0, 1, 258, 8745, 9001]])
+def test_grouped_linear_groups_of_one_piece_and_of_many(hip_backend, ends, dtype):
+    n = 9001
+    check_grouped(rnd((n, 48), 1, dtype), rnd((4, 40, 48), 2, dtype), ends, rnd((4, 40), 3, dtype), rnd((n, 40), 4, dtype, 0.1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("rows,inner,outer", [(50, 4100, 70), (200, 4100, 130), (600, 2100, 260), (1500, 1030, 136), (2500, 200, 700)])
+def test_grouped_linear_every_tile_and_cut(hip_backend, rows, inner, outer, dtype):
+    # sizes at which the expected times choose other tiles and numbers of pieces
+    ends = [0, rows // 5, rows // 5 + 1, rows - 3, rows]
+    check_grouped(rnd((rows, inner), 1, dtype), rnd((4, outer, inner), 2, dtype, inner ** -0.5), ends, rnd((4, outer), 3, dtype),
+                  rnd((rows, outer), 4, dtype, 0.1))
+
+
 def test_grouped_linear_many_groups(hip_backend):
     g = torch.Generator().manual_seed(3)
     sizes = torch.randint(0, 9, (200,), generator=g)

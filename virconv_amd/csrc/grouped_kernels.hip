@@ -824,13 +824,13 @@ __global__ void __launch_bounds__(512, 2) grouped_f32_kernel(GroupArgs a) {
 // step of 64) stay below what its products take (a 128 x 128 tile of four waves keeps LDS exactly as busy as the matrix units and reached 570
 // TFLOP/s).  The next step's operands come by LDS-direct loads into the other buffer while this one is multiplied: no registers, one barrier a
 // step.  What is left of the summed axis behind the last whole step goes through registers, with zeros behind its end.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
-  constexpr int BM = 256, BN = 256, BK = 64, WN = 4, FM = 8, FN = 4;
+constexpr int kLargeNarrow = 192, kLargeBuffer = (256 + 256) * 64 * 2;
+template <typename T, int BM, int MODE>
+__device__ __forceinline__ void large_products(const GroupArgs& a, Groups& groups, char* even, char* odd) {
+  constexpr int BN = 256, BK = 64, WN = 4, FM = BM / 32, FN = 4;
   typedef Tile<T, BM, MODE != kBackWeight, 512> TileA;
   typedef Tile<T, BN, MODE == kForward, 512> TileB;
-  __shared__ __align__(16) char even[TileA::bytes + TileB::bytes];
-  __shared__ __align__(16) char odd[TileA::bytes + TileB::bytes];
+  static_assert(TileA::bytes + TileB::bytes <= kLargeBuffer, "");
   const int wave = threadIdx.x >> 6, wm0 = (wave / WN) * (FM * 16), wn0 = (wave % WN) * (FN * 16);
   int at_a[FM], at_b[FN];
 #pragma unroll
@@ -838,7 +838,6 @@ __global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
 #pragma unroll
   for (int j = 0; j < FN; ++j) at_b[j] = TileB::lane_place(wn0 + j * 16);
 
-  Groups groups(a, MODE == kBackWeight ? a.per_split : BM);
   const unsigned xcd = blockIdx.x % 8, blocks = gridDim.x / 8;
   const Items items = items_of<MODE>(a, groups, BM, xcd);
   const unsigned block = blockIdx.x / 8;
@@ -971,6 +970,25 @@ __global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
   }
 }
 
+// Rows of a tile: 256, or 192 where that takes less time in whole rounds of the blocks: a round costs its products (at 192 rows at a rate that is
+// 3 per cent lower) and the way in and out, as much as 400 summed indices of 256 rows.  The groups' real tiles decide (32749 rows in 16 groups, the
+// largest three times the smallest, 4096 summed indices, 1024 columns: 2.2 rounds of 256 rows, 355 and 317 us; 2.8 of 192, 334 and 287).
+template <typename T, int MODE>
+__global__ void __launch_bounds__(512, 2) grouped_large_kernel(GroupArgs a) {
+  __shared__ __align__(16) char even[kLargeBuffer];
+  __shared__ __align__(16) char odd[kLargeBuffer];
+  Groups groups(a, MODE == kBackWeight ? a.per_split : 256);
+  if constexpr (MODE != kBackWeight) {
+    Groups narrow(a, kLargeNarrow);
+    auto rounds = [&](const Groups& g) { return (float)(((unsigned)g.total * a.ntiles + gridDim.x - 1) / gridDim.x); };
+    if (rounds(narrow) * (kLargeNarrow * 1.03f * a.k + 256 * 400) < rounds(groups) * (256.f * a.k + 256 * 400)) {
+      large_products<T, kLargeNarrow, MODE>(a, narrow, even, odd);
+      return;
+    }
+  }
+  large_products<T, 256, MODE>(a, groups, even, odd);
+}
+
 // the sum of `count` values `stride` apart, in order: a chain, its loads four at a time
 __device__ __forceinline__ float sum_along(const float* p, unsigned count, int64_t stride) {
   float s = 0.f;
@@ -1034,30 +1052,42 @@ __global__ void __launch_bounds__(256) grouped_weight_sum_kernel(GroupArgs a) {
 }
 
 // ------------------------------------------------------------------------------------------------ launch rules
-struct GroupPlan { int bm, bn, splits, per_split; bool two_kinds; int64_t partial_floats, mtiles_most; };
+struct GroupPlan { int bm, bn, splits, per_split; bool two_kinds; double us; int64_t partial_floats, mtiles_most; };
 
-// Row products.  Tiles of 128 x 128 where the groups have several of them on average, of 64 x 128 or 16 x 128 where they are shorter (a tile of a
-// short group is mostly padding), of 64 x 64 where there are no more than 64 columns; the inner axis is split where there are too few
-// tiles to fill 256 compute units.
+// Row products.  The tile and the number of pieces that the summed axis is cut into are those of the least expected time, in us:
+//
+//   5 + what the steps take + (4 + the pieces' sums, written and read at 2.6 TB/s, where there is more than one piece)
+//
+// The blocks of the kernel for every case share compute units, so the steps take the time of all of them at the rate of a full device (`full`, of
+// a compute unit) or that of one block alone (`alone`), whichever is more; the two-kind kernel has one block a compute unit and takes its tiles in
+// whole rounds.  Tiles of a group of r rows: r / bm and half a one for the last, as the sizes are not known here.  The figures were measured
+// over 23 to 26 shapes with every tile and 1 to 48 pieces: what the rule picks takes 3 per cent longer on average than the best of them (times for
+// bf16, 64 x 128 tile: 8 groups of 2048 rows in all, 1024 x 1024, 17 us whole, 29 in two pieces, 24 by 16-row tiles; 200 rows in 4 groups 9 us by
+// 16-row tiles, 11 by 64; fp32, 480 rows in 3 groups, 27648 summed: two kinds, 24 pieces, 61 us, whole 933, by 64-row tiles 65).
+// 128 x 128 tiles of 16-bit operands were at most 6 per cent faster than the best of the others.
 static GroupPlan plan_rows(int64_t rows, int64_t groups, int64_t n, int64_t k, int dtype) {
-  GroupPlan p;
-  const int64_t average = groups > 0 ? rows / groups : rows, bk = dtype == VC_F32 ? 32 : 64;
-  p.two_kinds = dtype == VC_F32 && average > 64 && n > 64;
-  if (p.two_kinds) { p.bm = average > 128 && average <= 192 ? 192 : 128; p.bn = 128; }
-  else if (average <= 24) { p.bm = 16; p.bn = 128; }
-  else if (n <= 64) { p.bm = 64; p.bn = 64; }
-  else { p.bm = average >= 256 ? 128 : 64; p.bn = 128; }
-  p.mtiles_most = rows / p.bm + groups + 2;
-  // tiles there will be: full ones, and one that is cut short for every group that has rows
-  const int64_t tiles = (rows / p.bm + (groups < rows ? groups : rows)) * cdiv(n, p.bn), steps = cdiv(k, bk);
-  int64_t splits = 1;
-  if (tiles < 256 && steps >= 16) splits = (p.two_kinds ? 256 : 512) / tiles;   // (one block of the two-kind kernel a compute unit)
-  if (splits > steps / 8) splits = steps / 8 > 0 ? steps / 8 : 1;
-  p.per_split = (int)(cdiv(steps, splits) * bk);
-  p.splits = (int)cdiv(k, p.per_split);
-  if (p.splits < 1) p.splits = 1;
-  p.partial_floats = p.splits > 1 ? p.splits * rows * n : 0;
-  return p;
+  struct Kind { int dtype_bits, bm, bn; bool two_kinds; double alone, full; };
+  static const Kind kinds[] = {{16, 16, 128, false, 0.36, 0.28}, {16, 64, 128, false, 0.48, 0.42},
+                               {32, 16, 128, false, 0.63, 0.57}, {32, 64, 128, false, 0.88, 1.0}, {32, 128, 128, true, 1.25, 1.25}, {32, 192, 128, true, 1.65, 1.65}};
+  const int bits = dtype == VC_F32 ? 32 : 16;
+  const int64_t bk = dtype == VC_F32 ? 32 : 64, steps = cdiv(k, bk), filled = groups < rows ? groups : rows;
+  GroupPlan best{};
+  for (const Kind& kind : kinds) {
+    if (kind.dtype_bits != bits || (kind.two_kinds && n <= 64)) continue;
+    const int bn = kind.bm == 64 && n <= 64 ? 64 : kind.bn;
+    const double cut = (double)rows / kind.bm + 0.5 * filled, tiles = (cut > filled ? cut : filled) * cdiv(n, bn);
+    for (int64_t want = 1; want <= 64; want = want & (want - 1) ? want / 3 * 4 : want == 1 ? 2 : want / 2 * 3) {   // 1, 2, 3, 4, 6, 8, 12, ...
+      const int64_t per = cdiv(steps, want), splits = cdiv(steps, per);
+      if (want > 1 && per * bk < 256) break;
+      double us;
+      if (kind.two_kinds) us = (double)(int64_t)((tiles * splits + 255) / 256) * per * kind.full;
+      else us = tiles * splits * per / 256 * kind.full;
+      if (us < per * kind.alone) us = per * kind.alone;
+      us += 5 + (splits > 1 ? 4 + 8e-6 / 2.6 * splits * rows * n : 0);
+      if (best.bm == 0 || us < best.us) best = {kind.bm, bn, (int)splits, (int)(per * bk), kind.two_kinds, us, splits > 1 ? splits * rows * n : 0, 0};
+    }
+  }
+  return best;
 }
 
 // Weight product.  The rows are split into pieces where the output has few tiles, a piece being long enough that the sums written for it
@@ -1079,14 +1109,19 @@ static GroupPlan plan_weight(int64_t rows, int64_t groups, int64_t m, int64_t n,
   return p;
 }
 
-// The large tiles take over where every piece of both operands is aligned and there are about enough of them for the compute units: below
-// that the finer cut of the 128-row tiles is worth more than the higher rate.
+// Large tiles need every piece of both operands to be aligned, sizes of 192 either way (of a tile's 256), and 32-bit offsets in a tile.
 static constexpr unsigned kLargeBlocks = 256;   // one a compute unit, each taking tiles until there are none
-static bool large_tiles(int dtype, int64_t m_average, int64_t n, int64_t tiles, int64_t longest, std::initializer_list<uintptr_t> aligned) {
-  if (longest >= (1 << 22) || dtype == VC_F32 || m_average < 192 || n < 192 || tiles < 160) return false;
+static bool large_tiles(int dtype, int64_t m, int64_t n, int64_t longest, std::initializer_list<uintptr_t> aligned) {
+  if (longest >= (1 << 22) || dtype == VC_F32 || m < 192 || n < 192) return false;
   for (uintptr_t v : aligned)
     if (v & 15) return false;
   return true;
+}
+// Their expected time as above, a step of all compute units taking 1.3 us, the way in and out of a round 4 (bf16, 8192 rows in 8 groups, 1024 x 1024:
+// 26 us, by 64 x 128 tiles 34; 4096 rows 24 and 22; 2560 rows in 16 groups, 1024 x 4096: 33 and 45).
+static double large_us(int64_t rows, int64_t groups, int64_t n, int64_t k) {
+  const double filled = (double)(groups < rows ? groups : rows), cut = rows / 256.0 + 0.5 * filled, tiles = (cut > filled ? cut : filled) * cdiv(n, 256);
+  return 5 + (tiles > 256 ? tiles / 256 : 1) * (cdiv(k, 64) * 1.3 + 4);
 }
 
 static bool small_operands(int64_t n, int64_t k, int64_t longest) { return n < 8 || k < 8 || longest >= (1 << 22) - 1 || n >= (1 << 22) - 1; }
@@ -1106,15 +1141,16 @@ static int launch_rows(const char* who, GroupArgs a, int mode, int dtype, const 
   const size_t need = (size_t)p.partial_floats * sizeof(float);
   VC_REQUIRE(need == 0 || (ws && ws_bytes >= need), "%s: workspace of %zu bytes, need %zu", who, ws_bytes, need);
   a.partial = (float*)ws;
-  a.splits = p.splits;
-  a.per_split = p.per_split;
   const uintptr_t size = 2;
-  const bool large = p.splits == 1 && large_tiles(dtype, a.groups ? a.rows / a.groups : 0, a.n, cdiv(a.rows, 256) * cdiv(a.n, 256), a.lda > a.n ? a.lda : a.n,
-                                                  {(uintptr_t)a.a, (uintptr_t)a.b, (uintptr_t)a.out, (uintptr_t)a.bias, a.lda * size, a.k * size, a.n * size});
+  const bool large = large_us(a.rows, a.groups, a.n, a.k) < p.us &&
+                     large_tiles(dtype, a.rows, a.n, a.lda > a.n ? a.lda : a.n,
+                                 {(uintptr_t)a.a, (uintptr_t)a.b, (uintptr_t)a.out, (uintptr_t)a.bias, a.lda * size, a.k * size, a.n * size});
+  a.splits = large ? 1 : p.splits;
+  a.per_split = large ? a.k : p.per_split;
   const bool small = small_operands(a.n, a.k, a.lda);
-  const int bm = large ? 256 : small ? 64 : p.bm, bn = large ? 256 : small ? 64 : p.bn;
+  const int bm = large ? kLargeNarrow : small ? 64 : p.bm, bn = large ? 256 : small ? 64 : p.bn;
   a.ntiles = (int)cdiv(a.n, bn);
-  const int64_t total = (a.rows / bm + a.groups + 2) * a.ntiles * p.splits;
+  const int64_t total = (a.rows / bm + a.groups + 2) * a.ntiles * a.splits;
   VC_REQUIRE(total < (1LL << 30), "%s: %lld tiles", who, (long long)total);
   const unsigned blocks = large || (p.two_kinds && !small) ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
 #define VC_GO(T, ...)                                                                                                             \
@@ -1123,7 +1159,6 @@ static int launch_rows(const char* who, GroupArgs a, int mode, int dtype, const 
   if (p.splits > 1) hipLaunchKernelGGL(grouped_row_sum_kernel<T>, dim3((unsigned)cdiv(a.rows * cdiv(a.n, 64), 4)), dim3(256), 0, st, a)
 #define VC_TILES(T)                                       \
   if (small) { VC_GO(T, 64, 64, 2, 1, true); }                          \
-  else if (p.bm == 128) { if constexpr (sizeof(T) == 2) { VC_GO(T, 128, 128, 2, 2, false); } }    \
   else if (p.bm == 64 && p.bn == 64) { VC_GO(T, 64, 64, 2, 3, false); }    \
   else if (p.bm == 64) { VC_GO(T, 64, 128, 2, 2, false); }                 \
   else { VC_GO(T, 16, 128, 1, 3, false); }
@@ -1206,8 +1241,10 @@ int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const voi
   a.rows = rows; a.groups = (int)groups; a.m = (int)out; a.n = (int)in;
   a.splits = p.splits; a.per_split = p.per_split;
   const uintptr_t size = 2;
-  const bool large = p.splits == 1 && large_tiles(dtype, out, in, groups * cdiv(out, 256) * cdiv(in, 256), x_stride > dy_stride ? x_stride : dy_stride,
-                                                  {(uintptr_t)x, (uintptr_t)dy, (uintptr_t)dweight, x_stride * size, dy_stride * size, in * size, out * size});
+  // (from 160 tiles on: of 2048 columns, 1024 and 4 groups of 512 rows 128 tiles took 23 us, 128 x 128 ones 20, and 256 of 4096 columns 25 and 34)
+  const bool large = p.splits == 1 && groups * cdiv(out, 256) * cdiv(in, 256) >= 160 &&
+                     large_tiles(dtype, out, in, x_stride > dy_stride ? x_stride : dy_stride,
+                                 {(uintptr_t)x, (uintptr_t)dy, (uintptr_t)dweight, x_stride * size, dy_stride * size, in * size, out * size});
   const bool small = small_operands(out, in, x_stride > dy_stride ? x_stride : dy_stride);
   a.mtiles = (int)cdiv(out, large ? 256 : small ? 64 : p.bm); a.ntiles = (int)cdiv(in, large ? 256 : small ? 64 : p.bn);
   a.partial = (float*)workspace;
