@@ -508,15 +508,24 @@ __device__ __forceinline__ Work<T> find_work(const GroupArgs& a, Groups& g, cons
 template <typename T, int FM, int FN, int MODE>
 __device__ __forceinline__ void write_results(const GroupArgs& a, const Work<T>& w, int wm0, int wn0, const v4f (&acc)[FM][FN], const v4f& accb, bool sum_bias) {
   const int lane = threadIdx.x & 63;
-  if (MODE != kForward && !sum_bias && w.rows_a >= wm0 + FM * 16 && w.rows_b >= wn0 + FN * 16) {   // the wave's part of the tile is whole
+  if (!sum_bias && w.rows_a >= wm0 + FM * 16 && w.rows_b >= wn0 + FN * 16) {   // the wave's part of the tile is whole
     const int64_t at = (int64_t)(wm0 + (lane & 15)) * a.n + wn0 + (lane >> 4) * 4;
     float* part = w.partial ? w.partial + at : nullptr;
     T* out = (T*)a.out + ((MODE == kBackWeight ? (int64_t)w.group * a.m : 0) + w.m0) * a.n + w.n0 + at;
+    struct __attribute__((packed, aligned(sizeof(T)))) Four { T v[4]; } bias[FN] = {};
+    if (MODE == kForward && a.bias && !part) {
+#pragma unroll
+      for (int j = 0; j < FN; ++j) __builtin_memcpy(&bias[j], (const T*)a.bias + (int64_t)w.group * a.n + w.n0 + wn0 + j * 16 + (lane >> 4) * 4, sizeof(bias[j]));
+    }
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
-        const float r[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        float r[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+        if (MODE == kForward) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) r[e] += (float)bias[j].v[e];
+        }
         if (part) store4(part + j * 16, 4, r);
         else store4(out + j * 16, 4, r);
       }
@@ -1017,11 +1026,12 @@ __global__ void __launch_bounds__(256) grouped_row_sum_kernel(GroupArgs a) {
   ((T*)a.out)[row * a.n + n] = (T)s;
 }
 
-// weight product: the pieces' sums of each group.  64 elements a block; its four waves add a quarter of the pieces each, in order, and the four
-// sums are added in order.
-template <typename T>
-__global__ void __launch_bounds__(256) grouped_weight_sum_kernel(GroupArgs a) {
-  __shared__ float part[4][64];
+// weight product: the pieces' sums of each group.  64 elements a block; its waves add a share of the pieces each, in order, and their sums are
+// added in order.  Sixteen waves where a group has many pieces, whose sums a wave reads one after the other (133578 rows, 64 x 64 in 4 groups of
+// about a hundred: the whole product 26.4 us, 28.2 with four waves); four where few pieces leave the others nothing.
+template <typename T, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) grouped_weight_sum_kernel(GroupArgs a) {
+  __shared__ float part[WAVES][64];
   const int group = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   // pieces in front of the group, and its own
   unsigned before = 0, mine = 0;
@@ -1036,14 +1046,16 @@ __global__ void __launch_bounds__(256) grouped_weight_sum_kernel(GroupArgs a) {
   }
   if (mine == 1) return;   // (written by the tiles' kernel; a group without rows is cleared here)
   const int64_t weights = (int64_t)a.m * a.n, size = weights + (a.dbias ? a.m : 0);
-  const unsigned per = (mine + 3) / 4, q0 = min(wave * per, mine), q1 = min(q0 + per, mine);
+  const unsigned per = (mine + WAVES - 1) / WAVES, q0 = min(wave * per, mine), q1 = min(q0 + per, mine);
   for (int64_t e0 = (int64_t)blockIdx.x * 64; e0 < size; e0 += (int64_t)gridDim.x * 64) {
     const int64_t e = e0 + lane, i = e - weights;
     if (e < weights) part[wave][lane] = sum_along(a.partial + (int64_t)(before + q0) * weights + e, q1 - q0, weights);
     else if (e < size) part[wave][lane] = sum_along(a.partial_bias + (int64_t)(before + q0) * a.m + i, q1 - q0, a.m);
     __syncthreads();
     if (wave == 0 && e < size) {
-      const float s = (part[0][lane] + part[1][lane]) + (part[2][lane] + part[3][lane]);
+      float s = part[0][lane];
+#pragma unroll
+      for (int q = 1; q < WAVES; ++q) s += part[q][lane];
       if (e < weights) ((T*)a.out)[group * weights + e] = (T)s;
       else ((T*)a.dbias)[group * (int64_t)a.m + i] = (T)s;
     }
@@ -1102,7 +1114,7 @@ static GroupPlan plan_weight(int64_t rows, int64_t groups, int64_t m, int64_t n,
   const int64_t least = 4 * m * n / (m + n) > 256 ? 4 * m * n / (m + n) : 256;
   if (piece < least) piece = least;
   piece = cdiv(piece, 64) * 64;
-  p.splits = tiles < 512 && groups * piece <= rows ? 2 : 1;
+  p.splits = tiles < 512 && groups * piece <= rows && groups < 65536 ? 2 : 1;   // (the groups are the sums' second grid dimension)
   p.per_split = (int)piece;
   p.mtiles_most = p.splits > 1 ? rows / piece + groups : groups;   // pieces
   p.partial_floats = p.splits > 1 ? p.mtiles_most * (m * n + m) : 0;
@@ -1151,7 +1163,7 @@ static int launch_rows(const char* who, GroupArgs a, int mode, int dtype, const 
   const int bm = large ? kLargeNarrow : small ? 64 : p.bm, bn = large ? 256 : small ? 64 : p.bn;
   a.ntiles = (int)cdiv(a.n, bn);
   const int64_t total = (a.rows / bm + a.groups + 2) * a.ntiles * a.splits;
-  VC_REQUIRE(total < (1LL << 30), "%s: %lld tiles", who, (long long)total);
+  VC_REQUIRE(total < (1LL << 24) - 8, "%s: %lld tiles", who, (long long)total);   // (2^32 threads)
   const unsigned blocks = large || (p.two_kinds && !small) ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
 #define VC_GO(T, ...)                                                                                                             \
   if (mode == kForward) hipLaunchKernelGGL((grouped_kernel<T, __VA_ARGS__, kForward>), dim3(blocks), dim3(256), 0, st, a);        \
@@ -1252,7 +1264,7 @@ int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const voi
   const int64_t tiles = (int64_t)a.mtiles * a.ntiles;
   // without splits every XCD takes an eighth of each group's tiles
   const int64_t total = p.splits == 1 && tiles >= 8 ? cdiv(tiles, 8) * 8 * groups : p.mtiles_most * tiles;
-  VC_REQUIRE(total < (1LL << 30), "%s: %lld tiles", who, (long long)total);
+  VC_REQUIRE(total < (1LL << 24) - 8, "%s: %lld tiles", who, (long long)total);   // (2^32 threads)
   const unsigned blocks = large || (p.two_kinds && !small) ? kLargeBlocks : (unsigned)cdiv(total, 8) * 8;
   hipStream_t st = (hipStream_t)stream;
   const int64_t sum_blocks = cdiv(out * in + out, 64);
@@ -1261,8 +1273,10 @@ int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const voi
   else if (p.two_kinds) hipLaunchKernelGGL((grouped_f32_kernel<128, 128, kBackWeight>), dim3(blocks), dim3(512), 0, st, a);                        \
   else if (p.bm == 128) { if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((grouped_kernel<T, 128, 128, 2, 2, false, kBackWeight>), dim3(blocks), dim3(256), 0, st, a); } \
   else hipLaunchKernelGGL((grouped_kernel<T, 64, 64, 2, 3, false, kBackWeight>), dim3(blocks), dim3(256), 0, st, a);                                      \
-  if (p.splits > 1)                                                                                                                           \
-    hipLaunchKernelGGL(grouped_weight_sum_kernel<T>, dim3((unsigned)(sum_blocks < 16384 ? sum_blocks : 16384), (unsigned)groups), dim3(256), 0, st, a)
+  if (p.splits > 1 && p.mtiles_most > 16 * groups)                                                                                            \
+    hipLaunchKernelGGL((grouped_weight_sum_kernel<T, 16>), dim3((unsigned)(sum_blocks < 16384 ? sum_blocks : 16384), (unsigned)groups), dim3(1024), 0, st, a);   \
+  else if (p.splits > 1)                                                                                                                      \
+    hipLaunchKernelGGL((grouped_weight_sum_kernel<T, 4>), dim3((unsigned)(sum_blocks < 16384 ? sum_blocks : 16384), (unsigned)groups), dim3(256), 0, st, a)
   if (large && dtype == VC_F16) hipLaunchKernelGGL((grouped_large_kernel<_Float16, kBackWeight>), dim3(blocks), dim3(512), 0, st, a);
   else if (large) hipLaunchKernelGGL((grouped_large_kernel<__bf16, kBackWeight>), dim3(blocks), dim3(512), 0, st, a);
   else if (dtype == VC_F32) { VC_GO(float); } else if (dtype == VC_F16) { VC_GO(_Float16); } else { VC_GO(__bf16); }
