@@ -13,6 +13,11 @@
 // channels a wave), a block for wide ones.  A row whose length is no multiple of VEC ends in a vector that overlaps the one before it; the
 // elements that are there twice count once in the sums and are written twice with one value.  Rows wider than a block's registers are read
 // three times (they come from the cache by then).
+//
+// Measured, with fp32 weights, tensors cycled through so that nothing is left in a cache (a large copy reaches 4.9 TB/s):
+//   forward   16381 x 4096 bf16 54 us (4.9 TB/s), fp32 99 us (5.4); 133578 x 64 fp32 14.5 us (4.7), bf16 8.0 us (4.3)
+//   backward  16381 x 4096 bf16 89 us (4.5 TB/s), fp32 163 us (4.9); 133578 x 64 fp32 27 us (3.8), bf16 14.2 us (3.6: as much time goes into the
+//             column sums, 2 fused operations an element and the launch that adds them, as into the memory's part)
 #include "common.h"
 
 namespace vc {
@@ -380,42 +385,41 @@ __global__ void __launch_bounds__(256) norm_param_grad_kernel(const float* __res
 
 // how a row of c elements is held: VEC elements a vector, LPR lanes, ITER vectors a lane; iter 0: wider than a block's registers
 struct NormShape { int vec, lpr, iter; };
-static NormShape norm_shape(int64_t c, int dtype, bool backward) {
+static NormShape norm_shape(int64_t c, int dtype) {
   const int full = dtype == VC_F32 ? 4 : 8;
   if (c < full) return {1, 8, 1};
   const int64_t vecs = cdiv(c, full);
   for (int lpr = 2; lpr <= 64; lpr *= 2)
     if (vecs <= lpr) return {full, lpr, 1};
-  if (vecs <= 128) return {full, 64, 2};
-  // (two vectors a lane hide more latency in the forward pass; the backward pass, which holds five values an element, would spill)
+  if (vecs <= 128) return {full, 64, 2};      // (32768 x 1000 bf16: forward 28 us, backward 54; by blocks of 256, one vector a lane, 42 and 60)
+  // (two vectors a lane up to 512 and 1024 vectors were no faster in the forward pass, and spill in the backward pass, which holds five values
+  // an element: 16381 x 4096 bf16, 138 us and 89)
   for (int lpr = 256; lpr <= 1024; lpr *= 2)
-    if (vecs <= (backward ? 1 : 2) * lpr) return {full, lpr, vecs <= lpr ? 1 : 2};
+    if (vecs <= lpr) return {full, lpr, 1};
   if (vecs <= 2048) return {full, 1024, 2};
   if (dtype == VC_F32 && vecs <= 4096) return {full, 1024, 4};
   return {1, 1024, 0};
 }
 
-// Blocks of the backward pass = rows of its partial sums: one of 1024 threads a compute unit for rows of several waves (each block's column sums are
-// written and read once more: at 4096 channels 1024 blocks of 256 threads would add 67 MB to the 402 MB of 16381 rows), four of 256 for
-// shorter ones.
-static int back_threads(const NormShape& s) { return s.lpr > 64 ? 1024 : 256; }
+// Blocks of the backward pass = rows of its partial sums, which are written and read once more: one a compute unit, of 1024 threads for rows of
+// several waves and of 512 for shorter ones.  (133578 x 64 fp32 and bf16, with the weights' gradients: 27 and 14 us; 1024 blocks of 256 threads 29
+// and 18, 256 of 1024 threads 26 and 16; 32768 x 1000 bf16: 47, 54 and, as that many threads leave too few registers, 80.)
+static int back_threads(const NormShape& s) { return s.lpr > 64 ? 1024 : 512; }
 static int64_t norm_blocks(int64_t n, int64_t c, const NormShape& s) {
   const int rows = s.iter ? back_threads(s) / s.lpr : 64;
-  const int64_t most = s.lpr > 64 ? (s.iter ? 256 : 512) : 1024, b = cdiv(n, rows);
+  const int64_t most = s.iter ? 256 : 512, b = cdiv(n, rows);
   return b < most ? (b > 0 ? b : 1) : most;
 }
 
 template <typename T> struct FullVec { static constexpr int value = sizeof(T) == 4 ? 4 : 8; };
 
-// DO: in both directions, ONE: in the backward pass, TWO: in the forward pass
-#define VC_NORM_SHAPES(DO, ONE, TWO)                                                                                                                  \
+#define VC_NORM_SHAPES(DO)                                                                                                                  \
   if (s.vec == 1) { DO(1, 8, 1); }                                                                                                          \
   else if (s.lpr == 2) { DO(V, 2, 1); } else if (s.lpr == 4) { DO(V, 4, 1); } else if (s.lpr == 8) { DO(V, 8, 1); }                         \
   else if (s.lpr == 16) { DO(V, 16, 1); } else if (s.lpr == 32) { DO(V, 32, 1); }                                                           \
   else if (s.lpr == 64 && s.iter == 1) { DO(V, 64, 1); } else if (s.lpr == 64) { DO(V, 64, 2); }                                            \
-  else if (s.lpr == 256 && s.iter == 1) { DO(V, 256, 1); } else if (s.lpr == 256) { TWO(V, 256, 2); }                                       \
-  else if (s.lpr == 512 && s.iter == 1) { ONE(V, 512, 1); } else if (s.lpr == 512) { TWO(V, 512, 2); }                                      \
-  else if (s.iter == 1) { ONE(V, 1024, 1); } else if (s.iter == 2) { DO(V, 1024, 2); } else if constexpr (V == 4) { DO(V, 1024, 4); }
+  else if (s.lpr == 256) { DO(V, 256, 1); } else if (s.lpr == 512) { DO(V, 512, 1); } else if (s.iter == 1) { DO(V, 1024, 1); }             \
+  else if (s.iter == 2) { DO(V, 1024, 2); } else if constexpr (V == 4) { DO(V, 1024, 4); }
 
 template <typename T>
 static void norm_forward_launch(const NormArgs& a, const NormShape& s, hipStream_t st) {
@@ -430,9 +434,7 @@ static void norm_forward_launch(const NormArgs& a, const NormShape& s, hipStream
   const unsigned blocks = (unsigned)(need < most ? need : most);
 #define VC_DO(VEC, LPR, ITER)                                                                                                               \
   hipLaunchKernelGGL((norm_forward_kernel<T, VEC, LPR, ITER, (LPR > 256 ? LPR : 256)>), dim3(blocks), dim3(threads), 0, st, a)
-#define VC_NO(...)
-  VC_NORM_SHAPES(VC_DO, VC_NO, VC_DO)
-#undef VC_NO
+  VC_NORM_SHAPES(VC_DO)
 #undef VC_DO
 }
 
@@ -445,10 +447,8 @@ static void norm_backward_launch(const NormBackArgs& a, const NormShape& s, int6
     return;
   }
 #define VC_DO(VEC, LPR, ITER)                                                                                                               \
-  hipLaunchKernelGGL((norm_backward_kernel<T, VEC, LPR, ITER, (LPR > 64 ? 1024 : 256)>), dim3((unsigned)blocks), dim3(back_threads(s)), 0, st, a)
-#define VC_NO(...)
-  VC_NORM_SHAPES(VC_DO, VC_DO, VC_NO)
-#undef VC_NO
+  hipLaunchKernelGGL((norm_backward_kernel<T, VEC, LPR, ITER, (LPR > 64 ? 1024 : 512)>), dim3((unsigned)blocks), dim3(back_threads(s)), 0, st, a)
+  VC_NORM_SHAPES(VC_DO)
 #undef VC_DO
 }
 
@@ -469,7 +469,7 @@ int vc_layer_norm_forward(const void* x, int64_t x_stride, int64_t n, int64_t c,
   if (n == 0) return VC_OK;
   VC_REQUIRE(x && y, "vc_layer_norm_forward: NULL pointer");
   NormArgs a{x, weight, bias, y, mean, rstd, n, x_stride, (int)c, weight_dtype, bias_dtype, eps};
-  const NormShape s = norm_shape(c, dtype, false);
+  const NormShape s = norm_shape(c, dtype);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == VC_F32) norm_forward_launch<float>(a, s, st);
   else if (dtype == VC_F16) norm_forward_launch<_Float16>(a, s, st);
@@ -480,7 +480,7 @@ int vc_layer_norm_forward(const void* x, int64_t x_stride, int64_t n, int64_t c,
 
 size_t vc_layer_norm_backward_workspace_bytes(int64_t n, int64_t c, int dtype) {
   if (n <= 0 || c <= 0 || !known_dtype(dtype)) return 0;
-  return (size_t)norm_blocks(n, c, norm_shape(c, dtype, true)) * 2 * (size_t)c * sizeof(float);
+  return (size_t)norm_blocks(n, c, norm_shape(c, dtype)) * 2 * (size_t)c * sizeof(float);
 }
 
 int vc_layer_norm_backward(const void* x, int64_t x_stride, const void* dy, int64_t dy_stride, int64_t n, int64_t c, int dtype,
@@ -491,7 +491,7 @@ int vc_layer_norm_backward(const void* x, int64_t x_stride, const void* dy, int6
   VC_REQUIRE((x_stride >= c && dy_stride >= c) || n <= 1, "vc_layer_norm_backward: row stride below %lld columns", (long long)c);
   hipStream_t st = (hipStream_t)stream;
   const bool sums = dweight || dbias;
-  const NormShape s = norm_shape(c, dtype, true);
+  const NormShape s = norm_shape(c, dtype);
   const int64_t blocks = norm_blocks(n, c, s);
   if (n > 0) {
     VC_REQUIRE(x && dy && mean && rstd, "vc_layer_norm_backward: NULL pointer");
