@@ -1102,8 +1102,11 @@ static GroupPlan plan_rows(int64_t rows, int64_t groups, int64_t n, int64_t k, i
   return best;
 }
 
-// Weight product.  The rows are split into pieces where the output has few tiles, a piece being long enough that the sums written for it
-// (and read once more) stay small beside the rows that it reads.
+// Weight product.  The rows are split into pieces where the groups' outputs have fewer than 128 tiles in all, or up to three groups, of which one
+// may hold nearly all rows, fewer than 512 each; a piece is long enough that the sums written for it (and read once more) stay small beside the
+// rows that it reads.  (bf16, groups of which the largest has four times the rows of the smallest: 65536 rows of 512 and 512 channels in 32 groups,
+// 512 tiles, 178 us in pieces and 75 whole; 16384 rows in 8 groups, 128 tiles, 66 and 51; 8192 rows of 1024 and 1024 in 2 groups, 128 tiles, 75
+// and 92.  128 x 128 tiles from 65 channels a side on, 64 x 64 below.)
 static GroupPlan plan_weight(int64_t rows, int64_t groups, int64_t m, int64_t n, int dtype) {
   GroupPlan p;
   p.two_kinds = dtype == VC_F32 && m > 64 && n > 64;
@@ -1114,7 +1117,7 @@ static GroupPlan plan_weight(int64_t rows, int64_t groups, int64_t m, int64_t n,
   const int64_t least = 4 * m * n / (m + n) > 256 ? 4 * m * n / (m + n) : 256;
   if (piece < least) piece = least;
   piece = cdiv(piece, 64) * 64;
-  p.splits = tiles < 512 && groups * piece <= rows && groups < 65536 ? 2 : 1;   // (the groups are the sums' second grid dimension)
+  p.splits = tiles < 512 && (groups < 4 || tiles * groups < 128) && groups * piece <= rows ? 2 : 1;
   p.per_split = (int)piece;
   p.mtiles_most = p.splits > 1 ? rows / piece + groups : groups;   // pieces
   p.partial_floats = p.splits > 1 ? p.mtiles_most * (m * n + m) : 0;
