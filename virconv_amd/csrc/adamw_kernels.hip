@@ -4,7 +4,9 @@
 //
 // in fp32 whatever the parameters' type, every operation rounded by itself (this file is built without contraction), the parameter rounded
 // once to its own type.  The step is one pass over its data and nothing else: what bounds it is HBM -- 28 bytes an element with fp32
-// parameters and 32-bit moments, 16 with 8-bit ones, 10 with bf16 parameters and 8-bit moments.
+// parameters and 32-bit moments, 16 with 8-bit ones, 10 with bf16 parameters and 8-bit moments.  Measured: 200 M bf16 parameters with 8-bit
+// moments 397 us (5.05 TB/s; a large copy 4.9), 13 M fp32 ones in 193 tensors 88 us with 32-bit moments (4.15 TB/s), 62 us with 8-bit ones (3.4: four
+// launches, as a launch's table holds 64 tensors, and their ends); 0.42 M in 87 tensors 11 us in two launches, 23 us of host time.
 //
 // 8-bit moments.  m and r = sqrt(v) are held as e4m3 values over a power of two per 128 elements: value * 2^(exponent - 7), the block's
 // largest magnitude lying in [128, 256) before the power is taken off.  r and not v: the root halves the range that a block has to span.
