@@ -294,6 +294,54 @@ def test_grouped_linear_every_tile_and_cut(hip_backend, rows, inner, outer, dtyp
                   rnd((rows, outer), 4, dtype, 0.1))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("count,inner,outer", [(100, 256, 512), (130, 520, 264)])
+def test_grouped_linear_many_long_groups(hip_backend, count, inner, outer, dtype):
+    # more groups than a wave has lanes, with work for the large tiles
+    g = torch.Generator().manual_seed(4)
+    sizes = torch.randint(0, 500, (count,), generator=g)
+    sizes[::7] = 0
+    ends = [3] + (3 + torch.cumsum(sizes, 0)).tolist()
+    n = ends[-1] + 4
+    check_grouped(rnd((n, inner), 1, dtype), rnd((count, outer, inner), 2, dtype, inner ** -0.5), ends, rnd((count, outer), 3, dtype),
+                  rnd((n, outer), 4, dtype, 0.1))
+
+
+def test_two_threads_on_streams_of_their_own(hip_backend):
+    import threading
+    from virconv_amd import ops
+
+    def work(seed):
+        x, dy = rnd((3000, 96), seed).requires_grad_(), rnd((3000, 80), seed + 1)
+        nw, w, b = rnd((96,), seed + 2).requires_grad_(), rnd((3, 80, 96), seed + 3).requires_grad_(), rnd((3, 80), seed + 4).requires_grad_()
+        offsets = torch.tensor([0, 1000, 1001, 2990], device="cuda")
+        y = ops.grouped_linear(ops.layer_norm(x, nw), w, offsets, b)
+        return [y.detach(), *torch.autograd.grad(y, (x, nw, w, b), dy)]
+
+    want = {s: work(s) for s in (10, 20)}
+    torch.cuda.synchronize()
+    bad = []
+
+    def run(seed):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(15):
+                    got = work(seed)
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[seed])):
+                        bad.append(seed)
+        except BaseException as e:      # noqa: BLE001
+            bad.append(e)
+
+    threads = [threading.Thread(target=run, args=(s,)) for s in want]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
+
+
 def test_grouped_linear_many_groups(hip_backend):
     g = torch.Generator().manual_seed(3)
     sizes = torch.randint(0, 9, (200,), generator=g)
@@ -646,6 +694,49 @@ def test_adamw_refusals(hip_backend):
             opt.step()
     torch.cuda.synchronize()
     assert torch.equal(p, before) and opt.state[p]["step"] == 1
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_types_and_missing_gradients_in_one_group(hip_backend, bits):
+    """A group of several types, some parameters without a gradient at some steps or at any: each as in an optimizer of its own."""
+    from virconv_amd.optim import AdamW
+    kinds = [((40, 7), F32), ((300,), BF16), ((129,), F32), ((64, 3), F16), ((5,), BF16), ((2000,), F32)]
+    joint = [torch.nn.Parameter(rnd(s, k, t)) for k, (s, t) in enumerate(kinds)]
+    apart = [torch.nn.Parameter(p.detach().clone()) for p in joint]
+    opt = AdamW(joint, state_bits=bits, seed=5, **HYPER)
+    # (a parameter's random numbers follow from its place in the group: the lone one has as many parameters without gradients in front of it)
+    ones = [AdamW([*(torch.nn.Parameter(torch.zeros(1, device="cuda")) for _ in range(k)), p], state_bits=bits, seed=5, **HYPER) for k, p in enumerate(apart)]
+    for t in range(5):
+        for k, (p, q) in enumerate(zip(joint, apart)):
+            p.grad = None if k == 2 or (k == 4 and t in (0, 3)) else rnd(p.shape, 100 * t + k, p.dtype)
+            q.grad = p.grad
+        opt.step()
+        for o in ones:
+            o.step()
+        for p, q in zip(joint, apart):
+            assert torch.equal(p, q)
+    assert [opt.state[p]["step"] if p in opt.state else 0 for p in joint] == [5, 5, 0, 5, 3, 5]
+    for p, o, q in zip(joint, ones, apart):
+        if p in opt.state:
+            assert all(torch.equal(a, b) for a, b in zip(opt.decoded_state(p), o.decoded_state(q)))
+
+
+@pytest.mark.parametrize("channels_last", [False, True])
+def test_adamw_looks_its_states_over_at_every_step(hip_backend, channels_last):
+    from virconv_amd.optim import AdamW
+    p = torch.nn.Parameter(rnd((8, 6, 3, 5), 1))
+    if channels_last:
+        p = torch.nn.Parameter(p.detach().to(memory_format=torch.channels_last))
+    for bits, second in ((32, "exp_avg_sq"), (8, "exp_avg_rms")):
+        opt = AdamW([p], state_bits=bits)
+        for t in range(2):
+            p.grad = rnd(p.shape, t)
+            opt.step()
+        before = p.detach().clone()
+        opt.state[p][second].data = opt.state[p][second].data.flatten()[:7].clone()     # the same tensor object, other memory
+        with pytest.raises(ValueError, match=second):
+            opt.step()
+        assert torch.equal(p, before) and opt.state[p]["step"] == 2
 
 
 # ---------------------------------------------------------------------------------------------------------------- together

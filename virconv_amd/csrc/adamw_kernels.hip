@@ -281,7 +281,7 @@ int vc_adamw(const vc_adamw_tensor* tensors, int64_t n_tensors, int dtype, int s
   size_t n_spans = 0;
   for (int64_t k = 0; k < n_tensors; ++k) {
     const vc_adamw_tensor& T = tensors[k];
-    VC_REQUIRE(T.n >= 0 && T.n < (1LL << 30) * kAdamwChunk, "vc_adamw: tensor %lld has n = %lld", (long long)k, (long long)T.n);
+    VC_REQUIRE(T.n >= 0 && T.n < (1LL << 35), "vc_adamw: tensor %lld has n = %lld", (long long)k, (long long)T.n);
     VC_REQUIRE(T.key < (1u << 20), "vc_adamw: tensor %lld has the place %u (at most 2^20 tensors)", (long long)k, T.key);
     if (T.n == 0) continue;
     VC_REQUIRE(T.param && T.grad && T.exp_avg && T.exp_avg_sq && (state_bits == 32 || T.exponents), "vc_adamw: tensor %lld has a NULL pointer", (long long)k);
@@ -312,7 +312,7 @@ int vc_adamw(const vc_adamw_tensor* tensors, int64_t n_tensors, int dtype, int s
       const vc_adamw_tensor& T = tensors[k];
       if (T.n == 0) continue;
       const int64_t need = cdiv(T.n, kAdamwChunk);
-      if (B.n && (int64_t)blocks + need >= (1LL << 30)) break;
+      if (B.n && (int64_t)blocks + need >= (1LL << 24)) break;     // (2^32 threads)
       B.t[B.n] = {T.param, T.grad, T.exp_avg, T.exp_avg_sq, T.exponents, (uint64_t)T.n | (uint64_t)T.key << 44};
       if (((((uintptr_t)T.param | (uintptr_t)T.grad) & 15) | (((uintptr_t)T.exp_avg | (uintptr_t)T.exp_avg_sq) & smask)) == 0) B.vec |= 1ull << B.n;
       B.block0[B.n++] = blocks;

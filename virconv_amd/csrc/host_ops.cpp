@@ -288,8 +288,8 @@ bool plain(const Tensor& t, const Tensor& p, at::ScalarType type) {   // a tenso
   return t.layout() == at::kStrided && t.scalar_type() == type && t.device() == p.device() && t.sizes() == p.sizes() && t.is_contiguous();
 }
 
-// One step of `params` with their state dicts, all in the ordinary case: gradients present, one type, one device, row-major, one step count,
-// moments as they are made.  -> the step taken, or -1 with nothing done: the caller sorts the case out.
+// One step of `params` (those with gradients) with their state dicts (None: not there yet), all in the ordinary case: one device, row-major, one
+// step count, moments as they are made; a call for each type.  -> the step taken, or -1 with nothing done: the caller sorts the case out.
 int64_t adamw(const py::list& params, const py::list& states, int64_t first_place, int state_bits, double lr, double b1, double b2, double eps,
               double weight_decay, int64_t seed) {
   static PyObject* const kStep = PyUnicode_InternFromString("step");
@@ -298,28 +298,36 @@ int64_t adamw(const py::list& params, const py::list& states, int64_t first_plac
   static PyObject* const kRms = PyUnicode_InternFromString("exp_avg_rms");
   static PyObject* const kExponents = PyUnicode_InternFromString("exponents");
   const size_t n = PyList_GET_SIZE(params.ptr());
-  if (n == 0 || (size_t)PyList_GET_SIZE(states.ptr()) != n) return -1;
+  if ((size_t)PyList_GET_SIZE(states.ptr()) != n) return -1;
   const at::ScalarType moment = state_bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
-  std::vector<vc_adamw_tensor> table(n);
-  int64_t step = -1;
+  std::vector<vc_adamw_tensor> table[3];     // by vc_dtype
+  std::vector<PyObject*> live;
+  int64_t step = 0;
   Tensor first;
   for (size_t k = 0; k < n; ++k) {
     PyObject *po = PyList_GET_ITEM(params.ptr(), k), *st = PyList_GET_ITEM(states.ptr(), k);
-    if (!THPVariable_Check(po) || !PyDict_Check(st)) return -1;
+    if (!THPVariable_Check(po)) return -1;
     const Tensor& p = THPVariable_Unpack(po);
-    if (k == 0) first = p;
-    if (!p.is_cuda() || p.scalar_type() != first.scalar_type() || p.device() != first.device() || p.layout() != at::kStrided || !p.is_contiguous()) return -1;
     const Tensor& g = p.grad();
-    if (!g.defined() || !plain(g, p, p.scalar_type())) return -1;
+    if (!g.defined()) continue;
+    if (!PyDict_Check(st)) return -1;
+    if (!first.defined()) first = p;
+    if (!p.is_cuda() || p.device() != first.device() || p.layout() != at::kStrided || !p.is_contiguous() || !plain(g, p, p.scalar_type())) return -1;
+    int dt;
+    switch (p.scalar_type()) {
+      case at::kFloat: dt = VC_F32; break;
+      case at::kHalf: dt = VC_F16; break;
+      case at::kBFloat16: dt = VC_BF16; break;
+      default: return -1;
+    }
     PyObject *so = PyDict_GetItem(st, kStep), *mo = PyDict_GetItem(st, kAvg), *vo = PyDict_GetItem(st, state_bits == 8 ? kRms : kSq);
     if (!so || !PyLong_CheckExact(so) || !mo || !vo || !THPVariable_Check(mo) || !THPVariable_Check(vo)) return -1;
     const int64_t s = PyLong_AsLongLong(so);
-    if (k == 0) step = s;
+    if (live.empty()) step = s;
     if (s != step || s < 0) return -1;
     const Tensor &m = THPVariable_Unpack(mo), &v = THPVariable_Unpack(vo);
     if (!plain(m, p, moment) || !plain(v, p, moment)) return -1;
-    vc_adamw_tensor& t = table[k];
-    t = {p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), nullptr, p.numel(), (uint32_t)(first_place + k), 0};
+    vc_adamw_tensor t = {p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), nullptr, p.numel(), (uint32_t)(first_place + k), 0};
     if (state_bits == 8) {
       PyObject* eo = PyDict_GetItem(st, kExponents);
       if (!eo || !THPVariable_Check(eo)) return -1;
@@ -328,20 +336,21 @@ int64_t adamw(const py::list& params, const py::list& states, int64_t first_plac
         return -1;
       t.exponents = (int8_t*)e.data_ptr();
     }
+    if (table[dt].empty()) table[dt].reserve(n - k);
+    table[dt].push_back(t);
+    live.push_back(st);
   }
-  int dt;
-  switch (first.scalar_type()) {
-    case at::kFloat: dt = VC_F32; break;
-    case at::kHalf: dt = VC_F16; break;
-    case at::kBFloat16: dt = VC_BF16; break;
-    default: return -1;
-  }
+  if (live.empty()) return 0;
   {
     const c10::DeviceGuard guard(first.device());
-    check(abi.adamw(table.data(), (int64_t)n, dt, state_bits, lr, b1, b2, eps, weight_decay, step + 1, (uint32_t)seed, stream_of(first)), "vc_adamw");
+    for (int dt = 0; dt < 3; ++dt)
+      if (!table[dt].empty())
+        check(abi.adamw(table[dt].data(), (int64_t)table[dt].size(), dt, state_bits, lr, b1, b2, eps, weight_decay, step + 1, (uint32_t)seed,
+                        stream_of(first)),
+              "vc_adamw");
   }
   PyObject* now = PyLong_FromLongLong(step + 1);
-  for (size_t k = 0; k < n; ++k) PyDict_SetItem(PyList_GET_ITEM(states.ptr(), k), kStep, now);
+  for (PyObject* st : live) PyDict_SetItem(st, kStep, now);
   Py_DECREF(now);
   return step + 1;
 }

@@ -154,7 +154,7 @@ class AdamW(torch.optim.Optimizer):
     def _attach(self):
         be = ops.get_backend()               # raises without libvirconv_hip.so
         self._lib, self._host = be.lib, be.host
-        self._seen, self._order, self._lists = {}, [], {}
+        self._order, self._lists = [], {}
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed}
@@ -251,30 +251,24 @@ class AdamW(torch.optim.Optimizer):
         for k, g in enumerate(self.param_groups):
             ps = g["params"]
             b1, b2 = g["betas"]
-            states = self._states_of(k, ps)
-            if states is not None and self._host.adamw(ps, states, place, self.state_bits, float(g["lr"]), float(b1), float(b2), float(g["eps"]),
-                                                       float(g["weight_decay"]), self.seed & 0xffffffff) >= 0:
+            if self._host.adamw(ps, self._states_of(k, ps), place, self.state_bits, float(g["lr"]), float(b1), float(b2), float(g["eps"]),
+                                float(g["weight_decay"]), self.seed & 0xffffffff) >= 0:
                 place += len(ps)
                 continue
-            # the first step, parameters without gradients, of several types or orders, or something to refuse
-            grads = [p.grad for p in ps]
-            if any(x is None for x in grads):
-                live = [k for k, x in enumerate(grads) if x is not None]
-                places = [place + k for k in live]
-                self._step_tensors(g, [ps[k] for k in live], [grads[k] for k in live], places)
-            else:
-                self._step_tensors(g, ps, grads, range(place, place + len(ps)))
+            # the first step, parameters that joined later or have other orders of their axes, or something to refuse
+            live = [k for k, p in enumerate(ps) if p.grad is not None]
+            self._step_tensors(g, [ps[k] for k in live], [ps[k].grad for k in live], [place + k for k in live])
             place += len(ps)
         return loss
 
     def _states_of(self, k, ps):
-        """The state dicts of group k's parameters, in order; None before all of them have one.  The list is kept as long as self.state holds
-        the same dicts and the group the same parameters."""
+        """The state dicts of group k's parameters, in order, None for one that has none.  The list is kept as long as self.state holds the same
+        dicts and the group the same parameters."""
         if not self._host.same_values(self.state, self._order):
             self._order, self._lists = list(self.state.values()), {}
         known = self._lists.get(k)
         if known is None or not self._host.same_objects(ps, known[0]):
-            known = self._lists[k] = (list(ps), [self.state[p] for p in ps] if all(p in self.state for p in ps) else None)
+            known = self._lists[k] = (list(ps), [self.state[p] if p in self.state else None for p in ps])
         return known[1]
 
     def _step_tensors(self, g, ps, grads, places):
@@ -286,8 +280,7 @@ class AdamW(torch.optim.Optimizer):
         states = [state[p] if p in state else self._new_state(p) for p in ps]
         second = "exp_avg_sq" if self.state_bits == 32 else "exp_avg_rms"
         for p, st in zip(ps, states):
-            if second not in st:
-                self._check_state(p, st)      # raises
+            self._check_state(p, st)
         steps = {st["step"] for st in states}
         dtypes = {p.dtype for p in ps}
         if len(steps) != 1 or len(dtypes) != 1 or not all(type(s) is int for s in steps):
@@ -309,11 +302,6 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: parameters and gradients have to be {dtype} on {first.device}")
         moments = [st["exp_avg"] for st in states], [st[second] for st in states], [st.get("exponents") for st in states]
         sizes = [p.numel() for p in ps]
-        seen = self._seen.get((id(g), places[0], len(ps)))
-        if seen is None or seen[0] != sizes or not all(a is b for x, y in zip(seen[1], moments) for a, b in zip(x, y)):
-            for p, st in zip(ps, states):     # moments that were not here at the last step (a checkpoint, a user's own): looked over once
-                self._check_state(p, st)
-            self._seen[id(g), places[0], len(ps)] = sizes, moments
         table = np.zeros((len(ps), 7), np.int64)
         table[:, 0] = [p.data_ptr() for p in ps]
         table[:, 1] = [x.data_ptr() for x in grads]
