@@ -307,6 +307,41 @@ def test_grouped_linear_many_long_groups(hip_backend, count, inner, outer, dtype
                   rnd((n, outer), 4, dtype, 0.1))
 
 
+@pytest.mark.parametrize("op", ["norm", "grouped"])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_a_captured_backward_beside_an_eager_graph_of_its_leaves_is_refused(hip_backend, op, accumulate):
+    from virconv_amd import ops
+    x, w, dy = rnd((300, 64), 1).requires_grad_(), rnd((64,) if op == "norm" else (2, 64, 64), 2).requires_grad_(), rnd((300, 64), 3)
+    offsets = torch.tensor([0, 100, 300], device="cuda")
+
+    def run():
+        y = ops.layer_norm(x, w) if op == "norm" else ops.grouped_linear(x, w, offsets)
+        if accumulate:
+            y.backward(dy)
+            return y.detach(), x.grad, w.grad
+        return (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+
+    want = [t.clone() for t in run()]
+    alive = ops.layer_norm(x, w) if op == "norm" else ops.grouped_linear(x, w, offsets)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="let go of that result"):
+        with torch.cuda.graph(graph):
+            run()
+    del alive, graph
+    torch.cuda.synchronize()
+    x.grad, w.grad = torch.zeros_like(x), torch.zeros_like(w)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for _ in range(3):
+        x.grad.zero_(), w.grad.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert all(torch.equal(a, b) for a, b in zip(run()[:1], want))
+
+
 def test_two_threads_on_streams_of_their_own(hip_backend):
     import threading
     from virconv_amd import ops
@@ -471,6 +506,51 @@ def test_grouped_linear_beyond_two_to_the_31_elements(hip_backend):
     for name, g, r, s, k in zip(("y", "dx", "dw"), (y[-40:], dx[-40:], dw), want, size, (inner, outer, 40)):
         within(g, r, half_step(BF16) * r.abs() + floor_step(BF16) + (k + 4) * U * s, name)
     assert not y[:100].any() and not dx[:100].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_grouped_linear_large_tiles_beyond_two_to_the_31_elements(hip_backend, dtype):
+    from virconv_amd import ops
+    n, inner, outer = 1_100_000, 2048, 512
+    x = torch.zeros((n, inner), dtype=dtype, device="cuda")
+    x[-40:] = rnd((40, inner), 1, dtype)
+    x.requires_grad_()
+    w = rnd((2, outer, inner), 2, dtype, inner ** -0.5).requires_grad_()
+    y = ops.grouped_linear(x, w, torch.tensor([0, n - 33, n], device="cuda"))
+    dy = torch.zeros((n, outer), dtype=dtype, device="cuda")
+    dy[-40:] = rnd((40, outer), 3, dtype)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    want, size = grouped64(x[-40:], w, [0, 7, 40], None, dy[-40:])
+    for name, g, r, s, k in zip(("y", "dx", "dw"), (y[-40:], dx[-40:], dw), want, size, (inner + 2, outer + 2, 42)):
+        within(g, r, half_step(dtype) * r.abs() + floor_step(dtype) + (k + 4) * U * s, name)
+    assert not y[:-40].any() and not dx[:-40].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_grouped_linear_large_tiles_keep_undefined_values_where_they_belong(hip_backend, dtype):
+    """NaN and infinities in one group's rows and in rows of no group: every other group's results as without them, bit for bit."""
+    from virconv_amd import ops
+    n, inner, outer, ends = 16001, 1032, 2056, [8, 4003, 4003, 9001, 15990]
+    offsets = torch.tensor(ends, device="cuda")
+    x, w, b, dy = rnd((n, inner), 1, dtype), rnd((4, outer, inner), 2, dtype, inner ** -0.5), rnd((4, outer), 3, dtype), rnd((n, outer), 4, dtype)
+
+    def run(x, dy):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        y = ops.grouped_linear(leaves[0], leaves[1], offsets, leaves[2])
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    want = run(x, dy)
+    for bad in (float("nan"), float("inf")):
+        xb, dyb = x.clone(), dy.clone()
+        for t in (xb, dyb):
+            t[:8], t[15990:], t[4003:9001] = bad, bad, bad
+        y, dx, dw, db = run(xb, dyb)
+        for g, r in ((y, want[0]), (dx, want[1])):
+            assert not g[:8].any() and not g[15990:].any()
+            assert torch.equal(g[8:4003], r[8:4003]) and torch.equal(g[9001:15990], r[9001:15990])
+        for g, r in ((dw, want[2]), (db, want[3])):
+            assert not g[1].any()      # (the empty group)
+            assert torch.equal(g[0], r[0]) and torch.equal(g[3], r[3]) and not torch.isfinite(g[2]).any()
 
 
 def test_gradients_are_of_first_order_and_say_so(hip_backend):
@@ -694,6 +774,23 @@ def test_adamw_refusals(hip_backend):
             opt.step()
     torch.cuda.synchronize()
     assert torch.equal(p, before) and opt.state[p]["step"] == 1
+
+
+def test_adamw_beyond_two_to_the_31_elements(hip_backend):
+    from virconv_amd.optim import AdamW
+    n, tail = 2 ** 31 + 5000, 3000
+    big = torch.nn.Parameter(torch.zeros(n, dtype=BF16, device="cuda"))
+    with torch.no_grad():
+        big[-tail:] = rnd((tail,), 1, BF16)
+    small = torch.nn.Parameter(big.detach()[-tail:].clone())
+    opts = AdamW([big], **HYPER), AdamW([small], **HYPER)
+    big.grad = torch.zeros_like(big)
+    for t in range(2):
+        small.grad = rnd((tail,), 2 + t, BF16)
+        big.grad[-tail:] = small.grad
+        for o in opts:
+            o.step()
+        assert torch.equal(big.detach()[-tail:], small.detach()) and not big.detach()[:-tail].any()
 
 
 @pytest.mark.parametrize("bits", [32, 8])

@@ -6,7 +6,9 @@
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <hip/hip_runtime_api.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/pybind.h>
 
@@ -104,6 +106,34 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
   return false;
 }
 
+bool capturing(hipStream_t stream) {     // (the legacy stream never is, and must not be asked while another one is)
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  return stream && hipStreamIsCapturing(stream, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
+}
+
+// A backward pass under capture whose gradients go to nodes recorded before it on a stream that is not captured (a leaf's, while an eager graph of
+// that leaf lives): the engine would make that stream wait for the captured one, which ends the process.  Said here instead.
+void refuse_uncaptured_consumers(const char* who, const Tensor& x) {
+  const c10::hip::HIPStream here = c10::hip::getCurrentHIPStream(x.get_device());
+  if (!capturing(here.stream())) return;
+  const auto node = torch::autograd::get_current_node();
+  const auto* tasks = torch::autograd::get_current_graph_task_exec_info();
+  if (!node) return;
+  for (const auto& edge : node->next_edges()) {
+    if (!edge.function) continue;
+    if (tasks && !tasks->empty()) {
+      const auto it = tasks->find(edge.function.get());
+      if (it == tasks->end() || !it->second.should_execute()) continue;
+    }
+    const auto there = edge.function->stream();
+    if (!there || there->id() == here.id() || there->device_index() != here.device_index()) continue;
+    const c10::Stream plain(c10::Stream::UNSAFE, c10::Device(here.unwrap().device_type(), here.device_index()), there->id());
+    if (!capturing(c10::hip::HIPStream(plain).stream()))
+      throw VirConvError(std::string(who) + ": this backward pass is being captured, and a graph recorded before it, on a stream that is not, holds a node "
+                         "its gradients go to (an eager result of the same leaf that is still alive): let go of that result before the capture");
+  }
+}
+
 // First-order gradients only: where a graph of the backward pass is asked for, its results hang on a node that says so when it is used.
 struct OnceOnly : torch::autograd::Function<OnceOnly> {
   static Tensor forward(AutogradContext*, const Tensor& result, const OptTensor&, const OptTensor&, const OptTensor&) { return result.clone(); }
@@ -150,6 +180,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &stats = saved[2], &dy = grads[0];
+    refuse_uncaptured_consumers("layer_norm", x);
     // (edges are counted over the tensors that are there)
     const bool need_x = ctx->needs_input_grad(0), need_w = w.defined() && ctx->needs_input_grad(1);
     const int64_t bias_type = ctx->saved_data["bias"].toInt();
@@ -228,6 +259,7 @@ struct GroupedLinear : torch::autograd::Function<GroupedLinear> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &offsets = saved[2], &dy = grads[0];
+    refuse_uncaptured_consumers("grouped_linear", x);
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     const bool need_b = ctx->saved_data["bias"].toBool() && ctx->needs_input_grad(3);
     Tensor dx, dw, db;
