@@ -359,20 +359,21 @@ __device__ __forceinline__ v4f mfma(v8s a, v8s b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-// accb += the sums of FM operands of a tile along the summed axis (dbias from dy): operand i times ones in row i, so that the sums of sixteen
-// operands fit in one accumulator.  It reads its operands once more: between the other products it would cut those into pieces that wait for
-// their own reads (weight product with a bias or without, 8192^3: 1010 TFLOP/s so).
-template <typename T, typename Tile, int FM>
-__device__ __forceinline__ void add_bias_sums(const char* lds, const int (&at)[FM], v4f& accb) {
+// accb += the sums of a wave's FM operands of a tile along the summed axis (dbias from dy): operand i times ones in row i, so that the sums of
+// sixteen operands fit in one accumulator.  The WN waves that hold the same operands take every WN-th.  They read them once more: between the
+// other products this would cut those into pieces that wait for their own reads (weight product with a bias or without, 8192^3: 1010 TFLOP/s so).
+template <typename T, typename Tile, int FM, int WN>
+__device__ __forceinline__ void add_bias_sums(const char* lds, int wm0, int wn, v4f& accb) {
 #pragma unroll 1
-  for (int kk = 0; kk < Tile::BK; kk += 32)
+  for (int i = wn; i < FM; i += WN) {
+    const int at = Tile::lane_place(wm0 + i * 16);
+    const short one = (threadIdx.x & 15) != (unsigned)i ? (short)0 : __is_same(T, _Float16) ? (short)0x3c00 : (short)0x3f80;
 #pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const short one = (threadIdx.x & 15) != (unsigned)i ? (short)0 : __is_same(T, _Float16) ? (short)0x3c00 : (short)0x3f80;
+    for (int kk = 0; kk < Tile::BK; kk += 32)
 #pragma unroll
       for (int q = Tile::planes - 1; q >= 0; --q)
-        accb = mfma<T>(v8s{one, one, one, one, one, one, one, one}, Tile::fragment(lds, q, at[i], kk), accb);
-    }
+        accb = mfma<T>(v8s{one, one, one, one, one, one, one, one}, Tile::fragment(lds, q, at, kk), accb);
+  }
 }
 
 template <typename T> __device__ __forceinline__ void store4(T* p, int valid, const float (&x)[4]) {
@@ -506,9 +507,9 @@ __device__ __forceinline__ Work<T> find_work(const GroupArgs& a, Groups& g, cons
 
 // Results of a wave: lane l holds row m = l % 16 and the columns n = 4 (l / 16) .. + 3 of each 16 x 16 tile; (wm0, wn0): the wave's place.
 template <typename T, int FM, int FN, int MODE>
-__device__ __forceinline__ void write_results(const GroupArgs& a, const Work<T>& w, int wm0, int wn0, const v4f (&acc)[FM][FN], const v4f& accb, bool sum_bias) {
+__device__ __forceinline__ void write_results(const GroupArgs& a, const Work<T>& w, int wm0, int wn0, const v4f (&acc)[FM][FN]) {
   const int lane = threadIdx.x & 63;
-  if (!sum_bias && w.rows_a >= wm0 + FM * 16 && w.rows_b >= wn0 + FN * 16) {   // the wave's part of the tile is whole
+  if (w.rows_a >= wm0 + FM * 16 && w.rows_b >= wn0 + FN * 16) {   // the wave's part of the tile is whole
     const int64_t at = (int64_t)(wm0 + (lane & 15)) * a.n + wn0 + (lane >> 4) * 4;
     float* part = w.partial ? w.partial + at : nullptr;
     T* out = (T*)a.out + ((MODE == kBackWeight ? (int64_t)w.group * a.m : 0) + w.m0) * a.n + w.n0 + at;
@@ -558,10 +559,19 @@ __device__ __forceinline__ void write_results(const GroupArgs& a, const Work<T>&
       else out += (w.m0 + m) * a.n + w.n0 + n;
       store4(out, w.rows_b - n, r);
     }
-    if (MODE == kBackWeight && sum_bias && lane >> 4 == i >> 2) {
-      if (w.partial) a.partial_bias[(int64_t)w.piece * a.m + w.m0 + m] = accb[i & 3];
-      else ((T*)a.dbias)[(int64_t)w.group * a.m + w.m0 + m] = (T)accb[i & 3];
-    }
+  }
+}
+
+// ... and what add_bias_sums made of a wave's operands
+template <typename T, int FM, int WN>
+__device__ __forceinline__ void write_bias(const GroupArgs& a, const Work<T>& w, int wm0, int wn, const v4f& accb) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = wm0 + i * 16 + (lane & 15);
+    if (i % WN != wn || lane >> 4 != i >> 2 || m >= w.rows_a) continue;
+    if (w.partial) a.partial_bias[(int64_t)w.piece * a.m + w.m0 + m] = accb[i & 3];
+    else ((T*)a.dbias)[(int64_t)w.group * a.m + w.m0 + m] = (T)accb[i & 3];
   }
 }
 
@@ -589,7 +599,7 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
   const T *const pa = (const T*)a.a + w.pa, *const pb = (const T*)a.b + w.pb;
   const int64_t lda = w.lda, ldb = w.ldb;
   const int rows_a = w.rows_a, rows_b = w.rows_b, depth = w.depth;
-  const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && __builtin_amdgcn_readfirstlane(wn) == 0;
+  const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0;
 
   TileA ta[STAGES];
   TileB tb[STAGES];
@@ -668,7 +678,7 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
         }
       }
     }
-    if (MODE == kBackWeight && sum_bias) add_bias_sums<O, TileA>(la, at_a, accb);
+    if (MODE == kBackWeight && sum_bias) add_bias_sums<O, TileA, FM, WN>(la, wm * (BM / WM), __builtin_amdgcn_readfirstlane(wn), accb);
   };
   int kb = 0;
   if (deep) {
@@ -697,7 +707,8 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
       multiply();
     }
   }
-  write_results<T, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc, accb, sum_bias);
+  write_results<T, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc);
+  if (MODE == kBackWeight && sum_bias) write_bias<T, FM, WN>(a, w, wm * (BM / WM), wn, accb);
 }
 
 // ------------------------------------------------------------------------------------------------ large tiles of fp32 operands
@@ -791,7 +802,7 @@ __global__ void __launch_bounds__(512, 2) grouped_f32_kernel(GroupArgs a) {
 #pragma unroll
   for (int j = 0; j < FN; ++j) at_b[j] = TileB::lane_place(wn * (BN / WN) + j * 16);
   while (!w.none) {
-    const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && wn == 0;
+    const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0;
     v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < FM; ++i)
@@ -825,9 +836,10 @@ __global__ void __launch_bounds__(512, 2) grouped_f32_kernel(GroupArgs a) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma<__bf16>(fb[j][0], fa[0], acc[i][j]);
       }
-      if (MODE == kBackWeight && sum_bias) add_bias_sums<__bf16, TileA>(la, at_a, accb);
+      if (MODE == kBackWeight && sum_bias) add_bias_sums<__bf16, TileA, FM, WN>(la, wm * (BM / WM), wn, accb);
     }
-    write_results<float, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc, accb, sum_bias);
+    write_results<float, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc);
+    if (MODE == kBackWeight && sum_bias) write_bias<float, FM, WN>(a, w, wm * (BM / WM), wn, accb);
     next(w);
   }
 }
@@ -897,7 +909,7 @@ __device__ __forceinline__ void large_products(const GroupArgs& a, Groups& group
   next(w);
   begin(w);
   while (!w.none) {
-    const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0 && __builtin_amdgcn_readfirstlane(wn0) == 0;
+    const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0;
     v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
@@ -924,7 +936,7 @@ __device__ __forceinline__ void large_products(const GroupArgs& a, Groups& group
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma<T>(fb[h][j], fa[q & 1], acc[i][j]);
       }
-      if (MODE == kBackWeight && sum_bias) add_bias_sums<T, TileA>(lds, at_a, accb);
+      if (MODE == kBackWeight && sum_bias) add_bias_sums<T, TileA, FM, WN>(lds, wm0, __builtin_amdgcn_readfirstlane(wave % WN), accb);
     };
     const int steps = w.depth / BK, rest = w.depth % BK;
     for (int t = 0; t < steps; t += 2) {
@@ -981,9 +993,8 @@ __device__ __forceinline__ void large_products(const GroupArgs& a, Groups& group
         }
       }
       out += (int64_t)16 * a.n;
-      if (MODE == kBackWeight && sum_bias && lane >> 4 == i >> 2 && m0 + i * 16 < w.rows_a)
-        ((T*)a.dbias)[(int64_t)w.group * a.m + w.m0 + m0 + i * 16] = (T)accb[i & 3];
     }
+    if (MODE == kBackWeight && sum_bias) write_bias<T, FM, WN>(a, w, wm0, wave % WN, accb);
     w = after;
   }
 }
