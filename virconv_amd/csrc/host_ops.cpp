@@ -320,6 +320,8 @@ bool plain(const Tensor& t, const Tensor& p, at::ScalarType type) {   // a tenso
   return t.layout() == at::kStrided && t.scalar_type() == type && t.device() == p.device() && t.sizes() == p.sizes() && t.is_contiguous();
 }
 
+constexpr const char* kCaptured = "AdamW: a step counts on the host (bias correction, random numbers): it cannot be captured into a graph";
+
 // One step of `params` (those with gradients) with their state dicts (None: not there yet), all in the ordinary case: one device, row-major, one
 // step count, moments as they are made; a call for each type.  -> the step taken, or -1 with nothing done: the caller sorts the case out.
 int64_t adamw(const py::list& params, const py::list& states, int64_t first_place, int state_bits, double lr, double b1, double b2, double eps,
@@ -375,6 +377,7 @@ int64_t adamw(const py::list& params, const py::list& states, int64_t first_plac
   if (live.empty()) return 0;
   {
     const c10::DeviceGuard guard(first.device());
+    if (capturing((hipStream_t)stream_of(first))) throw VirConvError(kCaptured);
     for (int dt = 0; dt < 3; ++dt)
       if (!table[dt].empty())
         check(abi.adamw(table[dt].data(), (int64_t)table[dt].size(), dt, state_bits, lr, b1, b2, eps, weight_decay, step + 1, (uint32_t)seed,
@@ -420,6 +423,7 @@ PYBIND11_MODULE(_host_ops, m) {
   m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
   m.def("grouped_linear", &grouped_linear, py::call_guard<py::gil_scoped_release>());
   m.def("adamw", &adamw);
+  m.attr("ADAMW_CAPTURED") = kCaptured;
   m.def("same_values", &same_values);
   m.def("same_objects", &same_objects);
 }

@@ -239,25 +239,21 @@ class AdamW(torch.optim.Optimizer):
             torch.as_strided(out[-1], (n,), (1,)).copy_(flat)
         return out[0], out[1] * out[1]
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError("AdamW: a step counts on the host (bias correction, random numbers): it cannot be captured into a graph")
         place = 0
         for k, g in enumerate(self.param_groups):
             ps = g["params"]
             b1, b2 = g["betas"]
             if self._host.adamw(ps, self._states_of(k, ps), place, self.state_bits, float(g["lr"]), float(b1), float(b2), float(g["eps"]),
-                                float(g["weight_decay"]), self.seed & 0xffffffff) >= 0:
-                place += len(ps)
-                continue
-            # the first step, parameters that joined later or have other orders of their axes, or something to refuse
-            live = [k for k, p in enumerate(ps) if p.grad is not None]
-            self._step_tensors(g, [ps[k] for k in live], [ps[k].grad for k in live], [place + k for k in live])
+                                float(g["weight_decay"]), self.seed & 0xffffffff) < 0:
+                # the first step, parameters that joined later or have other orders of their axes, or something to refuse
+                live = [k for k, p in enumerate(ps) if p.grad is not None]
+                with torch.no_grad():
+                    self._step_tensors(g, [ps[k] for k in live], [ps[k].grad for k in live], [place + k for k in live])
             place += len(ps)
         return loss
 
@@ -274,6 +270,8 @@ class AdamW(torch.optim.Optimizer):
     def _step_tensors(self, g, ps, grads, places):
         if not ps:
             return
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError(self._host.ADAMW_CAPTURED)
         first = ps[0]
         index = first.get_device()
         state = self.state
