@@ -818,6 +818,29 @@ def test_adamw_types_and_missing_gradients_in_one_group(hip_backend, bits):
             assert all(torch.equal(a, b) for a, b in zip(opt.decoded_state(p), o.decoded_state(q)))
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_many_tensors(hip_backend, bits):
+    """More tensors than a launch's table holds, of many sizes: those around the tables' ends as in optimizers of their own."""
+    from virconv_amd.optim import AdamW
+    g = torch.Generator().manual_seed(1)
+    sizes = [int(v) for v in torch.randint(1, 6000, (200,), generator=g)]
+    joint = [torch.nn.Parameter(rnd((n,), k)) for k, n in enumerate(sizes)]
+    places = [0, 1, 63, 64, 75, 76, 77, 87, 88, 89, 127, 128, 151, 152, 153, 175, 176, 199]
+    apart = {k: torch.nn.Parameter(joint[k].detach().clone()) for k in places}
+    opt = AdamW(joint, state_bits=bits, seed=3, **HYPER)
+    ones = {k: AdamW([*(torch.nn.Parameter(torch.zeros(1, device="cuda")) for _ in range(k)), p], state_bits=bits, seed=3, **HYPER) for k, p in apart.items()}
+    for t in range(3):
+        for k, p in enumerate(joint):
+            p.grad = rnd(p.shape, 1000 * t + k)
+            if k in apart:
+                apart[k].grad = p.grad
+        opt.step()
+        for o in ones.values():
+            o.step()
+        for k in places:
+            assert torch.equal(joint[k], apart[k]), k
+
+
 @pytest.mark.parametrize("channels_last", [False, True])
 def test_adamw_looks_its_states_over_at_every_step(hip_backend, channels_last):
     from virconv_amd.optim import AdamW

@@ -5,8 +5,8 @@
 // in fp32 whatever the parameters' type, every operation rounded by itself (this file is built without contraction), the parameter rounded
 // once to its own type.  The step is one pass over its data and nothing else: what bounds it is HBM -- 28 bytes an element with fp32
 // parameters and 32-bit moments, 16 with 8-bit ones, 10 with bf16 parameters and 8-bit moments.  Measured: 200 M bf16 parameters with 8-bit
-// moments 397 us (5.05 TB/s; a large copy 4.9), 13 M fp32 ones in 193 tensors 88 us with 32-bit moments (4.15 TB/s), 62 us with 8-bit ones (3.4: four
-// launches, as a launch's table holds 64 tensors, and their ends); 0.42 M in 87 tensors 11 us in two launches, 23 us of host time.
+// moments 389 us (5.16 TB/s; a large copy 4.9), 13 M fp32 ones in 193 tensors 81 us with 32-bit moments (4.5 TB/s), 56 us with 8-bit ones (3.7: three
+// launches and their ends; with 64 tensors a launch 88 and 62 us); 0.42 M in 87 tensors 18 us of host time, one launch (23 and two).
 //
 // 8-bit moments.  m and r = sqrt(v) are held as e4m3 values over a power of two per 128 elements: value * 2^(exponent - 7), the block's
 // largest magnitude lying in [128, 256) before the power is taken off.  r and not v: the root halves the range that a block has to span.
@@ -24,25 +24,27 @@
 
 namespace vc {
 
-static constexpr int kAdamwTensors = 64;    // per launch: the table travels in the kernel's arguments (64 x 48 + 64 x 4 bytes < 4 KB)
 static constexpr int kAdamwChunk = 2048;    // elements of one block: 256 threads x 8
 static constexpr int kStateBlock = 128;     // elements that share an exponent: 16 lanes x 8
 
-struct AdamwTensor {
+// A launch's tensors travel in the kernel's arguments, as many as fit: 4 KB.
+struct AdamwTensor32 {
   void* param;
   const void* grad;
   void *exp_avg, *exp_avg_sq;
-  int8_t* exponents;
-  uint64_t n_place;      // elements (44 bits), place in the model (20 bits)
+  uint64_t n_place;      // elements (40 bits), place in the model (20 bits), bit 63: the pointers allow 16-byte accesses (8-byte ones of 8-bit states)
 };
+struct AdamwTensor8 : AdamwTensor32 { int8_t* exponents; };
 
+template <typename Entry>
 struct AdamwTable {
-  AdamwTensor t[kAdamwTensors];
-  unsigned block0[kAdamwTensors];
-  uint64_t vec;          // a bit a tensor: its pointers allow 16-byte accesses (8-byte ones of the 8-bit states)
+  static constexpr int kMost = sizeof(Entry) == 40 ? 88 : 76;
+  Entry t[kMost];
+  unsigned block0[kMost];
   int n;
 };
-static_assert(sizeof(AdamwTable) < 3600, "kernel arguments are limited to 4 KB");
+typedef AdamwTable<AdamwTensor32> AdamwTable32;
+typedef AdamwTable<AdamwTensor8> AdamwTable8;
 
 __host__ __device__ static inline uint32_t mix32(uint32_t x) {   // the finalizer of MurmurHash3
   x ^= x >> 16; x *= 0x85ebca6bu; x ^= x >> 13; x *= 0xc2b2ae35u; x ^= x >> 16;
@@ -53,6 +55,8 @@ struct AdamwArgs {
   float beta1, beta2, one_minus_beta1, one_minus_beta2, eps, keep, step_size, inv_bc2_sqrt;
   uint32_t key;          // of the seed and the step
 };
+
+static_assert(sizeof(AdamwTable32) + sizeof(AdamwArgs) < 4096 && sizeof(AdamwTable8) + sizeof(AdamwArgs) < 4096, "kernel arguments are limited to 4 KB");
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
@@ -97,20 +101,23 @@ __device__ __forceinline__ void store8(T* p, int64_t i, int64_t n, bool vec, con
   }
 }
 
-__device__ __forceinline__ int adamw_find(const AdamwTable& B) {
-  // the last tensor that begins at or before this block: one lane a tensor
+template <typename Entry>
+__device__ __forceinline__ int adamw_find(const AdamwTable<Entry>& B) {
+  // the last tensor that begins at or before this block: one lane a tensor, twice
   const int lane = threadIdx.x & 63;
-  const unsigned b0 = lane < B.n ? B.block0[lane] : 0xffffffffu;
-  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(b0 <= blockIdx.x)) - 1);
+  const unsigned b0 = lane < B.n ? B.block0[lane] : 0xffffffffu, b1 = lane + 64 < B.n ? B.block0[lane + 64] : 0xffffffffu;
+  return __builtin_amdgcn_readfirstlane(__popcll(__ballot(b0 <= blockIdx.x)) + __popcll(__ballot(b1 <= blockIdx.x)) - 1);
 }
+template <typename Entry>
+__device__ __forceinline__ int64_t adamw_size(const Entry& S) { return (int64_t)(S.n_place & ((1ull << 40) - 1)); }
 
 template <typename T>
-__global__ void __launch_bounds__(256) adamw32_kernel(AdamwTable B, AdamwArgs a) {
+__global__ void __launch_bounds__(256) adamw32_kernel(AdamwTable32 B, AdamwArgs a) {
   const int s = adamw_find(B);
-  const AdamwTensor& S = B.t[s];
-  const int64_t n = (int64_t)(S.n_place & ((1ull << 44) - 1)), i = (int64_t)(blockIdx.x - B.block0[s]) * kAdamwChunk + threadIdx.x * 8;
+  const AdamwTensor32& S = B.t[s];
+  const int64_t n = adamw_size(S), i = (int64_t)(blockIdx.x - B.block0[s]) * kAdamwChunk + threadIdx.x * 8;
   if (i >= n) return;
-  const bool vec = B.vec >> s & 1;
+  const bool vec = S.n_place >> 63;
   float p[8], g[8], m[8], v[8];
   load8((const T*)S.grad, i, n, vec, g);
   load8((const float*)S.exp_avg, i, n, vec, m);
@@ -183,12 +190,12 @@ __device__ __forceinline__ void put8(void* codes, int64_t i, int64_t n, bool vec
 // v_rsq and v_rcp in place of the library's root and quotient, and the first product of the mixing function from its neighbour's: the eight
 // arguments of a lane differ in three bits, so their products differ by +-1, +-2, +-4 times the factor.
 template <typename T>
-__global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable B, AdamwArgs a) {
+__global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable8 B, AdamwArgs a) {
   const int s = adamw_find(B);
-  const AdamwTensor& S = B.t[s];
-  const int64_t n = (int64_t)(S.n_place & ((1ull << 44) - 1)), i = (int64_t)(blockIdx.x - B.block0[s]) * kAdamwChunk + threadIdx.x * 8;
+  const AdamwTensor8& S = B.t[s];
+  const int64_t n = adamw_size(S), i = (int64_t)(blockIdx.x - B.block0[s]) * kAdamwChunk + threadIdx.x * 8;
   // 16 lanes share an exponent, and all 16 are here for the maximum: the lanes behind the last element carry zeros
-  const bool vec = B.vec >> s & 1;
+  const bool vec = S.n_place >> 63;
   const int64_t blk = i / kStateBlock;
   const bool live = blk * kStateBlock < n;
   float p[8], g[8], m[8], r[8];
@@ -222,7 +229,7 @@ __global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable B, AdamwArgs a) 
   const int em = max((int)(mtop >> 23) - 127, -119), er = vtop ? ((int)(vtop >> 23) - 127) >> 1 : -119;
   const float mscale = __uint_as_float((uint32_t)(134 - em) << 23), rscale = __uint_as_float((uint32_t)(134 - er) << 23);   // 2^(7 - e)
   constexpr uint32_t kFirst = 0x85ebca6bu, kSecond = 0xc2b2ae35u;
-  uint32_t x0 = mix32(a.key + (uint32_t)(S.n_place >> 44)) ^ (uint32_t)i ^ (uint32_t)(i >> 32) * 0x9e3779b9u;
+  uint32_t x0 = mix32(a.key + ((uint32_t)(S.n_place >> 40) & 0xfffffu)) ^ (uint32_t)i ^ (uint32_t)(i >> 32) * 0x9e3779b9u;
   x0 ^= x0 >> 16;     // (i is a multiple of 8: the element's three bits come in unshifted)
   const uint32_t p0 = x0 * kFirst, d1 = x0 & 1 ? 0u - kFirst : kFirst, d2 = x0 & 2 ? 0u - 2 * kFirst : 2 * kFirst,
                  d4 = x0 & 4 ? 0u - 4 * kFirst : 4 * kFirst;
@@ -254,6 +261,46 @@ struct Span {
   bool operator<(const Span& o) const { return a < o.a; }
 };
 
+static void fill(AdamwTensor32& e, const vc_adamw_tensor& T, uint64_t n_place) { e = {T.param, T.grad, T.exp_avg, T.exp_avg_sq, n_place}; }
+static void fill(AdamwTensor8& e, const vc_adamw_tensor& T, uint64_t n_place) {
+  fill(static_cast<AdamwTensor32&>(e), T, n_place);
+  e.exponents = T.exponents;
+}
+
+template <typename Entry, typename Launch>
+static int adamw_tables(const vc_adamw_tensor* tensors, int64_t n_tensors, uintptr_t wide, uintptr_t wide_state, Launch launch) {
+  AdamwTable<Entry> B;
+  for (int64_t k = 0; k < n_tensors;) {
+    B.n = 0;
+    unsigned blocks = 0;
+    for (; k < n_tensors && B.n < B.kMost; ++k) {
+      const vc_adamw_tensor& T = tensors[k];
+      if (T.n == 0) continue;
+      const int64_t need = cdiv(T.n, kAdamwChunk);
+      if (B.n && (int64_t)blocks + need >= (1LL << 24)) break;     // (2^32 threads)
+      const bool vec = ((((uintptr_t)T.param | (uintptr_t)T.grad) & wide) | (((uintptr_t)T.exp_avg | (uintptr_t)T.exp_avg_sq) & wide_state)) == 0;
+      fill(B.t[B.n], T, (uint64_t)T.n | (uint64_t)T.key << 40 | (uint64_t)vec << 63);
+      B.block0[B.n++] = blocks;
+      blocks += (unsigned)need;
+    }
+    if (B.n == 0) break;
+    launch(B, blocks);
+    VC_CHECK_LAUNCH("adamw_kernel");
+  }
+  return VC_OK;
+}
+
+template <typename T>
+static int adamw_launch(const vc_adamw_tensor* tensors, int64_t n_tensors, int state_bits, const AdamwArgs& a, hipStream_t st) {
+  if (state_bits == 32)
+    return adamw_tables<AdamwTensor32>(tensors, n_tensors, 15, 15, [&](const AdamwTable32& B, unsigned blocks) {
+      hipLaunchKernelGGL(adamw32_kernel<T>, dim3(blocks), dim3(256), 0, st, B, a);
+    });
+  return adamw_tables<AdamwTensor8>(tensors, n_tensors, 15, 7, [&](const AdamwTable8& B, unsigned blocks) {
+    hipLaunchKernelGGL(adamw8_kernel<T>, dim3(blocks), dim3(256), 0, st, B, a);
+  });
+}
+
 }  // namespace vc
 
 using namespace vc;
@@ -268,7 +315,6 @@ int vc_adamw(const vc_adamw_tensor* tensors, int64_t n_tensors, int dtype, int s
   VC_REQUIRE(step >= 1, "vc_adamw: step = %lld (the first step is 1)", (long long)step);
   VC_REQUIRE(beta1 >= 0. && beta1 < 1. && beta2 >= 0. && beta2 < 1., "vc_adamw: betas (%g, %g) outside [0, 1)", beta1, beta2);
   const int64_t psize = dtype == VC_F32 ? 4 : 2, ssize = state_bits / 8;
-  const uintptr_t smask = ssize == 4 ? 15 : 7;
   hipStream_t st = (hipStream_t)stream;
   // what is written must not overlap: two blocks would race on it
   Span stack[256];
@@ -302,33 +348,9 @@ int vc_adamw(const vc_adamw_tensor* tensors, int64_t n_tensors, int dtype, int s
   a.step_size = (float)(lr / (1.0 - pow(beta1, (double)step)));
   a.inv_bc2_sqrt = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
   a.key = mix32(mix32(seed) + (uint32_t)step);
-  AdamwTable B;
-  int64_t k = 0;
-  while (k < n_tensors) {
-    B.n = 0;
-    B.vec = 0;
-    unsigned blocks = 0;
-    for (; k < n_tensors && B.n < kAdamwTensors; ++k) {
-      const vc_adamw_tensor& T = tensors[k];
-      if (T.n == 0) continue;
-      const int64_t need = cdiv(T.n, kAdamwChunk);
-      if (B.n && (int64_t)blocks + need >= (1LL << 24)) break;     // (2^32 threads)
-      B.t[B.n] = {T.param, T.grad, T.exp_avg, T.exp_avg_sq, T.exponents, (uint64_t)T.n | (uint64_t)T.key << 44};
-      if (((((uintptr_t)T.param | (uintptr_t)T.grad) & 15) | (((uintptr_t)T.exp_avg | (uintptr_t)T.exp_avg_sq) & smask)) == 0) B.vec |= 1ull << B.n;
-      B.block0[B.n++] = blocks;
-      blocks += (unsigned)need;
-    }
-    if (B.n == 0) break;
-#define VC_ADAMW_LAUNCH(T)                                                                                              \
-  if (state_bits == 32) hipLaunchKernelGGL(adamw32_kernel<T>, dim3(blocks), dim3(256), 0, st, B, a);                    \
-  else hipLaunchKernelGGL(adamw8_kernel<T>, dim3(blocks), dim3(256), 0, st, B, a)
-    if (dtype == VC_F32) { VC_ADAMW_LAUNCH(float); }
-    else if (dtype == VC_F16) { VC_ADAMW_LAUNCH(_Float16); }
-    else { VC_ADAMW_LAUNCH(__bf16); }
-#undef VC_ADAMW_LAUNCH
-    VC_CHECK_LAUNCH("adamw_kernel");
-  }
-  return VC_OK;
+  return dtype == VC_F32   ? adamw_launch<float>(tensors, n_tensors, state_bits, a, st)
+         : dtype == VC_F16 ? adamw_launch<_Float16>(tensors, n_tensors, state_bits, a, st)
+                           : adamw_launch<__bf16>(tensors, n_tensors, state_bits, a, st);
 }
 
 }  // extern "C"

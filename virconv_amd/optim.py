@@ -12,7 +12,7 @@ between the two.  It wants what ``feature_pass.flatten_parameters`` returns: a f
 There is no CPU path: without the HIP library the constructor raises.
 
 ``AdamW`` takes a model as it is -- any number of fp32, fp16 or bf16 parameters, any number of groups -- and keeps the moments in 32 or in
-8 bits (vc_adamw): one launch per 64 tensors, no clip inside.
+8 bits (vc_adamw): one launch per 88 or 76 tensors, no clip inside.
 """
 from __future__ import annotations
 
