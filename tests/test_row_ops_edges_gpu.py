@@ -1,0 +1,111 @@
+"""Layer norm, grouped products and the optimizers where a user's program meets something unusual: what else holds on to the tensors that a step
+writes, values that are not finite, products of worst-case mantissas, graphs with nodes in between.
+
+Tolerances are bounds, not fits: u = 2^-24 is half a step of fp32."""
+import copy
+import ctypes
+import math
+
+import pytest
+import torch
+
+from rowref import floor_step, half_step
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+HYPER = dict(lr=2e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.02)
+
+
+def rnd(shape, seed, dtype=F32, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(dtype).cuda()
+
+
+# ---------------------------------------------------------------------------------------------------------------- who else sees a step
+@pytest.mark.parametrize("channels_last", [False, True])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_raises_the_version_of_what_it_writes(hip_backend, bits, channels_last):
+    from virconv_amd.optim import AdamW
+    ps = [torch.nn.Parameter(rnd((8, 6, 3, 5), 1)), torch.nn.Parameter(rnd((70,), 2, BF16)), torch.nn.Parameter(rnd((9,), 3))]
+    if channels_last:     # (such a group takes the path for parameters of any order)
+        ps[0] = torch.nn.Parameter(ps[0].detach().to(memory_format=torch.channels_last))
+    opt = AdamW(ps, state_bits=bits, **HYPER)
+    for t in range(3):
+        for k, p in enumerate(ps):
+            p.grad = rnd(p.shape, 10 * t + k, p.dtype) if k < 2 else None
+        written = ps[:2] + [v for p in ps[:2] if p in opt.state for v in opt.state[p].values() if torch.is_tensor(v)]
+        read = [ps[2], *(p.grad for p in ps[:2])]
+        before = [v._version for v in written], [v._version for v in read]
+        opt.step()
+        assert all(v._version > b for v, b in zip(written, before[0])), t
+        assert [v._version for v in read] == before[1], t
+
+
+@pytest.mark.parametrize("scale_grads", [False, True])
+def test_clip_adamw_raises_the_version_of_what_it_writes(hip_backend, scale_grads):
+    from virconv_amd.optim import ClipAdamW
+    ps = [torch.nn.Parameter(rnd((500,), 1)), torch.nn.Parameter(rnd((70,), 2)), torch.nn.Parameter(rnd((9,), 3))]
+    opt = ClipAdamW(ps, scale_grads=scale_grads)
+    for t in range(3):
+        for k, p in enumerate(ps[:2]):
+            p.grad = rnd(p.shape, 10 * t + k)
+        grads = [p.grad for p in ps[:2]]
+        written = ps[:2] + [opt.state[p][k] for p in ps[:2] if p in opt.state for k in ("exp_avg", "exp_avg_sq")]
+        written += [opt.total_norm] if opt.total_norm is not None else []
+        read = [ps[2]]
+        (written if scale_grads else read).extend(grads)
+        before = [v._version for v in written], [v._version for v in read]
+        opt.step()
+        assert all(v._version > b for v, b in zip(written, before[0])), t
+        assert [v._version for v in read] == before[1], t
+
+
+@pytest.mark.parametrize("which", ["AdamW", "ClipAdamW"])
+@pytest.mark.parametrize("op", ["norm", "grouped", "torch"])
+def test_a_step_between_forward_and_backward_is_refused_by_autograd(hip_backend, op, which):
+    from virconv_amd import ops, optim
+    x, dy = rnd((30, 24), 1).requires_grad_(), rnd((30, 24), 2)
+    w = torch.nn.Parameter(rnd((24,) if op == "norm" else (1, 24, 24) if op == "grouped" else (24, 24), 3))
+    offsets = torch.tensor([0, 30], device="cuda")
+    run = {"norm": lambda: ops.layer_norm(x, w), "grouped": lambda: ops.grouped_linear(x, w, offsets), "torch": lambda: x @ w}[op]
+    opt = getattr(optim, which)([w], lr=1e-3)
+    run().backward(dy)
+    y = run()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
+    run().backward(dy)
+
+
+@pytest.mark.parametrize("which", ["AdamW", "AdamW8", "ClipAdamW"])
+def test_the_sparse_bev_stem_follows_its_optimizer(hip_backend, which):
+    """The stem keeps its conv weight in a packed form: after every step its map and gradients are those of the dense recipe on the new weight."""
+    from test_bev_stem import _backbone_out, _first_block
+    from virconv_amd import optim
+    from virconv_amd.backbone import HeightCompression
+    from virconv_amd.bev_stem import SparseBEVStem
+    bd = _backbone_out("cuda")
+    t = bd["encoded_spconv_tensor"]
+    block = _first_block().cuda().train()
+    stem = SparseBEVStem(block)
+    assert stem.sparse_path_usable(t)
+    opt = {"AdamW": lambda: optim.AdamW(block.parameters(), lr=2e-2), "AdamW8": lambda: optim.AdamW(block.parameters(), lr=2e-2, state_bits=8),
+           "ClipAdamW": lambda: optim.ClipAdamW(block.parameters(), lr=2e-2)}[which]()
+    pull = rnd((2, 64, 200, 176), 5)
+    last = None
+    for _ in range(3):
+        dense = copy.deepcopy(block)
+        opt.zero_grad()
+        got = stem(t)
+        (got * pull).mean().backward()
+        want = dense(HeightCompression({"NUM_BEV_FEATURES": 256})(dict(bd))["spatial_features"])
+        (want * pull).mean().backward()
+        # (the tolerances that the stem's own tests derive: 1e-4 of the value and of the largest one)
+        assert bool(((got - want).abs() <= 1e-4 * want.abs() + 1e-5 * max(1.0, float(want.detach().abs().max()))).all())
+        for p, q in zip(block.parameters(), dense.parameters()):
+            assert float((p.grad - q.grad).abs().max()) <= 1e-4 * float(q.grad.abs().max())
+        assert last is None or float((got - last).detach().abs().max()) > 1e-2     # the step is large enough to be seen
+        last = got
+        opt.step()

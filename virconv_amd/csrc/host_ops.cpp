@@ -320,6 +320,12 @@ bool plain(const Tensor& t, const Tensor& p, at::ScalarType type) {   // a tenso
   return t.layout() == at::kStrided && t.scalar_type() == type && t.device() == p.device() && t.sizes() == p.sizes() && t.is_contiguous();
 }
 
+// Memory that was written through a pointer: what keeps something by the tensor's version (autograd's saved tensors, packed weights) has to see it.
+// (A tensor made in inference mode has no version.)
+void written(c10::TensorImpl* t) {
+  if (t && !t->is_inference()) t->bump_version();
+}
+
 constexpr const char* kCaptured = "AdamW: a step counts on the host (bias correction, random numbers): it cannot be captured into a graph";
 
 // One step of `params` (those with gradients) with their state dicts (None: not there yet), all in the ordinary case: one device, row-major, one
@@ -336,6 +342,8 @@ int64_t adamw(const py::list& params, const py::list& states, int64_t first_plac
   const at::ScalarType moment = state_bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
   std::vector<vc_adamw_tensor> table[3];     // by vc_dtype
   std::vector<PyObject*> live;
+  struct Results { c10::TensorImpl* t[4]; };     // what a tensor's step writes
+  std::vector<Results> results[3];
   int64_t step = 0;
   Tensor first;
   for (size_t k = 0; k < n; ++k) {
@@ -362,6 +370,7 @@ int64_t adamw(const py::list& params, const py::list& states, int64_t first_plac
     const Tensor &m = THPVariable_Unpack(mo), &v = THPVariable_Unpack(vo);
     if (!plain(m, p, moment) || !plain(v, p, moment)) return -1;
     vc_adamw_tensor t = {p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), nullptr, p.numel(), (uint32_t)(first_place + k), 0};
+    Results r = {{p.unsafeGetTensorImpl(), m.unsafeGetTensorImpl(), v.unsafeGetTensorImpl(), nullptr}};
     if (state_bits == 8) {
       PyObject* eo = PyDict_GetItem(st, kExponents);
       if (!eo || !THPVariable_Check(eo)) return -1;
@@ -369,20 +378,28 @@ int64_t adamw(const py::list& params, const py::list& states, int64_t first_plac
       if (e.scalar_type() != at::kChar || e.device() != p.device() || e.dim() != 2 || e.size(0) != (t.n + 127) / 128 || e.size(1) != 2 || !e.is_contiguous())
         return -1;
       t.exponents = (int8_t*)e.data_ptr();
+      r.t[3] = e.unsafeGetTensorImpl();
     }
-    if (table[dt].empty()) table[dt].reserve(n - k);
+    if (table[dt].empty()) {
+      table[dt].reserve(n - k);
+      results[dt].reserve(n - k);
+    }
     table[dt].push_back(t);
+    results[dt].push_back(r);
     live.push_back(st);
   }
   if (live.empty()) return 0;
   {
     const c10::DeviceGuard guard(first.device());
     if (capturing((hipStream_t)stream_of(first))) throw VirConvError(kCaptured);
-    for (int dt = 0; dt < 3; ++dt)
-      if (!table[dt].empty())
-        check(abi.adamw(table[dt].data(), (int64_t)table[dt].size(), dt, state_bits, lr, b1, b2, eps, weight_decay, step + 1, (uint32_t)seed,
-                        stream_of(first)),
-              "vc_adamw");
+    for (int dt = 0; dt < 3; ++dt) {
+      if (table[dt].empty()) continue;
+      check(abi.adamw(table[dt].data(), (int64_t)table[dt].size(), dt, state_bits, lr, b1, b2, eps, weight_decay, step + 1, (uint32_t)seed,
+                      stream_of(first)),
+            "vc_adamw");
+      for (const Results& r : results[dt])
+        for (c10::TensorImpl* t : r.t) written(t);
+    }
   }
   PyObject* now = PyLong_FromLongLong(step + 1);
   for (PyObject* st : live) PyDict_SetItem(st, kStep, now);

@@ -26,6 +26,10 @@ from . import _lib, ops
 from ._lib import ADAM_MAX_TENSORS as MAX_TENSORS, AdamTensor
 
 
+_written = torch.autograd.graph.increment_version
+"""Memory that a kernel wrote through a pointer: autograd's saved tensors, and caches keyed on a version (SparseBEVStem's packed weight), see it by that."""
+
+
 def supports(params) -> bool:
     """Can ClipAdamW take this parameter list?  (a few contiguous fp32 CUDA tensors: the flat parameters of a flattened model)"""
     params = list(params)
@@ -104,6 +108,8 @@ class ClipAdamW(torch.optim.Optimizer):
                                            float(g["weight_decay"]), steps.pop(), float(max_norm) if max_norm else 0.0,
                                            int(bool(g["scale_grads"])), self._norm.data_ptr(), self._ws.data_ptr(), n_ws,
                                            torch._C._cuda_getCurrentRawStream(self._device.index)), "vc_clip_adamw")
+        _written([self._norm, *live, *(self.state[p][k] for p in live for k in ("exp_avg", "exp_avg_sq")),
+                  *((p.grad for p in live) if g["scale_grads"] else ())])
         return self._norm if loss is None else loss
 
     @property
@@ -314,6 +320,7 @@ class AdamW(torch.optim.Optimizer):
             _lib.check(self._lib.vc_adamw(table.ctypes.data, len(ps), _PARAM_DTYPES[dtype], self.state_bits, float(g["lr"]), float(b1), float(b2),
                                           float(g["eps"]), float(g["weight_decay"]), step, self.seed & 0xffffffff,
                                           torch._C._cuda_getCurrentRawStream(index)), "vc_adamw")
+        _written([*ps, *(t for ts in moments for t in ts if t is not None)])
         for st in states:
             st["step"] = step
 
