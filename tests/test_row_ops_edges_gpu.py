@@ -109,3 +109,37 @@ def test_the_sparse_bev_stem_follows_its_optimizer(hip_backend, which):
         assert last is None or float((got - last).detach().abs().max()) > 1e-2     # the step is large enough to be seen
         last = got
         opt.step()
+
+
+# ---------------------------------------------------------------------------------------------------------------- not finite
+BIAS_TILES = [  # (dtype, rows' bounds, inner, outer): the tiles of the weight product, its rows whole and in pieces
+    (F32, [0, 5, 300], 40, 48), (BF16, [0, 5, 300], 40, 48), (F16, [0, 9001], 40, 48),          # 64 x 64
+    (F32, [0, 5, 300], 200, 328), (BF16, [0, 5, 300], 200, 328), (F16, [0, 5, 300], 200, 328),  # 128 x 128
+    (F32, [0, 9001], 136, 264), (BF16, [0, 9001], 136, 264),                                    # ... in pieces
+    (BF16, [0, 5, 300], 2560, 4096), (F16, [0, 5, 300], 2560, 2056),                            # 256 x 256
+    (F32, [0, 5, 300], 5, 328), (BF16, [0, 5, 300], 5, 328),                                    # few channels
+]
+
+
+@pytest.mark.parametrize("dtype,ends,inner,outer", BIAS_TILES, ids=str)
+def test_a_bias_gradient_keeps_undefined_values_in_their_channel(hip_backend, dtype, ends, inner, outer):
+    from virconv_amd import ops
+    groups, n = len(ends) - 1, ends[-1]
+    x, w, b, dy = rnd((n, inner), 1, dtype), rnd((groups, outer, inner), 2, dtype), rnd((groups, outer), 3, dtype), rnd((n, outer), 4, dtype)
+    offsets = torch.tensor(ends, device="cuda")
+
+    def run(dy):
+        leaves = [w.detach().requires_grad_(), b.detach().requires_grad_()]
+        return torch.autograd.grad(ops.grouped_linear(x, leaves[0], offsets, leaves[1]), leaves, dy)
+
+    dw, db = run(dy)
+    for value in (math.inf, -math.inf, math.nan):
+        for c in (0, 17, outer // 2 + 3, outer - 1):
+            bad = dy.clone()
+            bad[n - 7, c] = value            # (a row of the last group)
+            gw, gb = run(bad)
+            keep = torch.ones(outer, dtype=torch.bool, device="cuda")
+            keep[c] = False
+            assert torch.equal(gb[:-1], db[:-1]) and torch.equal(gb[-1, keep], db[-1, keep]), (value, c)
+            assert torch.equal(gw[:-1], dw[:-1]) and torch.equal(gw[-1, keep], dw[-1, keep]), (value, c)
+            assert not bool(torch.isfinite(gb[-1, c])) and not bool(torch.isfinite(gw[-1, c]).any()), (value, c)

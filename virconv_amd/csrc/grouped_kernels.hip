@@ -359,20 +359,29 @@ __device__ __forceinline__ v4f mfma(v8s a, v8s b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
 
-// accb += the sums of a wave's FM operands of a tile along the summed axis (dbias from dy): operand i times ones in row i, so that the sums of
-// sixteen operands fit in one accumulator.  The WN waves that hold the same operands take every WN-th.  They read them once more: between the
-// other products this would cut those into pieces that wait for their own reads (weight product with a bias or without, 8192^3: 1010 TFLOP/s so).
+// The sums of a wave's operands of a tile along the summed axis (dbias from dy), by products with ones.  The WN waves that hold the same FM operands
+// take every WN-th.  Each operand's sum of a step stands by itself: with ones in one row of a result that several operands share, an infinite value
+// would bring 0 * inf into the sums of the others.  Every row of the result holds the same sums, of which a lane keeps one, that of channel lane % 16
+// (kept as the instruction's four, or unrolled, the 256 x 256 tiles spill; in a loop the fp32 tiles are 2 to 5 per cent slower).  The operands are
+// read once more: between the other products this would cut those into pieces that wait for their own reads (weight product with a bias or without,
+// 8192^3: 1010 TFLOP/s so).
+template <int FM, int WN> struct BiasSums { static constexpr int n = (FM + WN - 1) / WN; float acc[n]; };
 template <typename T, typename Tile, int FM, int WN>
-__device__ __forceinline__ void add_bias_sums(const char* lds, int wm0, int wn, v4f& accb) {
-#pragma unroll 1
-  for (int i = wn; i < FM; i += WN) {
-    const int at = Tile::lane_place(wm0 + i * 16);
-    const short one = (threadIdx.x & 15) != (unsigned)i ? (short)0 : __is_same(T, _Float16) ? (short)0x3c00 : (short)0x3f80;
+__device__ __forceinline__ void add_bias_sums(const char* lds, int wm0, int wn, BiasSums<FM, WN>& sums) {
+  static_assert(FM % WN == 0, "as many operands a wave");
+  constexpr short one = __is_same(T, _Float16) ? (short)0x3c00 : (short)0x3f80;
+  constexpr int kTogether = FM < 8 ? BiasSums<FM, WN>::n : 1;
+#pragma unroll kTogether
+  for (int s = 0; s < sums.n; ++s) {
+    const int at = Tile::lane_place(wm0 + (s * WN + wn) * 16);
+    v4f step = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int kk = 0; kk < Tile::BK; kk += 32)
 #pragma unroll
       for (int q = Tile::planes - 1; q >= 0; --q)
-        accb = mfma<T>(v8s{one, one, one, one, one, one, one, one}, Tile::fragment(lds, q, at, kk), accb);
+        step = mfma<T>(v8s{one, one, one, one, one, one, one, one}, Tile::fragment(lds, q, at, kk), step);
+#pragma unroll
+    for (int t = 0; t < sums.n; ++t) sums.acc[t] = t == s ? sums.acc[t] + step[0] : sums.acc[t];
   }
 }
 
@@ -564,14 +573,14 @@ __device__ __forceinline__ void write_results(const GroupArgs& a, const Work<T>&
 
 // ... and what add_bias_sums made of a wave's operands
 template <typename T, int FM, int WN>
-__device__ __forceinline__ void write_bias(const GroupArgs& a, const Work<T>& w, int wm0, int wn, const v4f& accb) {
+__device__ __forceinline__ void write_bias(const GroupArgs& a, const Work<T>& w, int wm0, int wn, const BiasSums<FM, WN>& sums) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = wm0 + i * 16 + (lane & 15);
-    if (i % WN != wn || lane >> 4 != i >> 2 || m >= w.rows_a) continue;
-    if (w.partial) a.partial_bias[(int64_t)w.piece * a.m + w.m0 + m] = accb[i & 3];
-    else ((T*)a.dbias)[(int64_t)w.group * a.m + w.m0 + m] = (T)accb[i & 3];
+  for (int s = 0; s < sums.n; ++s) {
+    const int m = wm0 + (s * WN + wn) * 16 + (lane & 15);
+    if (lane >= 16 || m >= w.rows_a) continue;
+    if (w.partial) a.partial_bias[(int64_t)w.piece * a.m + w.m0 + m] = sums.acc[s];
+    else ((T*)a.dbias)[(int64_t)w.group * a.m + w.m0 + m] = (T)sums.acc[s];
   }
 }
 
@@ -628,7 +637,8 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
 #pragma unroll
     for (int d = 0; d < STAGES; ++d) load(d, d * BK);
   }
-  v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
+  v4f acc[FM][FN];
+  BiasSums<FM, WN> bias_sums{};
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -678,7 +688,9 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
         }
       }
     }
-    if (MODE == kBackWeight && sum_bias) add_bias_sums<O, TileA, FM, WN>(la, wm * (BM / WM), __builtin_amdgcn_readfirstlane(wn), accb);
+    if constexpr (MODE == kBackWeight) {
+      if (sum_bias) add_bias_sums<O, TileA, FM, WN>(la, wm * (BM / WM), __builtin_amdgcn_readfirstlane(wn), bias_sums);
+    }
   };
   int kb = 0;
   if (deep) {
@@ -708,7 +720,7 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
     }
   }
   write_results<T, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc);
-  if (MODE == kBackWeight && sum_bias) write_bias<T, FM, WN>(a, w, wm * (BM / WM), wn, accb);
+  if (MODE == kBackWeight && sum_bias) write_bias<T, FM, WN>(a, w, wm * (BM / WM), wn, bias_sums);
 }
 
 // ------------------------------------------------------------------------------------------------ large tiles of fp32 operands
@@ -803,7 +815,8 @@ __global__ void __launch_bounds__(512, 2) grouped_f32_kernel(GroupArgs a) {
   for (int j = 0; j < FN; ++j) at_b[j] = TileB::lane_place(wn * (BN / WN) + j * 16);
   while (!w.none) {
     const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0;
-    v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
+    v4f acc[FM][FN];
+    BiasSums<FM, WN> bias_sums{};
 #pragma unroll
     for (int i = 0; i < FM; ++i)
 #pragma unroll
@@ -836,10 +849,12 @@ __global__ void __launch_bounds__(512, 2) grouped_f32_kernel(GroupArgs a) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma<__bf16>(fb[j][0], fa[0], acc[i][j]);
       }
-      if (MODE == kBackWeight && sum_bias) add_bias_sums<__bf16, TileA, FM, WN>(la, wm * (BM / WM), wn, accb);
+      if constexpr (MODE == kBackWeight) {
+        if (sum_bias) add_bias_sums<__bf16, TileA, FM, WN>(la, wm * (BM / WM), wn, bias_sums);
+      }
     }
     write_results<float, FM, FN, MODE>(a, w, wm * (BM / WM), wn * (BN / WN), acc);
-    if (MODE == kBackWeight && sum_bias) write_bias<float, FM, WN>(a, w, wm * (BM / WM), wn, accb);
+    if (MODE == kBackWeight && sum_bias) write_bias<float, FM, WN>(a, w, wm * (BM / WM), wn, bias_sums);
     next(w);
   }
 }
@@ -910,10 +925,11 @@ __device__ __forceinline__ void large_products(const GroupArgs& a, Groups& group
   begin(w);
   while (!w.none) {
     const bool sum_bias = MODE == kBackWeight && a.dbias && w.n0 == 0;
-    v4f acc[FM][FN], accb = v4f{0.f, 0.f, 0.f, 0.f};
+    v4f acc[FM][FN];
+    BiasSums<FM, WN> bias_sums{};
 #pragma unroll
     for (int j = 0; j < FN; ++j) {
-      v4f start = accb;
+      v4f start = v4f{0.f, 0.f, 0.f, 0.f};
       if (MODE == kForward && a.bias) start = v4f{(float)bias[j].v[0], (float)bias[j].v[1], (float)bias[j].v[2], (float)bias[j].v[3]};
 #pragma unroll
       for (int i = 0; i < FM; ++i) acc[i][j] = start;
@@ -936,7 +952,9 @@ __device__ __forceinline__ void large_products(const GroupArgs& a, Groups& group
 #pragma unroll
         for (int j = 0; j < FN; ++j) acc[i][j] = mfma<T>(fb[h][j], fa[q & 1], acc[i][j]);
       }
-      if (MODE == kBackWeight && sum_bias) add_bias_sums<T, TileA, FM, WN>(lds, wm0, __builtin_amdgcn_readfirstlane(wave % WN), accb);
+      if constexpr (MODE == kBackWeight) {
+        if (sum_bias) add_bias_sums<T, TileA, FM, WN>(lds, wm0, __builtin_amdgcn_readfirstlane(wave % WN), bias_sums);
+      }
     };
     const int steps = w.depth / BK, rest = w.depth % BK;
     for (int t = 0; t < steps; t += 2) {
@@ -994,7 +1012,7 @@ __device__ __forceinline__ void large_products(const GroupArgs& a, Groups& group
       }
       out += (int64_t)16 * a.n;
     }
-    if (MODE == kBackWeight && sum_bias) write_bias<T, FM, WN>(a, w, wm0, wave % WN, accb);
+    if (MODE == kBackWeight && sum_bias) write_bias<T, FM, WN>(a, w, wm0, wave % WN, bias_sums);
     w = after;
   }
 }
