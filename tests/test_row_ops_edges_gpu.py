@@ -143,3 +143,34 @@ def test_a_bias_gradient_keeps_undefined_values_in_their_channel(hip_backend, dt
             assert torch.equal(gb[:-1], db[:-1]) and torch.equal(gb[-1, keep], db[-1, keep]), (value, c)
             assert torch.equal(gw[:-1], dw[:-1]) and torch.equal(gw[-1, keep], dw[-1, keep]), (value, c)
             assert not bool(torch.isfinite(gb[-1, c])) and not bool(torch.isfinite(gw[-1, c]).any()), (value, c)
+
+
+# ---------------------------------------------------------------------------------------------------------------- operands of few elements
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("few", [1, 2, 3, 5, 7])
+@pytest.mark.parametrize("many", [8, 31, 33, 65, 200, 1030])
+def test_grouped_linear_with_few_channels_on_one_side(hip_backend, many, few, dtype):
+    """Heads of a few outputs, layers of a few inputs: summed axes of several steps, either way."""
+    from test_row_ops_gpu import check_grouped
+    ends = [2, 40, 40, 41, 230]
+    for inner, outer in ((few, many), (many, few)):
+        check_grouped(rnd((233, inner), 1, dtype), rnd((4, outer, inner), 2, dtype, inner ** -0.5), ends, rnd((4, outer), 3, dtype))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=str)
+@pytest.mark.parametrize("few", [4, 7])
+def test_grouped_linear_with_few_channels_and_many_rows(hip_backend, few, dtype):
+    from test_row_ops_gpu import check_grouped
+    ends = [0, 4000, 4001, 4001, 9001]
+    for inner, outer in ((few, 72), (72, few), (few, few)):
+        check_grouped(rnd((9001, inner), 1, dtype), rnd((4, outer, inner), 2, dtype), ends, rnd((4, outer), 3, dtype), rnd((9001, outer), 4, dtype, 0.1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+def test_grouped_linear_of_rows_far_apart(hip_backend, dtype):
+    """Row strides beyond 32-bit offsets in a tile."""
+    from test_row_ops_gpu import check_grouped
+    n, inner, outer, stride = 150, 100, 72, (1 << 22) + 8
+    x = torch.zeros((n - 1) * stride + inner, dtype=dtype, device="cuda").as_strided((n, inner), (stride, 1))
+    x.copy_(rnd((n, inner), 1, dtype))
+    check_grouped(x, rnd((3, outer, inner), 2, dtype, 0.1), [0, 70, 70, 150], rnd((3, outer), 3, dtype))

@@ -38,7 +38,10 @@ SOURCES = {
     # the AdamW step is defined operation by operation (8-bit states: bit-equal to the same operations of torch), so nothing is contracted
     "adamw_kernels.hip": ["-ffp-contract=off", *NO_PACKED_FP32],
     "norm_kernels.hip": [*NO_PACKED_FP32],
-    "grouped_kernels.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", *NO_PACKED_FP32],
+    # No memory clauses: the compiler's pass that forms them (they matter to page faults that are replayed, XNACK on, only) lost track of which
+    # registers hold a loaded piece where that meets elements loaded one by one, and fp32 products of operands with fewer than eight elements one
+    # way came out wrong.  The verifier (2 minutes instead of half of one) refuses such code instead of writing it.
+    "grouped_kernels.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form", *NO_PACKED_FP32, "-mllvm", "-amdgpu-max-memory-clause=1", "-mllvm", "-verify-machineinstrs"],
     "unit.hip": [],
     "pass.hip": [],
     "plan.hip": [],
