@@ -301,8 +301,9 @@ int vc_layer_norm_backward(const void* x, int64_t x_stride, const void* dy, int6
  *   forward          y_r  = weight[g] x_r + bias[g]
  *   backward_input   dx_r = weight[g]^T dy_r
  *   backward_weight  dweight[g] = sum of dy_r x_r^T, dbias[g] = sum of dy_r (dbias NULL: not wanted); zeros for a group without rows
- * Rows of no group come out as zeros and add to no gradient.  All tensors of one dtype; VC_F32 products are accurate to 2^-23 of each product
- * (operands cut exactly into three bf16 pieces; an infinite operand gives NaN).  x_stride, dy_stride: elements from row to row.
+ * Rows of no group come out as zeros and add to no gradient.  All tensors of one dtype.  VC_F32: operands as three bf16 pieces, what is left out of a
+ * product is below 2^-24 of it, sums in fp32 (a sum of one product: within 3 * 2^-24); an operand from 2^128 - 2^119 (3.396e38) on, infinite or not,
+ * gives NaN, and what of one lies below 2^-133 is lost.  x_stride, dy_stride: elements from row to row.
  * Refused: rows from 2^31 on, 2^20 groups, 2^24 channels, 2^24 tiles of results (of 16 x 128 to 192 x 256).
  * direction: 0 forward, 1 backward_input, 2 backward_weight.                                                                                */
 size_t vc_grouped_linear_workspace_bytes(int direction, int64_t rows, int64_t groups, int64_t in, int64_t out, int dtype);

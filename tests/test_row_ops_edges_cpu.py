@@ -47,3 +47,34 @@ def test_overlaps_of_any_two_written_tensors_are_refused(count, order, bits):
             for i, j in ((0, count - 1), (count - 1, 0), (count // 2, 0)):
                 if (a, i) != (b, j):
                     assert refused((a, i), (b, j)), (a, i, b, j)
+
+
+# ---------------------------------------------------------------------------------------------------------------- fp32 operands in three pieces
+def pieces(x):
+    """x = h + m + l as the kernels form them: each rounded to nearest bf16."""
+    h = x.bfloat16().float()
+    m = (x - h).bfloat16().float()
+    return h, m, (x - h - m).bfloat16().float()
+
+
+def test_pieces_are_exact_and_what_is_left_out_of_a_product_is_below_two_to_the_minus_24():
+    # every mantissa: the sizes of the pieces, relative to the value, and that nothing is left
+    x = (torch.arange(1 << 23, dtype=torch.int32) | 127 << 23).view(torch.float32)
+    h, m, low = (t.double() for t in pieces(x))
+    assert torch.equal(h + m + low, x.double())
+    m, low = m.abs() / x.double(), low.abs() / x.double()
+    assert float(m.max()) <= 2.0 ** -8 and float(low.max()) <= 2.0 ** -17
+    # m_x l_y + l_x m_y + l_x l_y over the worst pairs: those among the mantissas with the largest m, the largest l and the largest products of both
+    worst = torch.cat([t.topk(300).indices for t in (m, low, m * low, m + 512 * low)] + [torch.randint(0, 1 << 23, (300,), generator=torch.Generator().manual_seed(0))])
+    a, b = m[worst], low[worst]
+    assert float((a[:, None] * b + b[:, None] * a + b[:, None] * b).max()) <= 2.0 ** -24
+    # 1.03125 - 2^-23 squared, of which pieces that are cut off instead leave out 7.8 * 2^-24
+    cut = lambda t: (t.view(torch.int32) & -65536).view(torch.float32)        # noqa: E731
+    v = torch.tensor([1 + 2.0 ** -7 - 2.0 ** -23])
+    for form, low_, high in ((lambda t: cut(t), 7, 8), (lambda t: t.bfloat16().float(), -1, 1)):
+        h = form(v)
+        m = form(v - h)
+        rest = v - h - m
+        h, m, rest = h.double(), m.double(), rest.double()
+        kept = 2 * rest * h + m * m + 2 * m * h + h * h
+        assert low_ <= float((v.double() ** 2 - kept) / v.double() ** 2 * 2.0 ** 24) <= high

@@ -158,7 +158,7 @@ def test_grouped_linear_with_few_channels_on_one_side(hip_backend, many, few, dt
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16], ids=str)
-@pytest.mark.parametrize("few", [4, 7])
+@pytest.mark.parametrize("few", [1, 4, 7])
 def test_grouped_linear_with_few_channels_and_many_rows(hip_backend, few, dtype):
     from test_row_ops_gpu import check_grouped
     ends = [0, 4000, 4001, 4001, 9001]
@@ -174,3 +174,72 @@ def test_grouped_linear_of_rows_far_apart(hip_backend, dtype):
     x = torch.zeros((n - 1) * stride + inner, dtype=dtype, device="cuda").as_strided((n, inner), (stride, 1))
     x.copy_(rnd((n, inner), 1, dtype))
     check_grouped(x, rnd((3, outer, inner), 2, dtype, 0.1), [0, 70, 70, 150], rnd((3, outer), 3, dtype))
+
+
+# ---------------------------------------------------------------------------------------------------------------- fp32 products
+def one_sided(n, seed):
+    """Mantissas whose 16 low bits are nearly all set behind either piece's border, and random ones."""
+    g = torch.Generator().manual_seed(seed)
+    worst = torch.tensor([1 + 2.0 ** -7 - 2.0 ** -23, 1 + 2.0 ** -8 + 2.0 ** -16 - 2.0 ** -23, 1 + 2.0 ** -7 - 2.0 ** -15 - 2.0 ** -23, 1 + 2.0 ** -8 - 2.0 ** -23,
+                          1 + 2.0 ** -9 - 2.0 ** -17 - 2.0 ** -23, 2 - 2.0 ** -23, 1 + 2.0 ** -8 - 2.0 ** -17 - 2.0 ** -22, 1.0])
+    x = 1 + torch.rand(n, generator=g)
+    x[:worst.numel()] = worst
+    return x * torch.exp2(torch.randint(-6, 7, (n,), generator=g).float()) * (1 - 2 * torch.randint(0, 2, (n,), generator=g).float())
+
+
+@pytest.mark.parametrize("inner,outer,rows", [(1, 200, 64), (8, 40, 30), (100, 200, 500), (136, 264, 700), (520, 392, 2600), (4100, 72, 40)])
+def test_fp32_products_of_one_term(hip_backend, inner, outer, rows):
+    """One product a result (the other operands are zero).  The terms left out stay below u of it.  The six others are added the smallest first; the
+    matrix unit cuts what it adds to a larger product at one step of the result, 2 u, which comes once at the product's size and four times at 2^-7 of
+    it or less: 3 u + 4 * 2 u / 128 at most."""
+    from virconv_amd import ops
+    tol = (3 + 2.0 ** -4) * U
+    # forward and input gradient: one channel of each row is not zero
+    at = torch.arange(rows) % inner
+    x = torch.zeros(rows, inner)
+    x[torch.arange(rows), at] = one_sided(rows, 1)
+    w = one_sided(outer * inner, 2).view(1, outer, inner)
+    out_at = torch.arange(rows) % outer
+    dy = torch.zeros(rows, outer)
+    dy[torch.arange(rows), out_at] = one_sided(rows, 3)
+    xc, wc = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    y = ops.grouped_linear(xc, wc, torch.tensor([0, rows], device="cuda"))
+    dx, = torch.autograd.grad(y, xc, dy.cuda())
+    for got, want in ((y, x.double()[torch.arange(rows), at][:, None] * w.double()[0][:, at].T),
+                      (dx, dy.double()[torch.arange(rows), out_at][:, None] * w.double()[0][out_at])):
+        err = (got.detach().double().cpu() - want).abs() / want.abs()
+        assert float(err.max()) <= tol, float(err.max()) / U
+    # weight gradient: one row of each group is not zero
+    groups = 3
+    ends = [0, rows // 3, rows // 3 + 1, rows]
+    x, dy = torch.zeros(rows, inner), torch.zeros(rows, outer)
+    live = [0, rows // 3, rows - 1]
+    for k, r in enumerate(live):
+        x[r], dy[r] = one_sided(max(inner, 8), 10 + k)[:inner], one_sided(outer, 20 + k)
+    wc = torch.zeros(groups, outer, inner, device="cuda", requires_grad=True)
+    y = ops.grouped_linear(x.cuda(), wc, torch.tensor(ends, device="cuda"))
+    dw, = torch.autograd.grad(y, wc, dy.cuda())
+    want = torch.stack([dy[r].double()[:, None] * x[r].double() for r in live])
+    err = (dw.double().cpu() - want).abs() / want.abs()
+    assert float(err.max()) <= tol, float(err.max()) / U
+
+
+@pytest.mark.parametrize("rows,inner,outer", [(20, 8, 40), (500, 100, 200)])
+def test_fp32_products_at_the_ends_of_the_range(hip_backend, rows, inner, outer):
+    """Operands up to the largest number that rounds to a finite bf16; larger ones, infinities and NaN make their results undefined, and no others."""
+    from virconv_amd import ops
+    offsets = torch.tensor([0, rows], device="cuda")
+    w = one_sided(outer * inner, 2).view(1, outer, inner) * 2.0 ** -20
+    for size in (2.0 ** 128 - 2.0 ** 119 - 2.0 ** 104, -(2.0 ** 128 - 2.0 ** 120), 3e38, 2.0 ** -100):
+        x = torch.zeros(rows, inner)
+        x[:, inner // 2] = size
+        y = ops.grouped_linear(x.cuda(), w.cuda(), offsets)
+        want = x.double() @ w[0].double().T
+        assert float(((y.double().cpu() - want).abs() / want.abs()).max()) <= (3 + 2.0 ** -4) * U, size
+    x = rnd((rows, inner), 1)
+    want = ops.grouped_linear(x, w.cuda(), offsets)
+    for size in (2.0 ** 128 - 2.0 ** 119, torch.finfo(F32).min, math.inf, math.nan):
+        x[3, inner - 1] = size
+        y = ops.grouped_linear(x, w.cuda(), offsets)
+        keep = torch.arange(rows, device="cuda") != 3
+        assert not bool(torch.isfinite(y[3]).any()) and torch.equal(y[keep], want[keep]), size

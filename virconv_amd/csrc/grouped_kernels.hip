@@ -5,8 +5,12 @@
 //   backward weight dW_g = sum_r dy_r x_r^T, db_g = sum_r dy_r     both operands across the summed axis (the group's rows)
 //
 // One output tile per block on v_mfma_f32_16x16x32, fp32 accumulation, one rounding at the end.  The tile's operands go through LDS as
-// 16-bit values: as they are where the tensors are f16 or bf16, and cut exactly into three bf16 pieces where they are fp32 -- six of the
-// nine cross terms are issued, the dropped ones stay below 2^-24 of a product.  An operand that lies along the summed axis is read back
+// 16-bit values: as they are where the tensors are f16 or bf16, and where they are fp32 as three bf16 pieces x = h + m + l, each rounded to nearest,
+// so that |m| <= 2^-8 |x|, |l| <= 2^-17 |x| and nothing is left -- six of the nine cross terms are issued, the dropped ones (m l, l m, l l) stay below
+// 2^-24 of a product.  (Pieces that are cut off instead take as many operations and as long, and drop up to 2^-21, always towards zero.)  A number from
+// 2^128 - 2^119 on rounds to an infinite h, and its products are undefined; a largest finite h in its place is two operations more for two elements
+// and costs 2 to 6 per cent (4096^3: 620 and 665 us).  What lies below 2^-133 of an operand has no bf16 and is lost.  The matrix unit cuts what it
+// adds to a larger product at 2^-23 of that, so a sum of one product is within 3 x 2^-24 of it.  An operand that lies along the summed axis is read back
 // with ds_read_b128, one that lies across it with ds_read_b64_tr_b16 (four rows by sixteen columns a 16-lane group, transposed on the way);
 // the 16-byte (32-byte) pieces of a row are exchanged by a function of the row, so that either read touches every bank once.
 //
@@ -149,11 +153,14 @@ __device__ __forceinline__ void load8(const T* p, int valid, T (&out)[8]) {   //
   }
 }
 
-// the top 16 bits of x as a bf16 (cut, not rounded: x - top is exact and so is what is left of it)
-__device__ __forceinline__ uint32_t top16(float x) { return __float_as_uint(x) & 0xffff0000u; }
-
-__device__ __forceinline__ uint32_t top_halves(float lo, float hi) { return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u); }
-
+// two values as bf16, rounded to nearest; and what the two are
+__device__ __forceinline__ uint32_t nearest2(float lo, float hi) {
+  typedef float v2f __attribute__((ext_vector_type(2)));
+  typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2f{lo, hi}, v2bf));
+}
+__device__ __forceinline__ float low_half(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 // eight elements, as 32-bit words
 template <typename T> struct Words { static constexpr int n = sizeof(T) * 2; uint32_t w[n]; };
 
@@ -195,16 +202,14 @@ __device__ __forceinline__ void stage8(char* lds, int plane_bytes, int at, const
   if constexpr (sizeof(T) == 2) {
     *reinterpret_cast<uint4*>(lds + at) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
   } else {
-    // four operations an element, and a byte exchange that packs two of them for each plane
     uint32_t w[3][4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const float v0 = __uint_as_float(x.w[2 * i]), v1 = __uint_as_float(x.w[2 * i + 1]);
-      const float r0 = v0 - __uint_as_float(top16(v0)), r1 = v1 - __uint_as_float(top16(v1));
-      const float s0 = r0 - __uint_as_float(top16(r0)), s1 = r1 - __uint_as_float(top16(r1));
-      w[0][i] = top_halves(v0, v1);
-      w[1][i] = top_halves(r0, r1);
-      w[2][i] = top_halves(s0, s1);
+      w[0][i] = nearest2(v0, v1);
+      const float r0 = v0 - low_half(w[0][i]), r1 = v1 - high_half(w[0][i]);
+      w[1][i] = nearest2(r0, r1);
+      w[2][i] = nearest2(r0 - low_half(w[1][i]), r1 - high_half(w[1][i]));
     }
 #pragma unroll
     for (int q = 0; q < 3; ++q) *reinterpret_cast<uint4*>(lds + q * plane_bytes + at) = make_uint4(w[q][0], w[q][1], w[q][2], w[q][3]);

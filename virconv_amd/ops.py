@@ -632,7 +632,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor, bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A linear layer per row group: y_r = weight[g] @ x_r + bias[g] for the rows r in [offsets[g], offsets[g + 1]).
 
-    x: (N, in) rows sorted by group, in float32 (products accurate to fp32), float16 or bfloat16, on the GPU; rows may be strided.
+    x: (N, in) rows sorted by group, in float32 (what a product leaves out is below 2^-24 of it; operands from 3.396e38 on count as infinite,
+    and those give NaN), float16 or bfloat16, on the GPU; rows may be strided.
     weight: (G, out, in), bias: (G, out) or None, in x's type.  offsets: (G + 1,) int32 or int64 on the GPU, rising within [0, N]: they are
     never read on the host, so what a router counted needs no synchronisation.  A group may have no rows; rows of no group (before
     offsets[0], from offsets[G] on) give zeros and zero gradients.  First-order gradients; capture as for ``layer_norm``.  -> (N, out)"""
