@@ -78,3 +78,74 @@ def test_pieces_are_exact_and_what_is_left_out_of_a_product_is_below_two_to_the_
         h, m, rest = h.double(), m.double(), rest.double()
         kept = 2 * rest * h + m * m + 2 * m * h + h * h
         assert low_ <= float((v.double() ** 2 - kept) / v.double() ** 2 * 2.0 ** 24) <= high
+
+
+# ---------------------------------------------------------------------------------------------------------------- AdamW's checkpoints
+@pytest.fixture
+def AdamW(hip, monkeypatch):
+    """The optimizer with its host code alone: parameters on the CPU, no step."""
+    from virconv_amd import optim
+    monkeypatch.setattr(optim.AdamW, "_check_group", lambda self, g: None)
+    return optim.AdamW
+
+
+def moments(opt, p, seed):
+    """Random 8-bit moments, over a few binades, some zero, one undefined."""
+    g = torch.Generator().manual_seed(seed)
+    st = opt._new_state(p)
+    n, blocks = p.numel(), -(-p.numel() // 128)
+    for k in ("exp_avg", "exp_avg_rms"):
+        v = torch.randn(n, generator=g) * torch.exp(2 * torch.randn(n, generator=g))
+        v = (v.abs() if k == "exp_avg_rms" else v).clamp(-250, 250) * (torch.rand(n, generator=g) > 0.1)
+        v[0] = float("nan")
+        torch.as_strided(st[k].view(torch.uint8), (n,), (1,)).copy_(v.to(torch.float8_e4m3fn).view(torch.uint8))
+    st["exponents"].copy_(torch.randint(-20, 3, (blocks, 2), generator=g))
+    st["step"] = 7
+    return st
+
+
+@pytest.mark.parametrize("shape", [(8, 16, 3, 3), (5, 7, 2, 3), (130, 3, 1, 2)], ids=str)
+@pytest.mark.parametrize("back", [False, True])
+def test_8_bit_moments_survive_a_change_of_memory_order(AdamW, shape, back):
+    g = torch.Generator().manual_seed(1)
+    p = torch.nn.Parameter(torch.randn(shape, generator=g))
+    q = torch.nn.Parameter(p.detach().to(memory_format=torch.channels_last))
+    p, q = (q, p) if back else (p, q)
+    one, two = AdamW([p], state_bits=8), AdamW([q], state_bits=8)
+    moments(one, p, 2)
+    two.load_state_dict(one.state_dict())
+    want, got = one.decoded_state(p), two.decoded_state(q)
+    assert two.state[q]["step"] == 7 and all(t.stride() == q.stride() for t in got)
+    st = two.state[q]
+    for k, column, (a, b) in (("exp_avg", 0, (want[0], got[0])), ("exp_avg_rms", 1, (want[1].sqrt(), got[1].sqrt()))):
+        unit = torch.empty_like(q, dtype=torch.float64)
+        torch.as_strided(unit, (q.numel(),), (1,)).copy_((2.0 ** (st["exponents"][:, column].double() - 7)).repeat_interleave(128, 0)[:q.numel()])
+        nan = torch.isnan(a)
+        assert torch.equal(torch.isnan(b), nan) and int(nan.sum()) == 1
+        # to the nearest e4m3 value: 2^-4 of it, or half of the smallest ones' distance 2^-9; a root up to all of that (and the squares' own rounding)
+        bound = torch.maximum((2.0 ** -4 + 1e-6) * a.double().abs(), unit * 2.0 ** (-10 if column == 0 else -9))
+        assert bool(((a.double() - b.double()).abs() <= bound)[~nan].all())
+        assert bool((b[~nan & (a != 0)] != 0).all()) or column == 0
+
+
+@pytest.mark.parametrize("like", ["equal", "axes of one element"])
+def test_8_bit_moments_of_the_same_memory_order_stay_bit_for_bit(AdamW, like):
+    shape = (40, 1, 5, 6) if like != "equal" else (8, 16, 3, 3)
+    p = torch.nn.Parameter(torch.randn(shape))
+    q = torch.nn.Parameter(torch.empty_strided(shape, (30, 1, 6, 1)).copy_(p.detach()) if like != "equal" else p.detach().clone())
+    one, two = AdamW([p], state_bits=8), AdamW([q], state_bits=8)
+    a = moments(one, p, 3)
+    two.load_state_dict(one.state_dict())
+    b = two.state[q]
+    assert torch.equal(a["exponents"], b["exponents"])
+    assert all(torch.equal(a[k].view(torch.uint8), b[k].view(torch.uint8)) for k in ("exp_avg", "exp_avg_rms"))
+
+
+def test_a_moment_whose_blocks_are_not_known_is_refused(AdamW):
+    p = torch.nn.Parameter(torch.randn(16, 24))
+    opt = AdamW([p], state_bits=8)
+    moments(opt, p, 4)
+    saved = opt.state_dict()
+    saved["state"][0]["exp_avg"] = torch.zeros(16, 48, dtype=torch.uint8)[:, ::2].view(torch.float8_e4m3fn)
+    with pytest.raises(ValueError, match="not dense"):
+        AdamW([p], state_bits=8).load_state_dict(saved)

@@ -133,6 +133,20 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _order(t: torch.Tensor):
+    """What tells the order of t's elements in memory: the strides of its axes, those of one element apart."""
+    return [s for s, n in zip(t.stride(), t.shape) if n != 1]
+
+
+def _decode(codes: torch.Tensor, exponents: torch.Tensor) -> torch.Tensor:
+    """The values of an 8-bit moment, fp32, of its shape and order in memory."""
+    n = codes.numel()
+    scale = torch.exp2(exponents.float() - 7).repeat_interleave(STATE_BLOCK, 0)[:n]
+    out = torch.empty_like(codes, dtype=torch.float32, memory_format=torch.preserve_format)
+    torch.as_strided(out, (n,), (1,)).copy_(torch.as_strided(codes.view(torch.uint8), (n,), (1,)).view(torch.float8_e4m3fn).float() * scale)
+    return out
+
+
 class AdamW(torch.optim.Optimizer):
     """AdamW (torch.optim.AdamW's arithmetic: true weight decay, bias correction) over all parameters of a group in a few launches.
 
@@ -142,7 +156,9 @@ class AdamW(torch.optim.Optimizer):
     square root of the second moment) are float8_e4m3fn values over a power of two for every 128 elements (``exponents``, int8), rounded up or
     down at random in proportion so that a moment follows changes smaller than its resolution.  The random numbers follow from ``seed``, the
     step and the element's place: a run repeats, and resumes from a checkpoint, bit for bit.  ``decoded_state(p)`` gives the moments as
-    fp32 tensors.  A step counts on the host, so it cannot be captured into a graph."""
+    fp32 tensors.  The 128 elements of an exponent are neighbours in memory, so a checkpoint has to keep its tensors' strides (torch.save does);
+    loaded into a parameter of another order of its axes the moments are rounded once more, to the nearest.  A step counts on the host, so it
+    cannot be captured into a graph."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.99), eps=1e-8, weight_decay=0.01, state_bits=32, seed=0):
         if state_bits not in (8, 32):
@@ -222,28 +238,45 @@ class AdamW(torch.optim.Optimizer):
             st = self.state[p]
             for k, v in saved[i].items():
                 if k != "step" and torch.is_tensor(v):
-                    t = torch.empty_strided(p.shape, p.stride(), dtype=v.dtype, device=p.device) if v.shape == p.shape else \
-                        torch.empty(v.shape, dtype=v.dtype, device=p.device)
+                    like = k != "exponents" and v.shape == p.shape
+                    t = torch.empty_strided(p.shape, p.stride(), dtype=v.dtype, device=p.device) if like else torch.empty(v.shape, dtype=v.dtype, device=p.device)
                     st[k] = t.copy_(v)
+            if self.state_bits == 8 and "exponents" in st:
+                for column, k in enumerate(("exp_avg", "exp_avg_rms")):
+                    v = saved[i][k]
+                    if v.dtype == st[k].dtype and v.shape == p.shape and _order(v) != _order(p):
+                        # its elements lie in another order in memory than p's, so other ones share an exponent now
+                        if not _dense(v):
+                            raise ValueError(f"AdamW: state {k!r} of strides {v.stride()} is not dense: which of its elements share an exponent is not known")
+                        self._encode(p, st, column, k, _decode(v.to(p.device), saved[i]["exponents"].to(p.device)[:, column]))
             if self.state_bits == 32 and "exp_avg" in st:
                 for k in ("exp_avg", "exp_avg_sq"):
                     st[k] = st[k].float()
             st["step"] = int(saved[i]["step"])
             self._check_state(p, st)
 
+    @staticmethod
+    def _encode(p, st, column, k, values):
+        """`values` (fp32, p's shape) as the 8-bit moment k of p, to the nearest; a root that is not zero does not become zero (it divides)."""
+        n = p.numel()
+        flat = torch.as_strided(torch.empty_strided(p.shape, p.stride(), dtype=torch.float32, device=p.device).copy_(values), (n,), (1,))
+        blocks = torch.nn.functional.pad(flat, (0, -n % STATE_BLOCK)).view(-1, STATE_BLOCK)
+        top = torch.where(blocks.isfinite(), blocks.abs(), 0).amax(1)
+        exponents = ((top.view(torch.int32) >> 23) - 127).clamp(min=-119)
+        scaled = (blocks * torch.exp2(7.0 - exponents.float())[:, None])
+        if column == 1:
+            scaled = torch.where((scaled > 0) & (scaled < 2.0 ** -9), 2.0 ** -9, scaled)
+        codes = scaled.to(torch.float8_e4m3fn).view(torch.uint8).reshape(-1)[:n]
+        torch.as_strided(st[k].view(torch.uint8), (n,), (1,)).copy_(codes)
+        st["exponents"][:, column] = exponents
+
     def decoded_state(self, p):
         """The two moments of parameter p as fp32 tensors of its shape: (exp_avg, exp_avg_sq)."""
         st = self.state[p]
         if self.state_bits == 32:
             return st["exp_avg"].clone(), st["exp_avg_sq"].clone()
-        n = p.numel()
-        scale = torch.exp2(st["exponents"].float() - 7).repeat_interleave(STATE_BLOCK, 0)[:n]
-        out = []
-        for k, name in enumerate(("exp_avg", "exp_avg_rms")):
-            flat = torch.as_strided(st[name].view(torch.uint8), (n,), (1,)).view(torch.float8_e4m3fn).float() * scale[:, k]
-            out.append(torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format))
-            torch.as_strided(out[-1], (n,), (1,)).copy_(flat)
-        return out[0], out[1] * out[1]
+        m, r = (_decode(st[k], st["exponents"][:, column]) for column, k in enumerate(("exp_avg", "exp_avg_rms")))
+        return m, r * r
 
     def step(self, closure=None):
         loss = None
