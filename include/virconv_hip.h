@@ -322,8 +322,9 @@ int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const voi
  * dtype: of the parameters and gradients.  state_bits 32: exp_avg = m and exp_avg_sq = v are fp32.  state_bits 8: exp_avg = m and
  * exp_avg_sq = sqrt(v) are OCP e4m3 values over a power of two for every 128 elements: value * 2^(exponent - 7), exponents: (blocks, 2) int8
  * [of m, of sqrt(v)], blocks = ceil(n / 128).  A value is rounded to one of its two e4m3 neighbours with the probability of its distance
- * from the other: 16 bits of M(M(M(M(seed) + step) + key) ^ element), M the finalizer of MurmurHash3; the low half for m.  All-zero codes
- * and exponents are the state before step 1.  Descriptors with n = 0 are skipped.  Written memory must not overlap (checked).             */
+ * from the other: 16 bits of M(M(M(M(seed) + step) + key) ^ element), M the finalizer of MurmurHash3; the low half for m.  An infinite or
+ * undefined one is NaN; where v is infinite and m is not, the parameter only decays.  All-zero codes and exponents are the state before step
+ * 1.  Descriptors with n = 0 are skipped.  Written memory must not overlap (checked).                                                      */
 typedef struct vc_adamw_tensor {
   void* param;         /* n elements of dtype, updated in place */
   const void* grad;    /* n elements of dtype */

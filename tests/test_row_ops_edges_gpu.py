@@ -243,3 +243,31 @@ def test_fp32_products_at_the_ends_of_the_range(hip_backend, rows, inner, outer)
         y = ops.grouped_linear(x, w.cuda(), offsets)
         keep = torch.arange(rows, device="cuda") != 3
         assert not bool(torch.isfinite(y[3]).any()) and torch.equal(y[keep], want[keep]), size
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=str)
+@pytest.mark.parametrize("value", [2e19, 1e25, -3e38])
+def test_adamw_8_bit_with_a_square_beyond_fp32(hip_backend, value, dtype):
+    """A finite gradient whose square overflows: v is infinite, m / sqrt(v) is 0, and the parameter only decays, as with 32-bit moments."""
+    from virconv_amd.optim import AdamW
+    wide, narrow, clean = (torch.nn.Parameter(rnd((300,), 1, dtype)) for _ in range(3))
+    opts = AdamW([wide], **HYPER), AdamW([narrow], state_bits=8, **HYPER), AdamW([clean], state_bits=8, **HYPER)
+    at = torch.tensor([3, 130, 299], device="cuda")
+    rest = torch.ones(300, dtype=torch.bool, device="cuda")
+    rest[at] = False
+    for t in range(4):
+        for p in (wide, narrow, clean):
+            p.grad = rnd((300,), 10 + t, dtype)
+            if t == 1 and p is not clean:
+                p.grad[at] = value
+        for o in opts:
+            o.step()
+        assert bool(torch.isfinite(narrow).all()) and bool(torch.isfinite(wide).all()), t
+        if t >= 1:
+            before = wide_before.float(), narrow_before.float()
+            for p, b in zip((wide, narrow), before):
+                want = b[at].double() * (1 - HYPER["lr"] * HYPER["weight_decay"])
+                assert bool(((p[at].double() - want).abs() <= half_step(dtype) * want.abs() + 3 * U * want.abs() + floor_step(dtype)).all()), t
+        wide_before, narrow_before = wide.detach().clone(), narrow.detach().clone()
+    # the neighbours: their blocks' exponent of m may differ, by 8-bit roundings then, so steps of lr at most
+    assert float((narrow[rest].float() - clean[rest].float()).abs().max()) <= 3 * 4 * HYPER["lr"] + 4 * half_step(dtype) * float(clean.abs().max())

@@ -14,7 +14,9 @@
 // steps (6 to 12 per cent of a value) are far wider than what one step changes of a moment (1 - b2 = 1 per cent of v), so rounding to the
 // nearest value would leave a moment where it is for good; it is rounded up with the probability of its distance from the lower
 // neighbour instead, which keeps every moment's mean.  The random numbers are a function of (seed, step, tensor, element), so a run can be
-// repeated, and resumed, bit for bit.  An infinite or undefined moment is held as NaN and has no part in its block's exponent.
+// repeated, and resumed, bit for bit.  An infinite or undefined moment is held as NaN and has no part in its block's exponent.  A NaN in place of
+// r beside a number in place of m is a square beyond fp32 (a gradient from 1.8e19 on, not an undefined one): it counts as infinite, m / r as 0, and
+// the parameter only decays from then on, as it does with 32-bit moments.
 #include "common.h"
 
 #include <math.h>
@@ -214,15 +216,19 @@ __global__ void __launch_bounds__(256) adamw8_kernel(AdamwTable8 B, AdamwArgs a)
     mtop = max(mtop, __float_as_uint(m[k]) & 0x7fffffffu);
     vtop = max(vtop, __float_as_uint(v));
   }
-  store8((T*)S.param, i, n, vec, p);
   if (max(mtop, vtop) >= 0x7f800000u) {   // something infinite or undefined: it has no part in the block's exponents
     mtop = vtop = 0;
+    float before[8];
+    load8((const T*)S.param, i, n, vec, before);
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
+      // r = sqrt(v) is not a number then, infinite or not; m is where the gradient was
+      if ((__float_as_uint(m[k]) & 0x7fffffffu) < 0x7f800000u && (__float_as_uint(r[k]) & 0x7fffffffu) >= 0x7f800000u) p[k] = before[k] * a.keep;
       mtop = max(mtop, finite_bits(__float_as_uint(m[k]) & 0x7fffffffu));
       vtop = max(vtop, finite_bits(__float_as_uint(r[k] * r[k])));
     }
   }
+  store8((T*)S.param, i, n, vec, p);
   // the root's exponent is half of v's, whatever the root's last bit
   mtop = max16(mtop);
   vtop = max16(vtop);
