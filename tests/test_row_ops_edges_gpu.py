@@ -271,3 +271,25 @@ def test_adamw_8_bit_with_a_square_beyond_fp32(hip_backend, value, dtype):
         wide_before, narrow_before = wide.detach().clone(), narrow.detach().clone()
     # the neighbours: their blocks' exponent of m may differ, by 8-bit roundings then, so steps of lr at most
     assert float((narrow[rest].float() - clean[rest].float()).abs().max()) <= 3 * 4 * HYPER["lr"] + 4 * half_step(dtype) * float(clean.abs().max())
+
+
+def test_adamw_8_bit_second_moment_settles_where_it_is_said_to(hip_backend):
+    """Gaussian gradients of one size for many steps.  A rounding of r to its grid, s apart, adds s |d| to the mean of r^2 where a step changes r by
+    d, far less than s: E |d| = (1 - beta2) r E|g^2 / v - 1| / 2 = 0.484 (1 - beta2) r, and what a step adds stays for 1 / (1 - beta2) steps, so v
+    settles 0.484 s / r above its mean in 32 bits, s / r between 1/16 and 1/8."""
+    from virconv_amd.optim import AdamW
+    n, beta2 = 1 << 16, 0.99
+    narrow, wide = (torch.nn.Parameter(torch.zeros(n, device="cuda")) for _ in range(2))
+    opts = [AdamW([p], lr=0.0, betas=(0.9, beta2), state_bits=b) for p, b in ((narrow, 8), (wide, 32))]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    ratio = []
+    for t in range(900):
+        narrow.grad = torch.randn(n, device="cuda", generator=g)
+        wide.grad = narrow.grad
+        for o in opts:
+            o.step()
+        if t >= 800:
+            ratio.append(float(opts[0].decoded_state(narrow)[1].double().mean() / opts[1].decoded_state(wide)[1].double().mean()))
+    excess = sum(ratio) / len(ratio) - 1
+    # the estimate's own error: v of one element spreads by sqrt((1 - beta2)) = 10 per cent, of 65536 by 0.04; second-order terms below a tenth of it
+    assert 0.484 / 16 * 0.9 - 0.002 < excess < 0.484 / 8 * 1.1 + 0.002, excess
