@@ -149,3 +149,27 @@ def test_a_moment_whose_blocks_are_not_known_is_refused(AdamW):
     saved["state"][0]["exp_avg"] = torch.zeros(16, 48, dtype=torch.uint8)[:, ::2].view(torch.float8_e4m3fn)
     with pytest.raises(ValueError, match="not dense"):
         AdamW([p], state_bits=8).load_state_dict(saved)
+
+
+# ---------------------------------------------------------------------------------------------------------------- the native host side
+@pytest.mark.parametrize("what", ["missing", "of another layout", "of another torch", "no extension"])
+def test_what_does_not_use_the_native_host_side_does_without_it(what, monkeypatch, tmp_path):
+    from virconv_amd.backend_hip import HipBackend
+    monkeypatch.setattr(_lib, "_host", None)
+    if what == "missing":
+        monkeypatch.setattr(_lib, "HOST_PATH", str(tmp_path / "_host_ops.so"))
+    elif what == "no extension":
+        (tmp_path / "_host_ops.so").write_bytes(b"no shared object")
+        monkeypatch.setattr(_lib, "HOST_PATH", str(tmp_path / "_host_ops.so"))
+    elif what == "of another torch":
+        monkeypatch.setattr(torch, "__version__", "0.0")
+    else:
+        monkeypatch.setattr(_lib, "ABI_VERSION", _lib.ABI_VERSION + 1)
+    with ops.use_backend(HipBackend()) as be:     # everything that goes through the C ABI alone
+        assert be.lib.vc_abi_version() > 0
+        with pytest.raises(_lib.VirConvError, match="python -m virconv_amd.build"):
+            ops.layer_norm(torch.zeros(2, 4))
+        with pytest.raises(_lib.VirConvError, match="python -m virconv_amd.build"):
+            be.host
+    monkeypatch.undo()
+    assert _lib.load_host().ABI_VERSION == _lib.ABI_VERSION

@@ -268,14 +268,22 @@ def load_host():
     global _host
     if _host is not None:
         return _host
+    import torch
     lib = load()
+    again = "rebuild it with `python -m virconv_amd.build`"
     if not os.path.exists(HOST_PATH):
-        raise VirConvError(f"{HOST_PATH} is missing: build it with `python -m virconv_amd.build`")
+        raise VirConvError(f"{HOST_PATH} is missing: {again}")
     from importlib.machinery import ExtensionFileLoader
     from importlib.util import module_from_spec, spec_from_file_location
     spec = spec_from_file_location("_host_ops", HOST_PATH, loader=ExtensionFileLoader("_host_ops", HOST_PATH))
-    host = module_from_spec(spec)
-    spec.loader.exec_module(host)
+    try:
+        host = module_from_spec(spec)
+        spec.loader.exec_module(host)
+    except ImportError as e:
+        raise VirConvError(f"{HOST_PATH} cannot be loaded beside torch {torch.__version__}: {e}; {again}") from e
+    built = getattr(host, "ABI_VERSION", None), getattr(host, "TORCH_VERSION", None)
+    if built != (ABI_VERSION, torch.__version__):
+        raise VirConvError(f"{HOST_PATH} was built for struct layout version {built[0]} and torch {built[1]}, here are {ABI_VERSION} and {torch.__version__}: {again}")
     names = [n for n in SIGNATURES if n.startswith(("vc_layer_norm_", "vc_grouped_linear_"))] + ["vc_adamw", "vc_last_error"]
     host.bind({n: C.cast(getattr(lib, n), _P).value for n in names}, VirConvError)
     _host = host

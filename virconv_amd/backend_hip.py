@@ -16,6 +16,7 @@ from ._lib import CONV_SORTED_ROWS, OPERAND_TYPES, check, i32arr, f32arr
 
 
 import ctypes
+import functools
 import os
 
 # weight gradient of a conv+BN+ReLU unit on a side stream underneath its backward-input conv (fork / join inside the C call)
@@ -52,9 +53,14 @@ def conv_out_shape(in_shape, ksize, stride, padding, dilation):
 class HipBackend:
     name = "hip"
 
+    @functools.cached_property
+    def host(self):
+        """The native host side of layer norm, grouped products and AdamW (csrc/host_ops.cpp), loaded when the first of them is used: nothing else
+        needs it, nor a compiler and headers that fit the installed torch."""
+        return _lib.load_host()
+
     def __init__(self):
         self.lib = _lib.load()
-        self.host = _lib.load_host()   # layer norm, grouped products, AdamW: the native host side (csrc/host_ops.cpp)
         self._pinned = None
         self._pin_ev = None
         self._trace_cap, self._trace_pairs = 0, None

@@ -70,9 +70,9 @@ def build(force: bool = False, verbose: bool = True) -> str:
     # A/B builds (developer only): VIRCONV_LIB_OUT=<path> VIRCONV_HIPCC_EXTRA="-DVC_V2_SCHED=0" python -m virconv_amd.build
     # writes a second library that tools/kbench.py can load through VIRCONV_LIB=<path>
     out, extra_env = os.environ.get("VIRCONV_LIB_OUT"), os.environ.get("VIRCONV_HIPCC_EXTRA", "").split()
+    build_host(force, verbose)      # (it is bound to whatever library is loaded, one of VIRCONV_LIB_OUT too)
     if out:
         return _build_to(out, os.path.join(HERE, "build_ab"), extra_env, verbose)
-    build_host(force, verbose)
     if not force and not _stale():
         return LIB
     return _build_to(LIB, os.path.join(HERE, "build"), extra_env, verbose, force_all=force)
@@ -85,7 +85,7 @@ def build_host(force: bool = False, verbose: bool = True) -> str:
     src, header = os.path.join(CSRC, "host_ops.cpp"), os.path.join(HERE, "..", "include", "virconv_hip.h")
     root = os.path.dirname(torch.__file__)
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           "-DTORCH_EXTENSION_NAME=_host_ops", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-DTORCH_EXTENSION_NAME=_host_ops", f'-DVC_TORCH_VERSION="{torch.__version__}"', f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-isystem{d}" for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"),
                                       os.path.join(os.path.dirname(os.path.dirname(os.path.realpath(_hipcc()))), "include"),
                                       sysconfig.get_paths()["include"])),

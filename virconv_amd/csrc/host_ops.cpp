@@ -436,6 +436,8 @@ PYBIND11_MODULE(_host_ops, m) {
       PyErr_SetString(error_class ? error_class : PyExc_RuntimeError, e.what());
     }
   });
+  m.attr("ABI_VERSION") = VC_ABI_VERSION;       // of the structs that are filled here
+  m.attr("TORCH_VERSION") = VC_TORCH_VERSION;   // whose headers this was built against
   m.def("bind", &bind);
   m.def("layer_norm", &layer_norm, py::call_guard<py::gil_scoped_release>());
   m.def("grouped_linear", &grouped_linear, py::call_guard<py::gil_scoped_release>());
