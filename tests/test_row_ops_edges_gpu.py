@@ -293,3 +293,45 @@ def test_adamw_8_bit_second_moment_settles_where_it_is_said_to(hip_backend):
     excess = sum(ratio) / len(ratio) - 1
     # the estimate's own error: v of one element spreads by sqrt((1 - beta2)) = 10 per cent, of 65536 by 0.04; second-order terms below a tenth of it
     assert 0.484 / 16 * 0.9 - 0.002 < excess < 0.484 / 8 * 1.1 + 0.002, excess
+
+
+# ---------------------------------------------------------------------------------------------------------------- graphs, refusals
+@pytest.mark.parametrize("what", ["rows of three axes", "a transposed weight", "a layer in between"])
+def test_a_captured_backward_beside_an_eager_graph_is_refused_through_nodes_in_between(hip_backend, what):
+    from virconv_amd import ops
+    x, dy = rnd((30, 10, 64), 1).requires_grad_(), rnd((30, 10, 64), 3)
+    w = rnd((2, 64, 64), 2).requires_grad_()
+    scale = rnd((64,), 4).requires_grad_()
+    offsets = torch.tensor([0, 100, 300], device="cuda")
+
+    def forward():
+        if what == "rows of three axes":
+            return ops.layer_norm(x, scale.detach())
+        if what == "a transposed weight":
+            return ops.grouped_linear(x.detach().view(300, 64), w.transpose(1, 2), offsets).view(30, 10, 64)
+        return ops.layer_norm(torch.tanh(x * 2.0), scale.detach())
+
+    leaves = {"rows of three axes": (x,), "a transposed weight": (w,), "a layer in between": (x,)}[what]
+
+    def run():
+        y = forward()
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    want = [t.clone() for t in run()]
+    alive = forward()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="let go of that result"):
+        with torch.cuda.graph(graph):
+            run()
+    del alive, graph
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for _ in range(3):
+        for t in out:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))

@@ -13,6 +13,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <unordered_map>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/virconv_hip.h"
@@ -112,25 +113,34 @@ bool capturing(hipStream_t stream) {     // (the legacy stream never is, and mus
 }
 
 // A backward pass under capture whose gradients go to nodes recorded before it on a stream that is not captured (a leaf's, while an eager graph of
-// that leaf lives): the engine would make that stream wait for the captured one, which ends the process.  Said here instead.
+// that leaf lives): the engine would make that stream wait for the captured one, which ends the process.  Said here instead, also where nodes of the
+// capture lie in between (a view of the rows, a copy of a strided weight, layers in front of this one): all that this pass leads to is walked.
 void refuse_uncaptured_consumers(const char* who, const Tensor& x) {
   const c10::hip::HIPStream here = c10::hip::getCurrentHIPStream(x.get_device());
   if (!capturing(here.stream())) return;
   const auto node = torch::autograd::get_current_node();
   const auto* tasks = torch::autograd::get_current_graph_task_exec_info();
   if (!node) return;
-  for (const auto& edge : node->next_edges()) {
-    if (!edge.function) continue;
-    if (tasks && !tasks->empty()) {
-      const auto it = tasks->find(edge.function.get());
-      if (it == tasks->end() || !it->second.should_execute()) continue;
+  std::vector<torch::autograd::Node*> stack{node.get()};
+  std::unordered_set<torch::autograd::Node*> seen{node.get()};
+  while (!stack.empty()) {
+    torch::autograd::Node* const from = stack.back();
+    stack.pop_back();
+    for (const auto& edge : from->next_edges()) {
+      torch::autograd::Node* const to = edge.function.get();
+      if (!to || !seen.insert(to).second) continue;
+      if (tasks && !tasks->empty()) {
+        const auto it = tasks->find(to);
+        if (it == tasks->end() || !it->second.should_execute()) continue;
+      }
+      stack.push_back(to);
+      const auto there = to->stream();
+      if (!there || there->id() == here.id() || there->device_index() != here.device_index()) continue;
+      const c10::Stream plain(c10::Stream::UNSAFE, c10::Device(here.unwrap().device_type(), here.device_index()), there->id());
+      if (!capturing(c10::hip::HIPStream(plain).stream()))
+        throw VirConvError(std::string(who) + ": this backward pass is being captured, and a graph recorded before it, on a stream that is not, holds a node "
+                           "its gradients go to (an eager result of the same leaf that is still alive): let go of that result before the capture");
     }
-    const auto there = edge.function->stream();
-    if (!there || there->id() == here.id() || there->device_index() != here.device_index()) continue;
-    const c10::Stream plain(c10::Stream::UNSAFE, c10::Device(here.unwrap().device_type(), here.device_index()), there->id());
-    if (!capturing(c10::hip::HIPStream(plain).stream()))
-      throw VirConvError(std::string(who) + ": this backward pass is being captured, and a graph recorded before it, on a stream that is not, holds a node "
-                         "its gradients go to (an eager result of the same leaf that is still alive): let go of that result before the capture");
   }
 }
 
