@@ -173,3 +173,22 @@ def test_what_does_not_use_the_native_host_side_does_without_it(what, monkeypatc
             be.host
     monkeypatch.undo()
     assert _lib.load_host().ABI_VERSION == _lib.ABI_VERSION
+
+
+# ---------------------------------------------------------------------------------------------------------------- derivatives
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_forward_mode_derivatives_are_refused(hip, which):
+    """(They are refused before a tensor's device is looked at.)"""
+    from torch.autograd import forward_ad
+    norm = [torch.randn(4, 8), torch.randn(8), torch.randn(8)]
+    grouped = [torch.randn(4, 8), torch.randn(2, 5, 8), torch.randn(2, 5)]
+    offsets = torch.tensor([0, 1, 4])
+    with forward_ad.dual_level():
+        for args in (norm, grouped):
+            args[which] = forward_ad.make_dual(args[which], torch.ones_like(args[which]))
+        with pytest.raises(NotImplementedError, match="layer_norm: no forward-mode"):
+            ops.layer_norm(*norm)
+        with pytest.raises(NotImplementedError, match="grouped_linear: no forward-mode"):
+            ops.grouped_linear(grouped[0], grouped[1], offsets, grouped[2])
+    with pytest.raises(_lib.VirConvError, match="no CPU path"):
+        ops.layer_norm(torch.randn(4, 8))

@@ -107,6 +107,12 @@ bool wants_grad(std::initializer_list<Tensor> ts) {
   return false;
 }
 
+// Forward-mode derivatives: there are none here, and the passes below would drop a tangent without a word.
+void refuse_tangents(const char* who, std::initializer_list<Tensor> ts) {
+  for (const Tensor& t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(0).defined(), who, ": no forward-mode derivatives");
+}
+
 bool capturing(hipStream_t stream) {     // (the legacy stream never is, and must not be asked while another one is)
   hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
   return stream && hipStreamIsCapturing(stream, &status) == hipSuccess && status == hipStreamCaptureStatusActive;
@@ -230,6 +236,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& weight, const OptTensor& bia
                       x.scalar_type(), " rows it has to be of that type or float32");
   }
   TORCH_CHECK_VALUE(eps >= 0.0, "layer_norm: eps = ", eps);
+  refuse_tangents("layer_norm", {x, w, b});
   dtype_of(x, "layer_norm: x");
   need_gpu(x, "layer_norm: x");
   for (const auto& [t, name] : {std::pair<Tensor&, const char*>{w, "layer_norm: weight"}, {b, "layer_norm: bias"}})
@@ -315,6 +322,7 @@ Tensor grouped_linear(const Tensor& x, const Tensor& weight, const Tensor& offse
                     "grouped_linear: offsets have to be ", weight.size(0) + 1, " int32 or int64 values, got ", offsets.sizes(), " ", offsets.scalar_type());
   TORCH_CHECK_VALUE(!b0.defined() || (b0.dim() == 2 && b0.size(0) == weight.size(0) && b0.size(1) == weight.size(1)), "grouped_linear: bias has shape ",
                     b0.defined() ? b0.sizes() : x.sizes(), ", expected [", weight.size(0), ", ", weight.size(1), "]");
+  refuse_tangents("grouped_linear", {x, weight, b0});
   dtype_of(x, "grouped_linear: x");
   need_gpu(x, "grouped_linear: x");
   same_device(weight, x, "grouped_linear: weight");

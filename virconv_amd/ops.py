@@ -624,7 +624,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
     x: (..., C) in float32, float16 or bfloat16 on the GPU; the result has its shape and type and is dense.  Rows may be strided (a column
     slice of a wider matrix is not copied).  weight, bias: (C,) in x's type or float32, or None; their gradients have their own types and a
-    fixed order of additions.  First-order gradients.  Both directions can be captured into a graph; the backward pass is refused there
+    fixed order of additions.  First-order gradients in reverse mode.  Both directions can be captured into a graph; the backward pass is refused there
     while an eager result of the same leaves is alive."""
     return get_backend().host.layer_norm(x, weight, bias, eps)
 
@@ -636,7 +636,7 @@ def grouped_linear(x: torch.Tensor, weight: torch.Tensor, offsets: torch.Tensor,
     and those give NaN), float16 or bfloat16, on the GPU; rows may be strided.
     weight: (G, out, in), bias: (G, out) or None, in x's type.  offsets: (G + 1,) int32 or int64 on the GPU, rising within [0, N]: they are
     never read on the host, so what a router counted needs no synchronisation.  A group may have no rows; rows of no group (before
-    offsets[0], from offsets[G] on) give zeros and zero gradients.  First-order gradients; capture as for ``layer_norm``.  -> (N, out)"""
+    offsets[0], from offsets[G] on) give zeros and zero gradients.  First-order gradients in reverse mode; capture as for ``layer_norm``.  -> (N, out)"""
     return get_backend().host.grouped_linear(x, weight, offsets, bias)
 
 
