@@ -335,3 +335,27 @@ def test_a_captured_backward_beside_an_eager_graph_is_refused_through_nodes_in_b
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_adamw_counts_the_steps_that_it_took(hip_backend):
+    """Parameters of two types, one call each; the second is refused: the first has taken its step, and says so."""
+    from virconv_amd.optim import AdamW
+    a, b = torch.nn.Parameter(rnd((64,), 1)), torch.nn.Parameter(rnd((64,), 2, BF16))
+    twin = torch.nn.Parameter(a.detach().clone())
+    opt, alone = AdamW([a, b], **HYPER), AdamW([twin], **HYPER)
+    for t in range(4):
+        a.grad, b.grad = rnd((64,), 10 + t), rnd((64,), 20 + t, BF16)
+        twin.grad = a.grad
+        alone.step()
+        if t == 2:
+            kept = opt.state[b]["exp_avg"]
+            opt.state[b]["exp_avg"] = opt.state[b]["exp_avg_sq"]
+            before = b.detach().clone()
+            with pytest.raises(RuntimeError, match="overlap"):
+                opt.step()
+            opt.state[b]["exp_avg"] = kept
+            assert torch.equal(b, before) and opt.state[b]["step"] == 2
+        else:
+            opt.step()
+        assert torch.equal(a, twin) and opt.state[a]["step"] == t + 1
+    assert opt.state[b]["step"] == 3

@@ -359,8 +359,8 @@ int64_t adamw(const py::list& params, const py::list& states, int64_t first_plac
   if ((size_t)PyList_GET_SIZE(states.ptr()) != n) return -1;
   const at::ScalarType moment = state_bits == 8 ? at::kFloat8_e4m3fn : at::kFloat;
   std::vector<vc_adamw_tensor> table[3];     // by vc_dtype
-  std::vector<PyObject*> live;
-  struct Results { c10::TensorImpl* t[4]; };     // what a tensor's step writes
+  bool any = false;
+  struct Results { c10::TensorImpl* t[4]; PyObject* state; };     // what a tensor's step writes
   std::vector<Results> results[3];
   int64_t step = 0;
   Tensor first;
@@ -383,12 +383,12 @@ int64_t adamw(const py::list& params, const py::list& states, int64_t first_plac
     PyObject *so = PyDict_GetItem(st, kStep), *mo = PyDict_GetItem(st, kAvg), *vo = PyDict_GetItem(st, state_bits == 8 ? kRms : kSq);
     if (!so || !PyLong_CheckExact(so) || !mo || !vo || !THPVariable_Check(mo) || !THPVariable_Check(vo)) return -1;
     const int64_t s = PyLong_AsLongLong(so);
-    if (live.empty()) step = s;
+    if (!any) step = s;
     if (s != step || s < 0) return -1;
     const Tensor &m = THPVariable_Unpack(mo), &v = THPVariable_Unpack(vo);
     if (!plain(m, p, moment) || !plain(v, p, moment)) return -1;
     vc_adamw_tensor t = {p.data_ptr(), g.data_ptr(), m.data_ptr(), v.data_ptr(), nullptr, p.numel(), (uint32_t)(first_place + k), 0};
-    Results r = {{p.unsafeGetTensorImpl(), m.unsafeGetTensorImpl(), v.unsafeGetTensorImpl(), nullptr}};
+    Results r = {{p.unsafeGetTensorImpl(), m.unsafeGetTensorImpl(), v.unsafeGetTensorImpl(), nullptr}, st};
     if (state_bits == 8) {
       PyObject* eo = PyDict_GetItem(st, kExponents);
       if (!eo || !THPVariable_Check(eo)) return -1;
@@ -404,24 +404,22 @@ int64_t adamw(const py::list& params, const py::list& states, int64_t first_plac
     }
     table[dt].push_back(t);
     results[dt].push_back(r);
-    live.push_back(st);
+    any = true;
   }
-  if (live.empty()) return 0;
-  {
-    const c10::DeviceGuard guard(first.device());
-    if (capturing((hipStream_t)stream_of(first))) throw VirConvError(kCaptured);
-    for (int dt = 0; dt < 3; ++dt) {
-      if (table[dt].empty()) continue;
-      check(abi.adamw(table[dt].data(), (int64_t)table[dt].size(), dt, state_bits, lr, b1, b2, eps, weight_decay, step + 1, (uint32_t)seed,
-                      stream_of(first)),
-            "vc_adamw");
-      for (const Results& r : results[dt])
-        for (c10::TensorImpl* t : r.t) written(t);
+  if (!any) return 0;
+  const py::object now = py::reinterpret_steal<py::object>(PyLong_FromLongLong(step + 1));
+  const c10::DeviceGuard guard(first.device());
+  if (capturing((hipStream_t)stream_of(first))) throw VirConvError(kCaptured);
+  for (int dt = 0; dt < 3; ++dt) {
+    if (table[dt].empty()) continue;
+    check(abi.adamw(table[dt].data(), (int64_t)table[dt].size(), dt, state_bits, lr, b1, b2, eps, weight_decay, step + 1, (uint32_t)seed,
+                    stream_of(first)),
+          "vc_adamw");
+    for (const Results& r : results[dt]) {     // (what the next type's call refuses does not take this step back)
+      for (c10::TensorImpl* t : r.t) written(t);
+      PyDict_SetItem(r.state, kStep, now.ptr());
     }
   }
-  PyObject* now = PyLong_FromLongLong(step + 1);
-  for (PyObject* st : live) PyDict_SetItem(st, kStep, now);
-  Py_DECREF(now);
   return step + 1;
 }
 
