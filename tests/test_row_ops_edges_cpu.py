@@ -192,3 +192,21 @@ def test_forward_mode_derivatives_are_refused(hip, which):
             ops.grouped_linear(grouped[0], grouped[1], offsets, grouped[2])
     with pytest.raises(_lib.VirConvError, match="no CPU path"):
         ops.layer_norm(torch.randn(4, 8))
+
+
+# ---------------------------------------------------------------------------------------------------------------- AdamW's states
+def test_a_state_handed_to_another_parameter_is_followed(AdamW):
+    a, b, c = (torch.nn.Parameter(torch.zeros(4)) for _ in range(3))
+    opt = AdamW([a, b, c])
+    group = opt.param_groups[0]["params"]
+    one, two = opt._new_state(a), opt._new_state(c)
+    same = lambda *want: all(x is y for x, y in zip(opt._states_of(0, group), want))     # noqa: E731
+    assert same(one, None, two) and same(one, None, two)
+    opt.state[b] = opt.state.pop(c)                    # the same dicts in the same order, one of them for another parameter
+    assert same(one, two, None)
+    opt.state[a], opt.state[b] = opt.state[b], opt.state[a]
+    assert same(two, one, None)
+    group[0], group[1] = b, a
+    assert same(one, two, None)
+    del opt.state[a]
+    assert same(one, None, None)

@@ -423,14 +423,14 @@ int64_t adamw(const py::list& params, const py::list& states, int64_t first_plac
   return step + 1;
 }
 
-// are the values of `dict`, in order, the objects of `list`?
-bool same_values(const py::dict& dict, const py::list& list) {
+// are the keys and values of `dict`, in order, the objects of `list`, a key and its value in turn?
+bool same_items(const py::dict& dict, const py::list& list) {
   const Py_ssize_t n = PyList_GET_SIZE(list.ptr());
-  if (PyDict_Size(dict.ptr()) != n) return false;
+  if (2 * PyDict_Size(dict.ptr()) != n) return false;
   Py_ssize_t at = 0, k = 0;
   PyObject *key, *value;
-  while (PyDict_Next(dict.ptr(), &at, &key, &value))
-    if (k >= n || PyList_GET_ITEM(list.ptr(), k++) != value) return false;
+  for (; PyDict_Next(dict.ptr(), &at, &key, &value); k += 2)
+    if (k + 2 > n || PyList_GET_ITEM(list.ptr(), k) != key || PyList_GET_ITEM(list.ptr(), k + 1) != value) return false;
   return true;
 }
 
@@ -459,6 +459,6 @@ PYBIND11_MODULE(_host_ops, m) {
   m.def("grouped_linear", &grouped_linear, py::call_guard<py::gil_scoped_release>());
   m.def("adamw", &adamw);
   m.attr("ADAMW_CAPTURED") = kCaptured;
-  m.def("same_values", &same_values);
+  m.def("same_items", &same_items);
   m.def("same_objects", &same_objects);
 }

@@ -299,9 +299,9 @@ class AdamW(torch.optim.Optimizer):
 
     def _states_of(self, k, ps):
         """The state dicts of group k's parameters, in order, None for one that has none.  The list is kept as long as self.state holds the same
-        dicts and the group the same parameters."""
-        if not self._host.same_values(self.state, self._order):
-            self._order, self._lists = list(self.state.values()), {}
+        dicts for the same parameters and the group the same parameters."""
+        if not self._host.same_items(self.state, self._order):
+            self._order, self._lists = [x for item in self.state.items() for x in item], {}
         known = self._lists.get(k)
         if known is None or not self._host.same_objects(ps, known[0]):
             known = self._lists[k] = (list(ps), [self.state[p] if p in self.state else None for p in ps])
