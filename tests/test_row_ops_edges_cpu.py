@@ -210,3 +210,9 @@ def test_a_state_handed_to_another_parameter_is_followed(AdamW):
     assert same(one, two, None)
     del opt.state[a]
     assert same(one, None, None)
+
+
+def test_a_first_group_without_parameters(hip):
+    from virconv_amd.optim import AdamW
+    with pytest.raises(ValueError, match="no CPU path"):       # (of the second group's parameter)
+        AdamW([{"params": []}, {"params": [torch.nn.Parameter(torch.zeros(4))]}])

@@ -359,3 +359,14 @@ def test_adamw_counts_the_steps_that_it_took(hip_backend):
             opt.step()
         assert torch.equal(a, twin) and opt.state[a]["step"] == t + 1
     assert opt.state[b]["step"] == 3
+
+
+def test_adamw_with_a_group_without_parameters(hip_backend):
+    from virconv_amd.optim import AdamW
+    p, q = torch.nn.Parameter(rnd((64,), 1)), torch.nn.Parameter(rnd((64,), 1))
+    one, two = AdamW([{"params": []}, {"params": [p], "lr": 1e-2}], **HYPER), AdamW([q], **{**HYPER, "lr": 1e-2})
+    for t in range(2):
+        p.grad = q.grad = rnd((64,), 2 + t)
+        one.step()
+        two.step()
+        assert torch.equal(p, q)

@@ -193,7 +193,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: betas {g['betas']} outside [0, 1)")
         if not (g["lr"] >= 0.0 and g["eps"] >= 0.0 and g["weight_decay"] >= 0.0):
             raise ValueError(f"AdamW: lr {g['lr']}, eps {g['eps']}, weight_decay {g['weight_decay']} have to be 0 or more")
-        device = self.param_groups[0]["params"][0].device
+        device = next((p.device for group in self.param_groups for p in group["params"]), None)
         for p in g["params"]:
             if not p.is_cuda or p.device != device:
                 raise ValueError(f"AdamW: parameters have to be on one GPU, got {p.device} beside {device} (there is no CPU path)")
