@@ -151,6 +151,34 @@ def test_a_moment_whose_blocks_are_not_known_is_refused(AdamW):
         AdamW([p], state_bits=8).load_state_dict(saved)
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_checkpoints_of_steps_that_are_not_done_here_are_refused(AdamW, bits):
+    p = torch.nn.Parameter(torch.randn(16, 24))
+    p.grad = torch.randn(16, 24)
+    before = p.detach().clone()
+
+    def saved(kind, **options):
+        q = torch.nn.Parameter(p.detach().clone())
+        q.grad = p.grad.clone()
+        opt = kind([q], lr=1e-3, weight_decay=0.01, **options)
+        opt.step()
+        return opt.state_dict()
+
+    ours = AdamW([p], lr=2e-3, state_bits=bits)
+    for state, word in ((saved(torch.optim.AdamW, maximize=True), "maximize"), (saved(torch.optim.AdamW, amsgrad=True), "amsgrad"),
+                        (saved(torch.optim.Adam), "adds its weight decay")):
+        with pytest.raises(ValueError, match=word):
+            ours.load_state_dict(state)
+        assert ours.param_groups[0]["lr"] == 2e-3 and p not in ours.state and torch.equal(p, before)       # nothing of it was taken
+    if bits == 32:
+        ours.load_state_dict(saved(torch.optim.AdamW))
+        assert ours.state[p]["step"] == 1 and ours.param_groups[0]["lr"] == 1e-3
+        with pytest.raises(ValueError, match="state_bits"):
+            other = AdamW([p], state_bits=8)
+            moments(other, p, 1)
+            AdamW([p]).load_state_dict(other.state_dict())
+
+
 # ---------------------------------------------------------------------------------------------------------------- the native host side
 @pytest.mark.parametrize("what", ["missing", "of another layout", "of another torch", "no extension"])
 def test_what_does_not_use_the_native_host_side_does_without_it(what, monkeypatch, tmp_path):

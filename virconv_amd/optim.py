@@ -228,6 +228,13 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: state 'exponents' is {e.dtype} {tuple(e.shape)} on {e.device}")
 
     def load_state_dict(self, state_dict):
+        for g in state_dict["param_groups"]:
+            # what another optimizer's checkpoint may ask of a step, which this one does not do
+            for option in ("amsgrad", "maximize"):
+                if g.get(option):
+                    raise ValueError(f"AdamW: a state saved with {option}=True: there is no such step here")
+            if not g.get("decoupled_weight_decay", True) and g.get("weight_decay"):
+                raise ValueError("AdamW: a state saved by an optimizer that adds its weight decay to the gradient")
         # torch casts every floating-point state to the parameter's type: the moments keep their own here
         super().load_state_dict(state_dict)
         saved = state_dict["state"]
@@ -252,7 +259,8 @@ class AdamW(torch.optim.Optimizer):
                         self._encode(p, st, column, k, _decode(v.to(p.device), saved[i]["exponents"].to(p.device)[:, column]))
             if self.state_bits == 32 and "exp_avg" in st:
                 for k in ("exp_avg", "exp_avg_sq"):
-                    st[k] = st[k].float()
+                    if k in st:
+                        st[k] = st[k].float()
             st["step"] = int(saved[i]["step"])
             self._check_state(p, st)
 
