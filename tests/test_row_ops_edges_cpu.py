@@ -244,3 +244,25 @@ def test_a_first_group_without_parameters(hip):
     from virconv_amd.optim import AdamW
     with pytest.raises(ValueError, match="no CPU path"):       # (of the second group's parameter)
         AdamW([{"params": []}, {"params": [torch.nn.Parameter(torch.zeros(4))]}])
+
+
+def test_capture_is_looked_for_on_the_device_of_the_parameters(AdamW, monkeypatch):
+    """The first step, parameters of other memory orders: the path in Python.  (The current stream is one of the current device.)"""
+    inside = []
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            inside.append(self.device)
+
+        def __exit__(self, *error):
+            inside.pop()
+
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.ones(4)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: inside == [p.device])
+    with pytest.raises(RuntimeError, match="captured"):
+        AdamW([p]).step()

@@ -152,7 +152,7 @@ class AdamW(torch.optim.Optimizer):
 
     Parameters: fp32, fp16 or bf16 tensors on one GPU, dense in any order of their axes; gradients of the same type.  The step computes in
     fp32 and rounds a parameter once.  ``state_bits=32``: the moments are fp32, with the keys and shapes of torch.optim.AdamW's state (a
-    checkpoint of either loads into the other).  ``state_bits=8``: 2 bytes an element instead of 8 -- ``exp_avg`` and ``exp_avg_rms`` (the
+    checkpoint of either loads into the other, unless it asks for amsgrad or maximize).  ``state_bits=8``: 2 bytes an element instead of 8 -- ``exp_avg`` and ``exp_avg_rms`` (the
     square root of the second moment) are float8_e4m3fn values over a power of two for every 128 elements (``exponents``, int8), rounded up or
     down at random in proportion so that a moment follows changes smaller than its resolution.  The second moment gains the rounding's variance
     by it: under steady gradients it settles about 4 per cent (3 to 6) above its 32-bit value, so steps are 1 to 2 per cent shorter.  The
@@ -318,9 +318,10 @@ class AdamW(torch.optim.Optimizer):
     def _step_tensors(self, g, ps, grads, places):
         if not ps:
             return
-        if torch.cuda.is_current_stream_capturing():
-            raise RuntimeError(self._host.ADAMW_CAPTURED)
         first = ps[0]
+        with torch.cuda.device(first.device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(self._host.ADAMW_CAPTURED)
         index = first.get_device()
         state = self.state
         states = [state[p] if p in state else self._new_state(p) for p in ps]
