@@ -295,6 +295,27 @@ def test_adamw_8_bit_second_moment_settles_where_it_is_said_to(hip_backend):
     assert 0.484 / 16 * 0.9 - 0.002 < excess < 0.484 / 8 * 1.1 + 0.002, excess
 
 
+def test_one_row_with_any_stride_through_the_c_interface(hip_backend):
+    """A single row's stride means nothing, also where the row is longer than 32-bit offsets into the weights allow."""
+    from virconv_amd import _lib
+    lib = _lib.load()
+    inner, outer = (1 << 24) - 8, 136
+    x = torch.zeros(1, inner, device="cuda")
+    w = torch.zeros(1, outer, inner, device="cuda")
+    x[0, -3:] = torch.tensor([1.0, 2.0, 3.0])
+    w[0, :, -3:] = rnd((outer, 3), 1)
+    offsets = torch.tensor([0, 1], device="cuda")
+    size = lib.vc_grouped_linear_workspace_bytes(0, 1, 1, inner, outer, 0)
+    ws = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+    want = (w[0, :, -3:].double() @ x[0, -3:].double()).cpu()
+    for stride in (inner, 8, 0):
+        y = torch.full((1, outer), math.nan, device="cuda")
+        _lib.check(lib.vc_grouped_linear_forward(x.data_ptr(), stride, 1, w.data_ptr(), None, offsets.data_ptr(), 64, 1, inner, outer, 0, y.data_ptr(),
+                                                 ws.data_ptr(), size, torch.cuda.current_stream().cuda_stream), "forward")
+        torch.cuda.synchronize()
+        assert bool(((y[0].double().cpu() - want).abs() <= 8 * U * (w[0, :, -3:].abs().double().cpu() @ x[0, -3:].double().cpu())).all()), stride
+
+
 # ---------------------------------------------------------------------------------------------------------------- graphs, refusals
 @pytest.mark.parametrize("what", ["rows of three axes", "a transposed weight", "a layer in between"])
 def test_a_captured_backward_beside_an_eager_graph_is_refused_through_nodes_in_between(hip_backend, what):

@@ -1262,7 +1262,7 @@ int vc_grouped_linear_forward(const void* x, int64_t x_stride, int64_t rows, con
   VC_REQUIRE(x && y && (weight || groups == 0), "vc_grouped_linear_forward: NULL pointer");
   VC_REQUIRE(x_stride >= in || rows == 1, "vc_grouped_linear_forward: row stride %lld below %lld channels", (long long)x_stride, (long long)in);
   GroupArgs a{};
-  a.a = x; a.lda = x_stride; a.b = weight; a.bias = bias; a.offsets = offsets; a.off64 = offset_bits == 64; a.out = y;
+  a.a = x; a.lda = rows == 1 ? in : x_stride; a.b = weight; a.bias = bias; a.offsets = offsets; a.off64 = offset_bits == 64; a.out = y;
   a.rows = rows; a.groups = (int)groups; a.n = (int)out; a.k = (int)in;
   return launch_rows("vc_grouped_linear_forward", a, kForward, dtype, plan_rows(rows, groups, out, in, dtype), workspace, workspace_bytes, (hipStream_t)stream);
 }
@@ -1276,7 +1276,7 @@ int vc_grouped_linear_backward_input(const void* dy, int64_t dy_stride, int64_t 
   VC_REQUIRE(dy && dx && (weight || groups == 0), "vc_grouped_linear_backward_input: NULL pointer");
   VC_REQUIRE(dy_stride >= out || rows == 1, "vc_grouped_linear_backward_input: row stride %lld below %lld channels", (long long)dy_stride, (long long)out);
   GroupArgs a{};
-  a.a = dy; a.lda = dy_stride; a.b = weight; a.offsets = offsets; a.off64 = offset_bits == 64; a.out = dx;
+  a.a = dy; a.lda = rows == 1 ? out : dy_stride; a.b = weight; a.offsets = offsets; a.off64 = offset_bits == 64; a.out = dx;
   a.rows = rows; a.groups = (int)groups; a.n = (int)in; a.k = (int)out;
   return launch_rows("vc_grouped_linear_backward_input", a, kBackInput, dtype, plan_rows(rows, groups, in, out, dtype), workspace, workspace_bytes, (hipStream_t)stream);
 }
@@ -1291,6 +1291,7 @@ int vc_grouped_linear_backward_weight(const void* x, int64_t x_stride, const voi
   VC_REQUIRE(dweight && (rows == 0 || (x && dy)), "%s: NULL pointer", who);
   VC_REQUIRE((x_stride >= in && dy_stride >= out) || rows <= 1, "%s: row strides %lld, %lld below %lld, %lld channels", who, (long long)x_stride,
              (long long)dy_stride, (long long)in, (long long)out);
+  if (rows <= 1) { x_stride = in; dy_stride = out; }     // (a single row's stride may be anything; it decides on tiles and offsets all the same)
   const GroupPlan p = plan_weight(rows, groups, out, in, dtype);
   const size_t need = (size_t)p.partial_floats * sizeof(float);
   VC_REQUIRE(need == 0 || (workspace && workspace_bytes >= need), "%s: workspace of %zu bytes, need %zu", who, workspace_bytes, need);
