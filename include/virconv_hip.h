@@ -285,7 +285,8 @@ typedef enum vc_dtype { VC_F32 = 0, VC_F16 = 1, VC_BF16 = 2 } vc_dtype;
 
 /* Layer norm of n rows of c elements: y = (x - mean) * rstd * weight + bias, rstd = 1 / sqrt(var + eps), var the mean square of x - mean.
  * x: row r at x + r * x_stride (elements, >= c), y: (n, c) dense.  weight / bias: c elements of weight_dtype / bias_dtype (the tensors'
- * type or VC_F32), or NULL (1 / 0).  mean, rstd: n floats each for the backward pass, or both NULL.                                        */
+ * type or VC_F32), or NULL (1 / 0).  mean, rstd: n floats each for the backward pass, or both NULL.  Refused: 2^31 rows, 2^30 channels (2^27 with
+ * the weights' gradients), 2^22 rows of more than 16384 channels.                                                                          */
 int vc_layer_norm_forward(const void* x, int64_t x_stride, int64_t n, int64_t c, int dtype, const void* weight, int weight_dtype,
                           const void* bias, int bias_dtype, float eps, void* y, float* mean, float* rstd, void* stream);
 /* dx = rstd * (g - mean(g) - xh * mean(g * xh)) with g = dy * weight, xh = (x - mean) * rstd; dweight = sum over the rows of dy * xh, dbias

@@ -266,3 +266,18 @@ def test_capture_is_looked_for_on_the_device_of_the_parameters(AdamW, monkeypatc
     monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: inside == [p.device])
     with pytest.raises(RuntimeError, match="captured"):
         AdamW([p]).step()
+
+
+# ---------------------------------------------------------------------------------------------------------------- sizes
+def test_layer_norm_refuses_what_one_launch_cannot_hold():
+    fake = ctypes.c_void_p(4096)    # never dereferenced on the host
+    f, b = _lib.load().vc_layer_norm_forward, _lib.load().vc_layer_norm_backward
+
+    def refused(status):
+        return status == _lib.VC_EINVAL and b"too many for one launch" in _lib.load().vc_last_error()
+
+    for c, dtype in ((16385, 0), (16385, 2), (1 << 20, 1)):
+        assert refused(f(fake, c, 1 << 22, c, dtype, None, 0, None, 0, 1e-5, fake, None, None, None))
+        assert refused(b(fake, c, fake, c, 1 << 22, c, dtype, None, 0, 0, fake, fake, fake, None, None, None, 0, None))
+    for dw, db in ((fake, None), (None, fake)):
+        assert refused(b(fake, 1 << 27, fake, 1 << 27, 1, 1 << 27, 0, None, 0, 0, fake, fake, None, dw, db, fake, 1 << 40, None))

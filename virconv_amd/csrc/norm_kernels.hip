@@ -452,6 +452,9 @@ static void norm_backward_launch(const NormBackArgs& a, const NormShape& s, int6
 #undef VC_DO
 }
 
+// a launch has fewer than 2^32 threads: 1024 for a row beyond a block's registers, 256 for 16 of the two gradients' columns
+static bool launches(int64_t n, int64_t c, const NormShape& s, bool sums) { return (s.iter || n < (1LL << 22)) && (!sums || c < (1LL << 27)); }
+
 static bool known_dtype(int t) { return t == VC_F32 || t == VC_F16 || t == VC_BF16; }
 
 }  // namespace vc
@@ -470,6 +473,7 @@ int vc_layer_norm_forward(const void* x, int64_t x_stride, int64_t n, int64_t c,
   VC_REQUIRE(x && y, "vc_layer_norm_forward: NULL pointer");
   NormArgs a{x, weight, bias, y, mean, rstd, n, x_stride, (int)c, weight_dtype, bias_dtype, eps};
   const NormShape s = norm_shape(c, dtype);
+  VC_REQUIRE(launches(n, c, s, false), "vc_layer_norm_forward: %lld rows of %lld: too many for one launch", (long long)n, (long long)c);
   hipStream_t st = (hipStream_t)stream;
   if (dtype == VC_F32) norm_forward_launch<float>(a, s, st);
   else if (dtype == VC_F16) norm_forward_launch<_Float16>(a, s, st);
@@ -492,6 +496,7 @@ int vc_layer_norm_backward(const void* x, int64_t x_stride, const void* dy, int6
   hipStream_t st = (hipStream_t)stream;
   const bool sums = dweight || dbias;
   const NormShape s = norm_shape(c, dtype);
+  VC_REQUIRE(launches(dx ? n : 0, c, s, sums), "vc_layer_norm_backward: %lld rows of %lld: too many for one launch", (long long)n, (long long)c);
   const int64_t blocks = norm_blocks(n, c, s);
   if (n > 0) {
     VC_REQUIRE(x && dy && mean && rstd, "vc_layer_norm_backward: NULL pointer");
