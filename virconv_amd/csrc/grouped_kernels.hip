@@ -734,7 +734,7 @@ __global__ void __launch_bounds__(256, 2) grouped_kernel(GroupArgs a) {
 // one that multiplies them: four waves of each kind, two halves of LDS, one barrier a step.  The block takes tiles until there are none, and
 // the first kind is already at the next tile while the second writes its results.
 //
-// Measured: 4096^3 forward 205, backward input 205, weight 200 TFLOP/s (1230 of bf16 products; the clock falls with them: 170 to 208 by card); 480 x
+// Measured: 4096^3 forward 223, backward input 219, weight 199 TFLOP/s (1340 of bf16 products; the clock falls with them: 170 to 223 by card); 480 x
 // 27648 to 256 columns in 3 ragged groups 64, 75 and 67 us, 106 MB and 41 GFLOP of bf16 products each: tiles of rows that are not there and the
 // unequal groups leave the compute units without work for 40 per cent of that time.
 template <int BM, int BN, int MODE>
@@ -871,7 +871,7 @@ __global__ void __launch_bounds__(512, 2) grouped_f32_kernel(GroupArgs a) {
 // step.  Within a step each fragment is read while the products of the one before it run.  What is left of the summed axis behind the last whole
 // step goes through registers, with zeros behind its end.
 //
-// Measured, bf16: 8192^3 forward 1340, backward input 1350, weight 1185 TFLOP/s (a library product 1313; both operands of the weight product come
+// Measured, bf16: 8192^3 forward 1340 to 1385, backward input 1350 to 1380, weight 1140 to 1200 TFLOP/s by card (a library product 1313; both operands of the weight product come
 // by ds_read_b64_tr_b16, twice the instructions); 32749 x 1024 -> 4096 in 16 ragged groups 960, 910, 970.  A tile's way in and out costs about as
 // much as 400 summed indices, so short sums stay below the rate; steps of 32 in a ring of five buffers were 9 per cent slower.
 constexpr int kLargeNarrow = 192, kLargeBuffer = (256 + 256) * 64 * 2;
@@ -1149,7 +1149,8 @@ static GroupPlan plan_rows(int64_t rows, int64_t groups, int64_t n, int64_t k, i
 // may hold nearly all rows, fewer than 512 each; a piece is long enough that the sums written for it (and read once more) stay small beside the
 // rows that it reads.  (bf16, groups of which the largest has four times the rows of the smallest: 65536 rows of 512 and 512 channels in 32 groups,
 // 512 tiles, 178 us in pieces and 75 whole; 16384 rows in 8 groups, 128 tiles, 66 and 51; 8192 rows of 1024 and 1024 in 2 groups, 128 tiles, 75
-// and 92.  128 x 128 tiles from 65 channels a side on, 64 x 64 below.)
+// and 92.  128 x 128 tiles from 65 channels a side on, 64 x 64 below.)  From four groups on a group that holds nearly all rows has its own tiles' blocks
+// only: bf16, 32768 rows of 512 and 512 channels in 8 groups, 61 us with equal groups, 437 with all rows in one; 32749 of 1024 and 4096 in 16, 276 and 854.
 static GroupPlan plan_weight(int64_t rows, int64_t groups, int64_t m, int64_t n, int dtype) {
   GroupPlan p;
   p.two_kinds = dtype == VC_F32 && m > 64 && n > 64;
