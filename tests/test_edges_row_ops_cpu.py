@@ -179,6 +179,16 @@ def test_checkpoints_of_steps_that_are_not_done_here_are_refused(AdamW, bits):
             AdamW([p]).load_state_dict(other.state_dict())
 
 
+def test_8_bit_states_that_lack_a_moment_are_refused(AdamW):
+    p = torch.nn.Parameter(torch.randn(16, 24))
+    opt = AdamW([p], state_bits=8)
+    moments(opt, p, 5)
+    saved = opt.state_dict()
+    del saved["state"][0]["exp_avg_rms"]
+    with pytest.raises(ValueError, match="without 'exp_avg_rms'"):
+        AdamW([p], state_bits=8).load_state_dict(saved)
+
+
 # ---------------------------------------------------------------------------------------------------------------- the native host side
 @pytest.mark.parametrize("what", ["missing", "of another layout", "of another torch", "no extension"])
 def test_what_does_not_use_the_native_host_side_does_without_it(what, monkeypatch, tmp_path):

@@ -251,8 +251,8 @@ class AdamW(torch.optim.Optimizer):
                     st[k] = t.copy_(v)
             if self.state_bits == 8 and "exponents" in st:
                 for column, k in enumerate(("exp_avg", "exp_avg_rms")):
-                    v = saved[i][k]
-                    if v.dtype == st[k].dtype and v.shape == p.shape and _order(v) != _order(p):
+                    v = saved[i].get(k)
+                    if v is not None and v.dtype == st[k].dtype and v.shape == p.shape and _order(v) != _order(p):
                         # its elements lie in another order in memory than p's, so other ones share an exponent now
                         if not _dense(v):
                             raise ValueError(f"AdamW: state {k!r} of strides {v.stride()} is not dense: which of its elements share an exponent is not known")
